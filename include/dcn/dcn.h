@@ -696,6 +696,162 @@ dcn_status dcn_clip_run_with_fallback_dev(dcn_clip* clip, const void* d_spatial,
                                           const void* d_forward_flows, void* d_propagated, void* stream,
                                           dcn_report_fn report, void* report_user, int* recovered_with);
 
+/* ---- frame attention ------------------------------------------------------------------
+ * The operators of a block in which the tokens of a clip's frames attend to the frames
+ * before them: rotary positions with three axes, the paged key/value cache, attention over
+ * a window of frames with the first frames kept visible, and the gated norms around the
+ * block. No counterpart in the reference. The calls are asynchronous on the stream given
+ * and allocate nothing: what scratch they need is the caller's workspace (two calls that
+ * may run at the same time need two), so all of them can be captured into a hipGraph.
+ *
+ * A tensor of heads is [tokens][heads][head_dim]: element strides between tokens and
+ * between heads are given, channels are adjacent, so a slice of a packed projection is
+ * taken as it is. Pointers are aligned to their element type; 16-byte alignment and strides
+ * of 16 bytes are faster. */
+typedef enum dcn_dtype { DCN_DTYPE_F16 = 0, DCN_DTYPE_BF16 = 1, DCN_DTYPE_F32 = 2 } dcn_dtype;
+#define DCN_ATTENTION_MAX_HEAD_DIM 256
+
+/* Which pairs of a head's channels turn with which axis: pairs[0] with the time, then
+ * pairs[1] with the height, pairs[2] with the width; 2 * sum <= head_dim, channels past
+ * the pairs pass unchanged. Pair i is channels (2i, 2i + 1) if interleaved, else
+ * (i, i + sum). Its angle is position[axis] * freq[i], in radians: the product is taken and
+ * reduced in FP64, so large positions lose nothing. */
+typedef struct dcn_rotary {
+    int32_t dtype; /* dcn_dtype of the tensors */
+    int32_t head_dim;
+    int32_t pairs[3];
+    int32_t interleaved;
+} dcn_rotary;
+/* out = the rotation of x by its positions ([tokens][3]: time, height, width; any int32),
+ * (a, b) -> (a cos - b sin, a sin + b cos); inverse turns the other way, which is the
+ * gradient. freq holds sum(pairs) FP32 values. out may be x (with x's strides); it must not
+ * overlap x otherwise. */
+dcn_status dcn_rotary_dev(dcn_context* ctx, const dcn_rotary* rotary, int64_t tokens, int heads, const void* d_x,
+                          int64_t x_token_stride, int64_t x_head_stride, const int32_t* d_positions,
+                          const float* d_freq, int inverse, void* d_out, int64_t out_token_stride,
+                          int64_t out_head_stride, void* stream);
+
+/* The paged cache: k_pages and v_pages are [pages][page_tokens][kv_heads][head_dim], 16-byte
+ * aligned or not; sequence s keeps its token p in row p % page_tokens of page
+ * table[s][p / page_tokens] (table is [sequences][table_width]). page_tokens is a power of
+ * two. An entry outside [0, pages) is a page that the sequence does not have (any more). */
+typedef struct dcn_cache {
+    int32_t pages;
+    int32_t page_tokens;
+    int32_t table_width;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t dtype; /* dcn_dtype */
+} dcn_cache;
+/* Writes the new tokens' keys (rotated if rotary is not null) and values into the cache,
+ * and, if q is not null, the rotated queries to q_out, in one launch. The new tokens of
+ * sequence s are rows cu_q[s] .. cu_q[s + 1] of q, k, v and positions, the last of the
+ * kv_lens[s] tokens that it has with them. Rows of no sequence, tokens past the table's
+ * width and tokens whose page is not in the pool are not written. */
+typedef struct dcn_append_shape {
+    int32_t sequences;
+    int32_t q_heads; /* ignored when q is null */
+    int64_t tokens;  /* rows of q, k, v and positions */
+    int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2]; /* token, head */
+} dcn_append_shape;
+dcn_status dcn_cache_append_dev(dcn_context* ctx, const dcn_cache* cache, const dcn_append_shape* shape,
+                                const dcn_rotary* rotary, const void* d_q, const void* d_k, const void* d_v,
+                                const int32_t* d_positions, const float* d_freq, const int32_t* d_cu_q,
+                                const int32_t* d_kv_lens, const int32_t* d_table, void* d_q_out, void* d_k_pages,
+                                void* d_v_pages, void* stream);
+
+/* Attention with a window in frames. Query i of a sequence with nq queries and nk keys is
+ * its token p = nk - nq + i, of frame f = p / frame_tokens, and sees key j of frame fj when
+ * fj <= f + ahead (ahead < 0: any) and either fj >= f - back (back < 0: any) or fj < sinks.
+ * frame_tokens = 1 counts in tokens. out = softmax(scale q k^T over the visible keys) v,
+ * lse = the logarithm of the sum of exponentials; a query that sees no key (p < 0 too) has
+ * out 0 and lse -inf. What a query does not see does not reach its results, NaN and
+ * infinities included. Query head h reads key head h / (q_heads / kv_heads).
+ * Softmax statistics and sums are FP32. Sequence s holds rows cu_q[s] .. cu_q[s + 1] of the
+ * queries and cu_kv[s] .. cu_kv[s + 1] of the keys; null: rows s * max_q .. of max_q each
+ * (keys: max_kv). max_q and max_kv are at least the longest sequence's lengths: they size
+ * the launch. Rows of no sequence are not written. */
+typedef struct dcn_attention_shape {
+    int32_t dtype; /* dcn_dtype */
+    int32_t sequences;
+    int32_t q_heads;
+    int32_t kv_heads;
+    int32_t head_dim; /* 1 .. DCN_ATTENTION_MAX_HEAD_DIM; 64 and 128 in 16 bits run on the matrix cores */
+    int32_t frame_tokens;
+    int32_t back;
+    int32_t ahead;
+    int32_t sinks;
+    int32_t max_q;
+    int32_t max_kv;
+    float scale;
+    int64_t q_tokens;  /* rows of q, out, lse */
+    int64_t kv_tokens; /* rows of k, v (not used by the paged call) */
+    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* token, head */
+    int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
+} dcn_attention_shape;
+/* Bytes of workspace (16-byte aligned) that a call of this shape needs; 0: none. */
+typedef enum dcn_attention_pass {
+    DCN_ATTENTION_FORWARD = 0,
+    DCN_ATTENTION_BACKWARD = 1,
+    DCN_ATTENTION_PAGED = 2
+} dcn_attention_pass;
+size_t dcn_attention_workspace_bytes(const dcn_attention_shape* shape, dcn_attention_pass pass);
+/* lse ([q_tokens][q_heads] FP32, adjacent) may be null. */
+dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape* shape, const void* d_q,
+                                     const void* d_k, const void* d_v, const int32_t* d_cu_q,
+                                     const int32_t* d_cu_kv, void* d_out, float* d_lse, void* d_workspace,
+                                     size_t workspace_bytes, void* stream);
+/* The same over the paged cache, for one new token a sequence or many: kv_lens[s] keys,
+ * the queries being the last tokens. cu_kv's place is taken by kv_lens and the table. Keys
+ * on pages that are not in the pool are not visible. */
+dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_cache* cache,
+                                   const void* d_q, const void* d_k_pages, const void* d_v_pages,
+                                   const int32_t* d_cu_q, const int32_t* d_kv_lens, const int32_t* d_table,
+                                   void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                                   void* stream);
+/* Gradients of forward's out with respect to q, k and v, from its inputs, out, lse and
+ * dout. Sums over queries and over the heads that share a key head have a fixed order: the
+ * same inputs give the same bits. */
+dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shape* shape, const void* d_q,
+                                      const void* d_k, const void* d_v, const void* d_out, const float* d_lse,
+                                      const void* d_dout, const int32_t* d_cu_q, const int32_t* d_cu_kv, void* d_dq,
+                                      void* d_dk, void* d_dv, void* d_workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* The norms around a block's residual addition, over adjacent [tokens][channels] tensors:
+ *   n = h * r1, r1 = 1 / sqrt(mean(h^2) + eps);  x_out = x + residual_scale * gate * n * w_post
+ *   y = x_out * r2 * w_pre, r2 = 1 / sqrt(mean(x_out^2) + eps)
+ * h is a block's output, x the residual stream, y the next block's input. gate is
+ * [ceil(tokens / gate_tokens)][channels], a row for each run of gate_tokens tokens; null
+ * gates and weights are ones. y may be null (no block follows; w_pre is then ignored).
+ * rstd ([tokens][2] FP32: r1, r2) may be null where no backward follows. x_out may be x.
+ * low, where it is given, receives what rounding takes from x_out in 16 bits (with each
+ * row's r1 and r2), so that the backward has x_out in FP32 even where x is overwritten;
+ * dcn_gated_norm_low_bytes of it, 16-byte aligned (0: FP32, none is kept). */
+#define DCN_NORM_MAX_CHANNELS 8192
+typedef struct dcn_norm_shape {
+    int32_t dtype; /* dcn_dtype of every tensor but rstd, dw_post and dw_pre (FP32) */
+    int32_t channels;
+    int64_t tokens;
+    int64_t gate_tokens;
+    float residual_scale;
+    float eps;
+} dcn_norm_shape;
+dcn_status dcn_gated_norm_forward_dev(dcn_context* ctx, const dcn_norm_shape* shape, const void* d_h,
+                                      const void* d_x, const void* d_gate, const void* d_w_post, const void* d_w_pre,
+                                      void* d_x_out, void* d_y, float* d_rstd, void* d_low, void* stream);
+size_t dcn_gated_norm_low_bytes(const dcn_norm_shape* shape);
+/* Gradients from those of x_out and of y (dy null: y was not made): dh, dx, and where their
+ * pointers are given dgate, dw_post, dw_pre. Sums over tokens are FP32 in a fixed order.
+ * low may be null: x_out is then taken as it was rounded. A row of low that was left by
+ * another forward (its r1 or r2 differs from rstd's) counts as zeros. */
+size_t dcn_gated_norm_workspace_bytes(const dcn_norm_shape* shape);
+dcn_status dcn_gated_norm_backward_dev(dcn_context* ctx, const dcn_norm_shape* shape, const void* d_h,
+                                       const void* d_x_out, const void* d_gate, const void* d_w_post,
+                                       const void* d_w_pre, const float* d_rstd, const void* d_low,
+                                       const void* d_dx_out, const void* d_dy, void* d_dh, void* d_dx, void* d_dgate, float* d_dw_post,
+                                       float* d_dw_pre, void* d_workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

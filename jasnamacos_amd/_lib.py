@@ -84,6 +84,45 @@ class DcnBodyWeights(C.Structure):
     ]
 
 
+def _fields(i32=(), tail=()):
+    return [(n, C.c_int32) for n in i32] + list(tail)
+
+
+class DcnRotary(C.Structure):
+    """dcn_rotary."""
+
+    _fields_ = _fields(("dtype", "head_dim"), [("pairs", C.c_int32 * 3), ("interleaved", C.c_int32)])
+
+
+class DcnCache(C.Structure):
+    """dcn_cache."""
+
+    _fields_ = _fields(("pages", "page_tokens", "table_width", "kv_heads", "head_dim", "dtype"))
+
+
+class DcnAppendShape(C.Structure):
+    """dcn_append_shape."""
+
+    _fields_ = _fields(("sequences", "q_heads"),
+                       [("tokens", C.c_int64)] + [(n + "_stride", C.c_int64 * 2) for n in ("q", "k", "v", "q_out")])
+
+
+class DcnAttentionShape(C.Structure):
+    """dcn_attention_shape."""
+
+    _fields_ = _fields(("dtype", "sequences", "q_heads", "kv_heads", "head_dim", "frame_tokens", "back", "ahead",
+                        "sinks", "max_q", "max_kv"),
+                       [("scale", C.c_float), ("q_tokens", C.c_int64), ("kv_tokens", C.c_int64)]
+                       + [(n + "_stride", C.c_int64 * 2) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")])
+
+
+class DcnNormShape(C.Structure):
+    """dcn_norm_shape."""
+
+    _fields_ = _fields(("dtype", "channels"), [("tokens", C.c_int64), ("gate_tokens", C.c_int64),
+                                               ("residual_scale", C.c_float), ("eps", C.c_float)])
+
+
 ShapeP = C.POINTER(DcnShape)
 CtxP = c_void
 PackedP = c_void
@@ -216,6 +255,20 @@ SIGNATURES: dict[str, tuple] = {
     "dcn_clip_capture": (C.c_int, [c_void, c_void, c_void, c_void, c_void, C.c_int, C.POINTER(c_void)]),
     "dcn_clip_run_with_fallback_dev": (C.c_int, [c_void, c_void, c_void, c_void, c_void, c_void, ReportFn, c_void,
                                                  C.POINTER(C.c_int)]),
+    # frame attention
+    "dcn_rotary_dev": (C.c_int, [CtxP, C.POINTER(DcnRotary), C.c_int64, C.c_int, c_void, C.c_int64, C.c_int64, c_void,
+                                 c_void, C.c_int, c_void, C.c_int64, C.c_int64, c_void]),
+    "dcn_cache_append_dev": (C.c_int, [CtxP, C.POINTER(DcnCache), C.POINTER(DcnAppendShape), C.POINTER(DcnRotary)]
+                             + [c_void] * 12),
+    "dcn_attention_workspace_bytes": (c_size, [C.POINTER(DcnAttentionShape), C.c_int]),
+    "dcn_attention_forward_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape)] + [c_void] * 8 + [c_size, c_void]),
+    "dcn_attention_paged_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape), C.POINTER(DcnCache)] + [c_void] * 9
+                                + [c_size, c_void]),
+    "dcn_attention_backward_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape)] + [c_void] * 12 + [c_size, c_void]),
+    "dcn_gated_norm_forward_dev": (C.c_int, [CtxP, C.POINTER(DcnNormShape)] + [c_void] * 10),
+    "dcn_gated_norm_low_bytes": (c_size, [C.POINTER(DcnNormShape)]),
+    "dcn_gated_norm_workspace_bytes": (c_size, [C.POINTER(DcnNormShape)]),
+    "dcn_gated_norm_backward_dev": (C.c_int, [CtxP, C.POINTER(DcnNormShape)] + [c_void] * 15 + [c_size, c_void]),
 }
 
 _LIB: C.CDLL | None = None

@@ -1,0 +1,93 @@
+// Frame attention: kernel arguments shared by the C-ABI layer and the kernel files, and the
+// device helpers of its kernels.
+#pragma once
+
+#include <hip/hip_runtime_api.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "dcn/dcn.h"
+
+namespace dcn {
+
+// A [tokens][heads][head_dim] tensor: element strides, adjacent channels.
+struct HeadsIn {
+    const void* p;
+    int64_t ts, hs;
+};
+struct HeadsOut {
+    void* p;
+    int64_t ts, hs;
+};
+
+struct RotaryArgs {
+    int dim, st, sh, pairs, interleaved;  // pairs < st: time, < sh: height, else width
+    float sign;                           // -1: the inverse
+    const int32_t* positions;             // null: no rotation
+    const float* freq;
+};
+
+struct PagesArgs {
+    int pages, shift, width;  // tokens a page = 1 << shift; entries a table row
+    const int32_t* table;
+};
+
+struct AttentionArgs {
+    int sequences, q_heads, kv_heads, dim, group;
+    int frame, back, ahead, sinks;
+    int max_q, max_kv;
+    float scale;
+    int64_t q_tokens, kv_tokens;
+    const int32_t* cu_q;
+    const int32_t* cu_kv;   // the paged call: kv_lens
+    PagesArgs pages;        // table null: contiguous keys
+    HeadsIn q, k, v;        // paged: k and v are pages, ts between a page's tokens
+    HeadsOut out;
+    float* lse;             // may be null
+    // backward
+    HeadsIn o, dout;
+    HeadsOut dq, dk, dv;
+    const float* lse_in;
+    void* workspace;
+};
+
+hipError_t launch_rotary(int dtype, int64_t tokens, int heads, const HeadsIn& x, const HeadsOut& out,
+                         const RotaryArgs& r, hipStream_t stream);
+
+struct AppendArgs {
+    int sequences, q_heads, kv_heads;
+    int64_t tokens;
+    HeadsIn q, k, v;  // q.p null: keys and values only
+    HeadsOut q_out, k_pages, v_pages;
+    const int32_t* cu_q;
+    const int32_t* kv_lens;
+    PagesArgs pages;
+};
+hipError_t launch_append(int dtype, const AppendArgs& a, const RotaryArgs& r, hipStream_t stream);
+
+struct NormArgs {
+    int channels;
+    int64_t tokens, gate_tokens;
+    float alpha, eps;
+    const void *h, *x, *gate, *w_post, *w_pre;
+    void *x_out, *y;
+    float* rstd;
+    void* low;  // [tokens][2] FP32 (r1, r2), then [tokens][channels] of 16 bits; may be null
+    // backward
+    const void *dx_out, *dy;
+    void *dh, *dx, *dgate;
+    float *dw_post, *dw_pre;
+    float* workspace;
+};
+hipError_t launch_norm_forward(int dtype, const NormArgs& a, hipStream_t stream);
+hipError_t launch_norm_backward(int dtype, const NormArgs& a, hipStream_t stream);
+// Bytes before the rounded-off halves in `low`.
+constexpr size_t norm_low_header(int64_t tokens) { return ((size_t)tokens * 8 + 15) / 16 * 16; }
+size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
+
+// Row kernels: any head size and type (dcn_kernels_attention_rows.hip).
+hipError_t launch_attention_rows(int dtype, const AttentionArgs& a, hipStream_t stream);
+hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
+
+}  // namespace dcn

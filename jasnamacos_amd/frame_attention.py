@@ -1,0 +1,329 @@
+"""Frame attention over libdcn: the operators of a block in which the tokens of a clip's
+frames attend to the frames before them.
+
+  Rotary          rotary positions with three axes (time, height, width), and their gradient
+  CacheAppend     new keys and values into a paged cache, rotated on the way
+  FrameAttention  attention over a window of frames with the first ones kept visible:
+                  forward, backward, and over the paged cache
+  GatedNorm       the norms after and before a block, its gate and its residual scale
+
+No counterpart in the reference. Tensors are torch tensors on the context's device;
+tensors of heads are [tokens][heads][channels] with adjacent channels, so a slice of a
+packed projection is taken as it is. As elsewhere in this package outputs are the caller's,
+calls are asynchronous on `stream` (None: the default stream), and errors are
+DeformConvError. A FrameAttention or GatedNorm keeps the workspace of its calls: calls that
+may run at the same time need a handle each, and a handle sizes its workspace in its first
+call of a size (reserve it before a graph capture by running that call once)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from .deform_conv import INVALID_ARGUMENT, INVALID_SHAPE, DeformConvError, HipDeformConv, _ptr, _stream
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+PASS_FORWARD, PASS_BACKWARD, PASS_PAGED = 0, 1, 2
+
+
+def _dtype(t) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise DeformConvError(INVALID_ARGUMENT, f"dtype {t.dtype} is not float16, bfloat16 or float32")
+    return code
+
+
+def _need(condition, message: str) -> None:
+    if not condition:
+        raise DeformConvError(INVALID_SHAPE, message)
+
+
+def _heads(name: str, t, dtype, tokens, heads, dim) -> tuple:
+    """The strides of a tensor of heads, after its checks (None: any)."""
+    if t.dim() != 3 or (tokens is not None and t.shape[0] != tokens) or t.shape[1] != heads or t.shape[2] != dim:
+        raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected "
+                                             f"[{'tokens' if tokens is None else tokens}][{heads}][{dim}]")
+    if t.dtype != dtype:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
+    ts, hs, cs = t.stride()
+    if cs != 1 and dim > 1:
+        raise DeformConvError(INVALID_SHAPE, f"{name} channels are not adjacent")
+    return ts, hs
+
+
+def _whole(name: str, t, dtype, *shape) -> None:
+    """An adjacent tensor of this type and shape."""
+    if t.dtype != dtype:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}, adjacent")
+
+
+class _Handle:
+    def __init__(self, ctx: HipDeformConv):
+        self.ctx = ctx
+        self._lib = ctx._lib
+        self._workspace = None
+
+    def _room(self, count: int, like):
+        """(pointer, bytes) of a workspace of `count` bytes that the handle keeps."""
+        if not count:
+            return None, 0
+        w = self._workspace
+        if w is None or w.numel() < count:
+            if w is not None:
+                torch.cuda.synchronize(w.device)  # calls in flight still use the old one
+            self._workspace = w = torch.empty(count, dtype=torch.uint8, device=like.device)
+        return w.data_ptr(), w.numel()
+
+
+class Rotary(_Handle):
+    """Rotary positions with three axes (dcn_rotary): pairs = (time, height, width) pairs of a
+    head's channels that turn with each axis; channels past them pass."""
+
+    def __init__(self, ctx: HipDeformConv, head_dim: int, pairs, interleaved: bool = False):
+        super().__init__(ctx)
+        self.head_dim, self.pairs, self.interleaved = int(head_dim), tuple(int(p) for p in pairs), bool(interleaved)
+        _need(len(self.pairs) == 3, "rotary pairs are three numbers (time, height, width)")
+        self._c = {code: _lib.DcnRotary(code, self.head_dim, (C.c_int32 * 3)(*self.pairs), int(self.interleaved))
+                   for code in DTYPES.values()}
+
+    def frequencies(self, base: float = 10000.0, device="cuda"):
+        """A usual choice of freq: each axis from 1 down to 1 / base."""
+        parts = [base ** (-torch.arange(n, dtype=torch.float64) / max(1, n)) for n in self.pairs]
+        return torch.cat(parts).float().to(device)
+
+    def _check(self, positions, freq, tokens) -> None:
+        _whole("positions", positions, torch.int32, tokens, 3)
+        _whole("freq", freq, torch.float32, sum(self.pairs))
+
+    def run_dev(self, x, positions, freq, out, inverse: bool = False, stream=None) -> None:
+        """out = x turned by positions ([tokens][3] int32) times freq; inverse: the gradient."""
+        tokens, heads = x.shape[0], x.shape[1]
+        xs = _heads("x", x, x.dtype, tokens, heads, self.head_dim)
+        os = _heads("out", out, x.dtype, tokens, heads, self.head_dim)
+        self._check(positions, freq, tokens)
+        self.ctx._check(self._lib.dcn_rotary_dev(
+            self.ctx.ctx, C.byref(self._c[_dtype(x)]), tokens, heads, x.data_ptr(), xs[0], xs[1], positions.data_ptr(),
+            freq.data_ptr(), int(inverse), out.data_ptr(), os[0], os[1], _stream(stream)))
+
+
+def _cache(k_pages, v_pages, table) -> _lib.DcnCache:
+    if k_pages.dim() != 4 or table.dim() != 2:
+        raise DeformConvError(INVALID_SHAPE, "pages are [pages][page_tokens][heads][channels], the table "
+                                             "[sequences][width]")
+    _whole("k_pages", k_pages, k_pages.dtype, *k_pages.shape)
+    _whole("v_pages", v_pages, k_pages.dtype, *k_pages.shape)
+    _whole("table", table, torch.int32, *table.shape)
+    pages, page_tokens, heads, dim = k_pages.shape
+    return _lib.DcnCache(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
+
+
+def _starts(name: str, t, sequences) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != sequences or not t.is_contiguous():
+        raise DeformConvError(INVALID_SHAPE, f"{name} is not {sequences} int32 values")
+
+
+class CacheAppend(_Handle):
+    """Writes new tokens into a paged cache (dcn_cache_append_dev)."""
+
+    def run_dev(self, k, v, k_pages, v_pages, table, cu_q, kv_lens, rotary: Rotary | None = None, positions=None,
+                freq=None, q=None, q_out=None, stream=None) -> None:
+        """k, v: the new tokens of all sequences, sequence s in rows cu_q[s] .. cu_q[s + 1], the
+        last of its kv_lens[s] tokens. Keys are turned by `rotary` on the way, and so is q into
+        q_out where it is given."""
+        cache = _cache(k_pages, v_pages, table)
+        tokens, sequences = k.shape[0], table.shape[0]
+        s = _lib.DcnAppendShape(sequences, 0, tokens)
+        s.k_stride[:] = _heads("k", k, k_pages.dtype, tokens, cache.kv_heads, cache.head_dim)
+        s.v_stride[:] = _heads("v", v, k_pages.dtype, tokens, cache.kv_heads, cache.head_dim)
+        _starts("cu_q", cu_q, sequences + 1)
+        _starts("kv_lens", kv_lens, sequences)
+        if q is not None:
+            s.q_heads = q.shape[1]
+            s.q_stride[:] = _heads("q", q, k_pages.dtype, tokens, q.shape[1], cache.head_dim)
+            s.q_out_stride[:] = _heads("q_out", q_out, k_pages.dtype, tokens, q.shape[1], cache.head_dim)
+        r = None
+        if rotary is not None:
+            rotary._check(positions, freq, tokens)
+            r = C.byref(rotary._c[cache.dtype])
+        self.ctx._check(self._lib.dcn_cache_append_dev(
+            self.ctx.ctx, C.byref(cache), C.byref(s), r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions),
+            _ptr(freq), cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(),
+            v_pages.data_ptr(), _stream(stream)))
+
+
+class FrameAttention(_Handle):
+    """Attention over a window of frames (dcn_attention_shape): a token of frame f sees the
+    frames f - back .. f + ahead (negative: without an end) and the first `sinks` ones, frames
+    having frame_tokens tokens. frame_tokens = 1 counts in tokens."""
+
+    def __init__(self, ctx: HipDeformConv, q_heads: int, kv_heads: int, head_dim: int, frame_tokens: int = 1,
+                 back: int = -1, ahead: int = 0, sinks: int = 0, scale: float | None = None):
+        super().__init__(ctx)
+        self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
+        _need(self.q_heads > 0 and self.kv_heads > 0 and self.q_heads % self.kv_heads == 0,
+              "q_heads must be a positive multiple of kv_heads")
+        _need(self.head_dim > 0, "head_dim must be positive")
+        self.frame_tokens, self.back, self.ahead, self.sinks = int(frame_tokens), int(back), int(ahead), int(sinks)
+        self.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+
+    def _shape(self, q, sequences, max_q, max_kv, kv_tokens) -> _lib.DcnAttentionShape:
+        return _lib.DcnAttentionShape(_dtype(q), sequences, self.q_heads, self.kv_heads, self.head_dim,
+                                      self.frame_tokens, self.back, self.ahead, self.sinks, max_q, max_kv, self.scale,
+                                      q.shape[0], kv_tokens)
+
+    def _runs(self, q, k, cu_q, cu_kv, max_q, max_kv):
+        """(sequences, max_q, max_kv): without index arrays, one sequence of all rows, or the
+        rows in equal runs of max_q and max_kv."""
+        max_q = q.shape[0] if max_q is None else int(max_q)
+        max_kv = k.shape[0] if max_kv is None else int(max_kv)
+        if cu_q is not None:
+            sequences = cu_q.shape[0] - 1
+        elif cu_kv is not None:
+            sequences = cu_kv.shape[0] - 1
+        else:
+            sequences = q.shape[0] // max_q if max_q else (k.shape[0] // max_kv if max_kv else 0)
+        if cu_q is not None:
+            _starts("cu_q", cu_q, sequences + 1)
+        if cu_kv is not None:
+            _starts("cu_kv", cu_kv, sequences + 1)
+        return sequences, max_q, max_kv
+
+    def _forward_shape(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv):
+        sequences, max_q, max_kv = self._runs(q, k, cu_q, cu_kv, max_q, max_kv)
+        s = self._shape(q, sequences, max_q, max_kv, k.shape[0])
+        s.q_stride[:] = _heads("q", q, q.dtype, None, self.q_heads, self.head_dim)
+        s.k_stride[:] = _heads("k", k, q.dtype, None, self.kv_heads, self.head_dim)
+        s.v_stride[:] = _heads("v", v, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
+        s.out_stride[:] = _heads("out", out, q.dtype, q.shape[0], self.q_heads, self.head_dim)
+        if lse is not None:
+            _whole("lse", lse, torch.float32, q.shape[0], self.q_heads)
+        return s
+
+    def forward_dev(self, q, k, v, out, lse=None, cu_q=None, cu_kv=None, max_q=None, max_kv=None, stream=None) -> None:
+        """out = softmax(scale q k^T over what is visible) v; lse ([tokens][q_heads] FP32) is what
+        backward_dev reads. cu_q, cu_kv: int32 starts of the sequences and the end of the last;
+        max_q and max_kv bound their lengths."""
+        s = self._forward_shape(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
+        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_FORWARD), q)
+        self.ctx._check(self._lib.dcn_attention_forward_dev(
+            self.ctx.ctx, C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_q), _ptr(cu_kv), out.data_ptr(),
+            _ptr(lse), w, size, _stream(stream)))
+
+    def backward_dev(self, q, k, v, out, lse, dout, dq, dk, dv, cu_q=None, cu_kv=None, max_q=None, max_kv=None,
+                     stream=None) -> None:
+        """The gradients of forward_dev's out, from its arguments, out, lse and dout."""
+        s = self._forward_shape(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
+        s.dout_stride[:] = _heads("dout", dout, q.dtype, q.shape[0], self.q_heads, self.head_dim)
+        s.dq_stride[:] = _heads("dq", dq, q.dtype, q.shape[0], self.q_heads, self.head_dim)
+        s.dk_stride[:] = _heads("dk", dk, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
+        s.dv_stride[:] = _heads("dv", dv, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
+        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_BACKWARD), q)
+        self.ctx._check(self._lib.dcn_attention_backward_dev(
+            self.ctx.ctx, C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            dout.data_ptr(), _ptr(cu_q), _ptr(cu_kv), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), w, size,
+            _stream(stream)))
+
+    def paged_dev(self, q, k_pages, v_pages, table, cu_q, kv_lens, out, lse=None, max_q=None, max_kv=None,
+                  stream=None) -> None:
+        """forward_dev over a paged cache: sequence s has kv_lens[s] keys, its queries being the
+        last tokens (one, or a frame's). cu_q None: max_q queries each. max_kv bounds kv_lens
+        (default: the table's width)."""
+        cache = _cache(k_pages, v_pages, table)
+        sequences = table.shape[0]
+        if cu_q is not None:
+            _starts("cu_q", cu_q, sequences + 1)
+        _starts("kv_lens", kv_lens, sequences)
+        if max_q is None:
+            max_q = q.shape[0] if cu_q is not None else (q.shape[0] // sequences if sequences else 0)
+        if max_kv is None:
+            max_kv = cache.table_width * cache.page_tokens
+        s = self._shape(q, sequences, int(max_q), int(max_kv), 0)
+        s.q_stride[:] = _heads("q", q, k_pages.dtype, None, self.q_heads, self.head_dim)
+        s.out_stride[:] = _heads("out", out, k_pages.dtype, q.shape[0], self.q_heads, self.head_dim)
+        if lse is not None:
+            _whole("lse", lse, torch.float32, q.shape[0], self.q_heads)
+        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_PAGED), q)
+        self.ctx._check(self._lib.dcn_attention_paged_dev(
+            self.ctx.ctx, C.byref(s), C.byref(cache), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q),
+            kv_lens.data_ptr(), table.data_ptr(), out.data_ptr(), _ptr(lse), w, size, _stream(stream)))
+
+
+class GatedNorm(_Handle):
+    """The norms around a block (dcn_norm_shape): x_out = x + residual_scale * gate * norm(h) *
+    w_post, y = norm(x_out) * w_pre, with a row of gates for each run of gate_tokens tokens."""
+
+    def __init__(self, ctx: HipDeformConv, channels: int, gate_tokens: int = 1, residual_scale: float = 1.0,
+                 eps: float = 1e-6):
+        super().__init__(ctx)
+        self.channels, self.gate_tokens = int(channels), int(gate_tokens)
+        self.residual_scale, self.eps = float(residual_scale), float(eps)
+        self._kept = None
+        _need(self.channels > 0 and self.gate_tokens > 0, "channels and gate_tokens must be positive")
+
+    def _shape(self, x, gate, vectors, tensors) -> _lib.DcnNormShape:
+        tokens, dtype = x.shape[0], x.dtype
+        for name, t in tensors:
+            if t is not None:
+                _whole(name, t, dtype, tokens, self.channels)
+        for name, t in gate:
+            if t is not None:
+                _whole(name, t, dtype, -(-tokens // self.gate_tokens), self.channels)
+        for name, t, kind in vectors:
+            if t is not None:
+                _whole(name, t, kind or dtype, self.channels)
+        return _lib.DcnNormShape(_dtype(x), self.channels, tokens, self.gate_tokens, self.residual_scale, self.eps)
+
+    def low_bytes(self, x) -> int:
+        """Bytes of forward_dev's `low` for a residual stream like x."""
+        return int(self._lib.dcn_gated_norm_low_bytes(C.byref(self._shape(x, [], [], [("x", x)]))))
+
+    def _low(self, s, low, like, make: bool):
+        """The pointer of the caller's low, or of the handle's own."""
+        count = self._lib.dcn_gated_norm_low_bytes(C.byref(s))
+        if not count:
+            return None
+        if low is not None:
+            if low.dtype != torch.uint8 or low.numel() < count or not low.is_contiguous():
+                raise DeformConvError(INVALID_SHAPE, f"low is not {count} adjacent uint8 values")
+            return low.data_ptr()
+        if self._kept is None or self._kept.numel() < count:
+            if not make:
+                return None
+            if self._kept is not None:
+                torch.cuda.synchronize(like.device)
+            self._kept = torch.empty(count, dtype=torch.uint8, device=like.device)
+        return self._kept.data_ptr()
+
+    def forward_dev(self, h, x, gate, w_post, w_pre, x_out, y=None, rstd=None, low=None, stream=None) -> None:
+        """gate, w_post, w_pre may be None (ones); y None: no block follows. rstd ([tokens][2]
+        FP32) is what backward_dev reads; with it, 16-bit calls keep what rounding takes from
+        x_out (low_bytes(x) uint8 values) in `low`, or in the handle for its next backward_dev."""
+        s = self._shape(x, [("gate", gate)], [("w_post", w_post, None), ("w_pre", w_pre, None)],
+                        [("h", h), ("x", x), ("x_out", x_out), ("y", y)])
+        if rstd is not None:
+            _whole("rstd", rstd, torch.float32, x.shape[0], 2)
+        self.ctx._check(self._lib.dcn_gated_norm_forward_dev(
+            self.ctx.ctx, C.byref(s), h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
+            x_out.data_ptr(), _ptr(y), _ptr(rstd), None if rstd is None else self._low(s, low, x, True),
+            _stream(stream)))
+
+    def backward_dev(self, h, x_out, gate, w_post, w_pre, rstd, dx_out, dy, dh, dx, dgate=None, dw_post=None,
+                     dw_pre=None, low=None, stream=None) -> None:
+        """Gradients from those of x_out and y (dy None where y was not made); dgate, dw_post and
+        dw_pre (FP32) where they are given. Rows whose low halves are not those of the forward
+        that made rstd (the handle ran another one since, and `low` is None) take x_out as it
+        was rounded."""
+        s = self._shape(x_out, [("gate", gate), ("dgate", dgate)],
+                        [("w_post", w_post, None), ("w_pre", w_pre, None), ("dw_post", dw_post, torch.float32),
+                         ("dw_pre", dw_pre, torch.float32)],
+                        [("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dy", dy), ("dh", dh), ("dx", dx)])
+        _whole("rstd", rstd, torch.float32, x_out.shape[0], 2)
+        w, size = self._room(self._lib.dcn_gated_norm_workspace_bytes(C.byref(s)), x_out)
+        self.ctx._check(self._lib.dcn_gated_norm_backward_dev(
+            self.ctx.ctx, C.byref(s), h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
+            rstd.data_ptr(), self._low(s, low, x_out, False), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw_post),
+            _ptr(dw_pre), w, size, _stream(stream)))
