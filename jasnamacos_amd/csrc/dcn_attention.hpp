@@ -90,4 +90,8 @@ size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 hipError_t launch_attention_rows(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 
+// Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).
+hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream);
+size_t attention_forward_workspace(const dcn_attention_shape& s);
+
 }  // namespace dcn

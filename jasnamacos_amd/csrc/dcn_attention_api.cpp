@@ -143,9 +143,24 @@ dcn_status check_even(dcn_context* ctx, const dcn_attention_shape* s, const void
     return DCN_OK;
 }
 
+// Whether the matrix kernels take heads of this kind: 16 bits, 64 or 128 channels, a scale that
+// keeps the order of the scores, and packed rows that an int counts. The rest runs a row at a
+// time, as do tensors that are not aligned to 16 bytes.
+bool matrix_heads(const dcn_attention_shape* s) {
+    return s->dtype != DCN_DTYPE_F32 && (s->head_dim == 64 || s->head_dim == 128) && s->scale > 0.f &&
+           (int64_t)s->max_q * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
+}
+// 16-byte rows, and rows of one tile within 32-bit offsets.
+template <typename H>
+bool matrix_tensor(const H& h) {
+    return (uintptr_t)h.p % 16 == 0 && h.ts % 8 == 0 && h.hs % 8 == 0 && h.ts < (INT64_C(1) << 24);
+}
+// Pages of whole runs of 8 keys, and rows of the pool that an int counts.
+bool matrix_pool(const dcn_cache* c) { return c->page_tokens >= 8 && (int64_t)c->pages * c->page_tokens <= INT32_MAX; }
+
 size_t attention_workspace(const dcn_attention_shape* s, int pass) {
     if (pass == DCN_ATTENTION_BACKWARD) return (size_t)s->q_tokens * s->q_heads * sizeof(float);  // delta
-    return 0;
+    return matrix_heads(s) ? dcn::attention_forward_workspace(*s) : 0;
 }
 
 dcn_status check_workspace(dcn_context* ctx, const void* p, size_t have, size_t need) {
@@ -315,7 +330,8 @@ dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape
         a.cu_q = d_cu_q;
         a.cu_kv = d_cu_kv;
         a.workspace = d_workspace;
-        DCN_HIP(ctx, dcn::launch_attention_rows(shape->dtype, a, (hipStream_t)stream));
+        const bool matrix = matrix_heads(shape) && matrix_tensor(a.q) && matrix_tensor(a.k) && matrix_tensor(a.v) && matrix_tensor(a.out);
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_rows)(shape->dtype, a, (hipStream_t)stream));
         return DCN_OK;
     });
 }
@@ -355,7 +371,9 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
         a.cu_kv = d_kv_lens;
         a.pages.table = d_table;
         a.workspace = d_workspace;
-        DCN_HIP(ctx, dcn::launch_attention_rows(shape->dtype, a, (hipStream_t)stream));
+        const bool matrix = matrix_heads(shape) && matrix_pool(cache) && matrix_tensor(a.q) && matrix_tensor(a.k) &&
+                            matrix_tensor(a.v) && matrix_tensor(a.out);
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_rows)(shape->dtype, a, (hipStream_t)stream));
         return DCN_OK;
     });
 }

@@ -1,0 +1,583 @@
+// Windowed attention forward on the matrix cores: FP16 and BF16 heads of 64 and 128 channels,
+// contiguous or paged keys.
+//
+// Rows are packed: the heads that share a key head stand side by side (row = token, head of
+// the group), so that a key tile is read once for all of them and single tokens fill a
+// wave's rows. One pass over the visible key tiles with the running maximum and sum of the
+// softmax; the maximum is raised (and the sums rescaled) only when a score passes it by more
+// than 2^8, which FP32 sums do not notice. Two shapes:
+//   tile kernel  four waves of 32 rows each share tiles of 64 keys;
+//   few kernel   up to 32 rows: four waves take tiles of 32 keys in turn, each with its own
+//                buffers and no barrier, and are joined at the end.
+// Both may split the key tiles over workgroups; a second kernel then joins the parts.
+#include "dcn_attention_mfma.hpp"
+
+namespace dcn {
+namespace fa {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+// A weight is 2^(score - maximum + kLift): FP16 keeps weights of 2^-20 of the largest normal.
+template <typename T>
+constexpr float kLift = __is_same(T, _Float16) ? 6.f : 0.f;
+constexpr float kSlack = 8.f;
+
+// Where one workgroup works, and the key tiles that its rows see: `near` tiles from the
+// first key (sinks), then those from `first` on.
+struct Place {
+    int seq, kh, split, splits;
+    Run q, kv;
+    int rows;   // packed rows of this (sequence, key head)
+    int row0;   // the workgroup's first
+    int offset; // position of query 0
+};
+
+template <bool PAGED>
+struct Keys {
+    HeadsIn k, v;
+    PagesArgs pages;
+    const char *kp, *vp;  // the head's first row (contiguous: of the sequence)
+    int seq, count;
+
+    __device__ __forceinline__ Keys(const AttentionArgs& a, int s, int kh, const Run& kv) : k(a.k), v(a.v), pages(a.pages) {
+        seq = s;
+        count = kv.count;
+        const int64_t first = PAGED ? 0 : kv.first;
+        kp = (const char*)a.k.p + (first * k.ts + kh * k.hs) * 2;
+        vp = (const char*)a.v.p + (first * v.ts + kh * v.hs) * 2;
+    }
+    // Row of the pool of key j (uniform); -1 where its page is not there. A scalar load: it is not
+    // counted with the copies, so waiting for it does not wait for them.
+    __device__ __forceinline__ int pool_row(int j) const {
+        typedef const __attribute__((address_space(4))) int* scalar;
+        const int page = ((scalar)(uintptr_t)(pages.table + (int64_t)seq * pages.width))[j >> pages.shift];
+        return (unsigned)page >= (unsigned)pages.pages ? -1 : (page << pages.shift) + (j & ((1 << pages.shift) - 1));
+    }
+    // Value row of key j, or null.
+    __device__ __forceinline__ const uint16_t* value(int j) const {
+        const int64_t row = PAGED ? pool_row(j) : j;
+        return row < 0 ? nullptr : (const uint16_t*)(vp + row * v.ts * 2);
+    }
+};
+
+// Pages have 8 tokens at least, and every run of 8 keys from a multiple of 8 lies on one. What
+// the copies of a tile of ROWS keys need of the table, looked up a tile ahead: the rows of the
+// pool that copy instructions wave, wave + WAVES, ... start at (past the sequence's end: those
+// of its last run; rows past it are in the pool, and not visible), and a bit per key whose page
+// is not there.
+template <int D, int ROWS, int WAVES, bool PAGED>
+struct TilePages {
+    static constexpr int kCopies = ROWS / Tile<D>::kRowsPerCopy / WAVES;
+    int row[kCopies];
+    unsigned long long holes = 0;
+
+    __device__ __forceinline__ void find(const Keys<PAGED>& keys, int t0, int wave) {
+        if constexpr (PAGED) {
+            const int last = (keys.count - 1) & ~7;
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) {
+                const int in = (n * WAVES + wave) * Tile<D>::kRowsPerCopy, j = t0 + (in & ~7);
+                const int r = keys.pool_row(j < last ? j : last);
+                row[n] = r < 0 ? 0 : r + (in & 7);
+            }
+            holes = 0;
+#pragma unroll
+            for (int g = 0; g < ROWS / 8; ++g) {
+                const int j = t0 + 8 * g;
+                if (keys.pool_row(j < last ? j : last) < 0) holes |= 0xffull << (8 * g);
+            }
+        }
+    }
+};
+
+// Copies the tile of ROWS keys from t0 (below the sequence's end) to `k` and `v`; this wave's
+// part. Contiguous rows past the end are copies of the last one.
+template <int D, int ROWS, int WAVES, bool PAGED>
+__device__ __forceinline__ void copy_tile(const Keys<PAGED>& keys, int t0, const TilePages<D, ROWS, WAVES, PAGED>& pages, char* k,
+                                          char* v, int wave, int lane) {
+    using Ti = Tile<D>;
+    const char* kb = keys.kp + (int64_t)t0 * keys.k.ts * 2;
+    const char* vb = keys.vp + (int64_t)t0 * keys.v.ts * 2;
+    const int last = keys.count - 1 - t0;
+#pragma unroll
+    for (int n = 0; n < pages.kCopies; ++n) {
+        const int i = n * WAVES + wave, r = Ti::copy_row(i, lane), c = Ti::copy_channel(r, lane);
+        if constexpr (PAGED) {
+            const uint32_t in = lane / Ti::kChunks;
+            copy16(keys.kp + (int64_t)pages.row[n] * keys.k.ts * 2, (in * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
+            copy16(keys.vp + (int64_t)pages.row[n] * keys.v.ts * 2, (in * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
+        } else {
+            const uint32_t at = r < last ? r : last;
+            copy16(kb, (at * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
+            copy16(vb, (at * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
+        }
+    }
+}
+
+// One wave's 32 rows: queries, sums and the running maximum.
+template <typename T, int D>
+struct RowState {
+    u32x4 q[D / 16];
+    f32x16 o[D / 32];
+    float m, l;  // m: in units of log2, over the scaled scores
+    Span sp;
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+    // The queries are there: no wait for them later, which would wait for the copies too.
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
+    }
+    // ROWS keys from t0. MASKED: some row may not see some key (holes: bit per key that is not there).
+    template <int ROWS, bool MASKED>
+    __device__ __forceinline__ void add(const char* kt, const char* vt, int t0, float c, unsigned long long holes, int lane) {
+        constexpr int MB = ROWS / 32;
+        using Ti = Tile<D>;
+        f32x16 s[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) s[mb] = mma<T>(Ti::rows(kt, mb, i, lane), q[i], s[mb]);
+        }
+        const int base = t0 + 4 * (lane >> 5);
+        if constexpr (MASKED) {
+            const unsigned long long gone = holes >> (4 * (lane >> 5));
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int in = 32 * mb + 8 * (r >> 2) + (r & 3), j = base + in;
+                    const bool on = sees(sp, j) && !((uint32_t)(gone >> (in & 32)) >> (in & 31) & 1);
+                    s[mb][r] = on ? s[mb][r] : -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[mb][r]);
+        top = both_max(top) * c;
+        if (__any(top > m + kSlack)) {
+            const float next = fmaxf(m, top);
+            const float old = exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= old;
+        }
+        const float ref = kLift<T> - (m == -INFINITY ? 0.f : m);
+        float sum[4] = {};
+        u32x4 p[MB * 2];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[mb][r] = __builtin_amdgcn_exp2f(fmaf(s[mb][r], c, ref));
+                sum[r & 3] += s[mb][r];
+            }
+            p[2 * mb] = pack8<T>(s[mb], 0);
+            p[2 * mb + 1] = pack8<T>(s[mb], 8);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] = mma<T>(Ti::columns(vt, mb, st, i, lane), p[2 * mb + st], o[i]);
+    }
+};
+
+// Infinities and NaN of the values in [from, to) of a tile, which stand as zeros in LDS, to the
+// sums of the rows that see them.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void add_nonfinite(RowState<T, D>& st, const Keys<PAGED>& keys, int t0, int rows, unsigned long long holes,
+                                              int lane) {
+    const int to = t0 + rows < keys.count ? t0 + rows : keys.count;
+    for (int j = t0; j < to; ++j) {
+        const uint16_t* v = keys.value(j);
+        if (!v) continue;
+        const bool on = sees(st.sp, j) && !(holes >> (j - t0) & 1);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const u32x2 four = *(const u32x2*)(v + 32 * i + 8 * a + 4 * (lane >> 5));
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const uint16_t bits = (uint16_t)(four[b >> 1] >> (16 * (b & 1)));
+                    if (on && !finite16<T>(bits)) st.o[i][4 * a + b] += widen(__builtin_bit_cast(T, bits));
+                }
+                asm volatile("" ::: "memory");  // one load at a time: few registers, and this is rare
+            }
+    }
+}
+
+// Zeros for the infinities and NaN of a tile of values, by `threads` threads; whether a thread saw one.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ bool clean_tile(char* v, int thread, int threads) {
+    bool bad = false;
+    for (int i = thread; i < ROWS * D / 8; i += threads) {
+        u32x4 x = *(const u32x4*)(v + i * 16);
+        if (clean16<T>(x)) {
+            *(u32x4*)(v + i * 16) = x;
+            bad = true;
+        }
+    }
+    return bad;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void load_queries(RowState<T, D>& st, const AttentionArgs& a, const Place& pl, const Rows& rw, int r,
+                                             int lane) {
+    r = r < pl.rows ? r : pl.rows - 1;
+    const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+    const char* p = (const char*)a.q.p + ((pl.q.first + tok) * a.q.ts + head * a.q.hs + 8 * (lane >> 5)) * 2;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) st.q[i] = *(const u32x4*)(p + i * 32);
+}
+
+// A row's result, or its part (splits > 1): FP32 sums with the weights' reference.
+template <typename T, int D>
+__device__ __forceinline__ void store_row4(const AttentionArgs& a, const Place& pl, int64_t index, int64_t row, int head, int at,
+                                           const float* o, float inv) {
+    if (pl.splits == 1) {
+        typedef T four __attribute__((ext_vector_type(4)));
+        four v;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[b] = narrow<T>(o[b] * inv);
+        *(four*)((T*)a.out.p + row * a.out.ts + head * a.out.hs + at) = v;
+    } else {
+        float* w = (float*)a.workspace + (index * pl.splits + pl.split) * (D + 4) + at;
+        *(f32x4*)w = f32x4{o[0], o[1], o[2], o[3]};
+    }
+}
+template <int D>
+__device__ __forceinline__ void store_sums(const AttentionArgs& a, const Place& pl, int64_t index, float m, float l, float lift) {
+    if (pl.splits == 1) {
+        if (a.lse) a.lse[index] = l == 0.f ? -INFINITY : (m - lift + __builtin_amdgcn_logf(l)) * kLn2;
+    } else {
+        float* w = (float*)a.workspace + (index * pl.splits + pl.split) * (D + 4) + D;
+        w[0] = m;
+        w[1] = l;
+    }
+}
+
+// blockIdx.x = split + splits * row block (the last rows first: they see the most keys).
+template <int ROWS_WG>
+__device__ __forceinline__ bool place_of(const AttentionArgs& a, int splits, Place* pl) {
+    pl->seq = blockIdx.z;
+    pl->kh = blockIdx.y;
+    pl->splits = splits;
+    const int block = gridDim.x / splits - 1 - blockIdx.x / splits;
+    pl->split = blockIdx.x % splits;
+    pl->q = run_of(a.cu_q, pl->seq, a.max_q, a.q_tokens);
+    pl->kv = kv_run_of(a, pl->seq);
+    pl->q.count = uniform(pl->q.count);
+    pl->kv.count = uniform(pl->kv.count);
+    pl->offset = pl->kv.count - pl->q.count;
+    const int64_t rows = (int64_t)(pl->q.count < a.max_q ? pl->q.count : a.max_q) * a.group;
+    pl->rows = (int)rows;
+    pl->row0 = block * ROWS_WG;
+    return pl->row0 < pl->rows;
+}
+
+struct Spread {
+    Span first, last;  // of the first and the last row of a run of rows: all three ends grow with the position
+};
+__device__ __forceinline__ Spread spread_of(const AttentionArgs& a, const Place& pl, const Rows& rw, int from, int to) {
+    Spread s;
+    s.first = span_of(a, pl.offset + rw.token(from), pl.kv.count);
+    s.last = span_of(a, pl.offset + rw.token(to), pl.kv.count);
+    return s;
+}
+// Tiles of ROWS keys that some row of the run sees.
+template <int ROWS>
+struct TileList {
+    int near, first, count;
+    __device__ __forceinline__ TileList(const Spread& s) {
+        const int end = (s.last.hi + ROWS - 1) / ROWS;
+        first = s.first.lo / ROWS;
+        near = (s.last.sink + ROWS - 1) / ROWS;
+        if (near > first) near = first;
+        count = near + (end > first ? end - first : 0);
+    }
+    __device__ __forceinline__ int tile(int i) const { return (i < near ? i : first + (i - near)) * ROWS; }
+};
+template <int ROWS>
+__device__ __forceinline__ bool all_see(const Spread& s, int t0) {
+    const int t1 = t0 + ROWS;
+    return t1 <= s.first.hi && (t0 >= s.last.lo || t1 <= s.first.sink);
+}
+template <int ROWS>
+__device__ __forceinline__ bool none_sees(const Spread& s, int t0) {
+    return t0 >= s.last.hi || (t0 + ROWS <= s.first.lo && t0 >= s.last.sink);
+}
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionArgs a, int splits) {
+    constexpr int ROWS = 64, BYTES = ROWS * D * 2;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    Place pl;
+    if (!place_of<32 * kWaves>(a, splits, &pl)) return;
+    const Rows rw = rows_of(a.group);
+    const int last_row = pl.rows - 1;
+    const int w0 = pl.row0 + 32 * wave, w1 = w0 + 31 < last_row ? w0 + 31 : last_row;
+    const Spread all = spread_of(a, pl, rw, pl.row0, pl.row0 + 32 * kWaves - 1 < last_row ? pl.row0 + 32 * kWaves - 1 : last_row);
+    const bool idle = w0 > last_row;  // the wave has no rows: it copies only
+    const Spread mine = idle ? all : spread_of(a, pl, rw, w0, w1);
+    RowState<T, D> st;
+    st.clear();
+    const int r = w0 + (lane & 31);
+    st.sp = r <= last_row ? span_of(a, pl.offset + rw.token(r), pl.kv.count) : Span{0, 0, 0};
+    load_queries(st, a, pl, rw, r, lane);
+    const TileList<ROWS> list(all);
+    const int per = (list.count + splits - 1) / splits;
+    const int from = pl.split * per, to = from + per < list.count ? from + per : list.count;
+    const Keys<PAGED> keys(a, pl.seq, pl.kh, pl.kv);
+    const float c = a.scale * kLog2e;
+    TilePages<D, ROWS, kWaves, PAGED> pages, next;  // of the tile whose copies are next; one further
+    if (from < to) {
+        pages.find(keys, list.tile(from), wave);
+        copy_tile<D, ROWS, kWaves, PAGED>(keys, list.tile(from), pages, lds[0][0], lds[0][1], wave, lane);
+    }
+    unsigned long long holes = pages.holes;
+    if (from + 1 < to) next.find(keys, list.tile(from + 1), wave);
+    st.settle();
+    for (int i = from; i < to; ++i) {
+        char(*now)[BYTES] = lds[(i - from) & 1], (*other)[BYTES] = lds[((i - from) & 1) ^ 1];
+        const int t0 = list.tile(i);
+        wait_copies<0>();
+        __syncthreads();
+        if (i + 1 < to) {
+            pages = next;
+            copy_tile<D, ROWS, kWaves, PAGED>(keys, list.tile(i + 1), pages, other[0], other[1], wave, lane);
+            if (i + 2 < to) next.find(keys, list.tile(i + 2), wave);
+        }
+        bool bad = false;
+        if (holes || !all_see<ROWS>(all, t0)) bad = __syncthreads_or(clean_tile<T, D, ROWS>(now[1], threadIdx.x, kThreads));
+        if (!idle && !none_sees<ROWS>(mine, t0)) {
+            if (!holes && all_see<ROWS>(mine, t0)) st.template add<ROWS, false>(now[0], now[1], t0, c, 0, lane);
+            else st.template add<ROWS, true>(now[0], now[1], t0, c, holes, lane);
+            if (bad) add_nonfinite(st, keys, t0, ROWS, holes, lane);
+        }
+        holes = pages.holes;
+    }
+    if (r > last_row) return;
+    const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+    const int64_t row = pl.q.first + tok, index = row * a.q_heads + head;
+    const float l = both_sum(st.l), inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float o[4] = {st.o[i][4 * x], st.o[i][4 * x + 1], st.o[i][4 * x + 2], st.o[i][4 * x + 3]};
+            store_row4<T, D>(a, pl, index, row, head, 32 * i + 8 * x + 4 * (lane >> 5), o, inv);
+        }
+    if (lane < 32) store_sums<D>(a, pl, index, st.m, l, kLift<T>);
+}
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kernel(AttentionArgs a, int splits) {
+    constexpr int ROWS = 32, BYTES = ROWS * D * 2, COPIES = 2 * ROWS / Tile<D>::kRowsPerCopy;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];  // [wave][2][2][BYTES], then the join
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    Place pl;
+    if (!place_of<32>(a, splits, &pl)) return;
+    const Rows rw = rows_of(a.group);
+    const int last_row = pl.rows - 1;
+    const Spread all = spread_of(a, pl, rw, pl.row0, pl.row0 + 31 < last_row ? pl.row0 + 31 : last_row);
+    RowState<T, D> st;
+    st.clear();
+    const int r = pl.row0 + (lane & 31);
+    st.sp = r <= last_row ? span_of(a, pl.offset + rw.token(r), pl.kv.count) : Span{0, 0, 0};
+    load_queries(st, a, pl, rw, r, lane);
+    const TileList<ROWS> list(all);
+    const int per = (list.count + splits - 1) / splits;
+    const int from = pl.split * per, to = from + per < list.count ? from + per : list.count;
+    const Keys<PAGED> keys(a, pl.seq, pl.kh, pl.kv);
+    const float c = a.scale * kLog2e;
+    char* own = lds + wave * 4 * BYTES;
+    int n = 0;
+    TilePages<D, ROWS, 1, PAGED> pages, next;
+    if (from + wave < to) {
+        pages.find(keys, list.tile(from + wave), 0);
+        copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(from + wave), pages, own, own + BYTES, 0, lane);
+    }
+    unsigned long long holes = pages.holes;
+    if (from + wave + kWaves < to) next.find(keys, list.tile(from + wave + kWaves), 0);
+    st.settle();
+    for (int i = from + wave; i < to; i += kWaves, ++n) {
+        char *kt = own + (n & 1) * 2 * BYTES, *vt = kt + BYTES, *other = own + ((n + 1) & 1) * 2 * BYTES;
+        const int t0 = list.tile(i);
+        if (i + kWaves < to) {
+            pages = next;
+            copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(i + kWaves), pages, other, other + BYTES, 0, lane);
+            if (i + 2 * kWaves < to) next.find(keys, list.tile(i + 2 * kWaves), 0);
+            wait_copies<COPIES>();
+        } else {
+            wait_copies<0>();
+        }
+        const bool whole = !holes && all_see<ROWS>(all, t0);
+        bool bad = false;
+        if (!whole) bad = __any(clean_tile<T, D, ROWS>(vt, lane, 64));
+        if (whole) st.template add<ROWS, false>(kt, vt, t0, c, 0, lane);
+        else st.template add<ROWS, true>(kt, vt, t0, c, holes, lane);
+        if (bad) add_nonfinite(st, keys, t0, ROWS, holes, lane);
+        holes = pages.holes;
+        wait_reads();  // the next copies go where this tile was
+    }
+    // Join the waves: [wave][32 rows][D + 4] FP32 (rows of D + 4 keep the stores off each other's banks).
+    __syncthreads();
+    float* mem = (float*)lds;
+    constexpr int LINE = D + 4;
+    float* line = mem + (wave * 32 + (lane & 31)) * LINE;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            *(f32x4*)(line + 32 * i + 8 * x + 4 * (lane >> 5)) =
+                f32x4{st.o[i][4 * x], st.o[i][4 * x + 1], st.o[i][4 * x + 2], st.o[i][4 * x + 3]};
+    const float l = both_sum(st.l);
+    if (lane < 32) {
+        line[D] = st.m;
+        line[D + 1] = l;
+    }
+    __syncthreads();
+    // Eight threads a row.
+    const int jr = threadIdx.x >> 3, part = threadIdx.x & 7;
+    if (pl.row0 + jr > last_row) return;
+    float m = -INFINITY, sum = 0.f, w[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, mem[(i * 32 + jr) * LINE + D]);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        w[i] = exp2f(mem[(i * 32 + jr) * LINE + D] - (m == -INFINITY ? 0.f : m));
+        sum = fmaf(w[i], mem[(i * 32 + jr) * LINE + D + 1], sum);
+    }
+    const int tok = rw.token(pl.row0 + jr), head = pl.kh * a.group + (pl.row0 + jr - tok * a.group);
+    const int64_t row = pl.q.first + tok, index = row * a.q_heads + head;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int at = part * 4; at < D; at += 32) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const f32x4 v = *(const f32x4*)(mem + (i * 32 + jr) * LINE + at);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) o[b] = fmaf(w[i], v[b], o[b]);
+        }
+        const float four[4] = {o[0], o[1], o[2], o[3]};
+        store_row4<T, D>(a, pl, index, row, head, at, four, inv);
+    }
+    if (part == 0) store_sums<D>(a, pl, index, m, sum, kLift<T>);
+}
+
+// One wave a row and head: the parts of all splits, in their order.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs a, int splits) {
+    const int lane = threadIdx.x & 63;
+    const Run q = run_of(a.cu_q, blockIdx.z, a.max_q, a.q_tokens);
+    const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int tok = (int)(item / a.q_heads), head = (int)(item % a.q_heads);
+    if (tok >= q.count || tok >= a.max_q) return;
+    const int64_t row = q.first + tok, index = row * a.q_heads + head;
+    const float* parts = (const float*)a.workspace + index * splits * (D + 4);
+    float m = -INFINITY;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, parts[s * (D + 4) + D]);
+    float sum = 0.f, o[D / 64] = {};
+    for (int s = 0; s < splits; ++s) {
+        const float* p = parts + s * (D + 4);
+        const float w = exp2f(p[D] - (m == -INFINITY ? 0.f : m));
+        sum = fmaf(w, p[D + 1], sum);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) o[i] = fmaf(w, p[lane + 64 * i], o[i]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)a.out.p + row * a.out.ts + head * a.out.hs;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) out[lane + 64 * i] = narrow<T>(o[i] * inv);
+    if (a.lse && lane == 0) a.lse[index] = sum == 0.f ? -INFINITY : (m - kLift<T> + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// Row blocks, and over how many workgroups each one's key tiles are split.
+struct Plan {
+    bool few;
+    int blocks, splits;
+};
+Plan plan_of(int sequences, int kv_heads, int group, int max_q, int max_kv, int frame, int back, int sinks) {
+    Plan p;
+    const int64_t rows = (int64_t)max_q * group;
+    p.few = rows <= 32;
+    const int per_block = p.few ? 32 : 128, tile = p.few ? 32 : 64;
+    p.blocks = (int)((rows + per_block - 1) / per_block);
+    // Keys that one row block sees at most.
+    int64_t keys = max_kv;
+    if (back >= 0) {
+        const int64_t window = ((int64_t)back + 1 + sinks) * frame + per_block / group + 2 * tile;
+        keys = window < keys ? window : keys;
+    }
+    const int64_t tiles = (keys + tile - 1) / tile, groups = (int64_t)p.blocks * kv_heads * sequences;
+    // Two workgroups a CU, each with at least four tiles (few: four a wave).
+    const int64_t least = p.few ? 16 : 4;
+    int64_t splits = groups > 0 ? (512 + groups - 1) / groups : 1;
+    if (splits > tiles / least) splits = tiles / least;
+    p.splits = (int)(splits < 1 ? 1 : (splits > 64 ? 64 : splits));
+    return p;
+}
+
+template <typename T, int D, bool PAGED>
+hipError_t run(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
+    const dim3 grid((unsigned)p.blocks * p.splits, a.kv_heads, a.sequences);
+    if (p.few) {
+        constexpr int copies = kWaves * 4 * 32 * D * 2, join = kWaves * 32 * (D + 4) * 4;
+        constexpr int bytes = copies > join ? copies : join;
+        const void* f = (const void*)attention_few_kernel<T, D, PAGED>;
+        if (hipError_t e = allow_dynamic_lds(f, bytes)) return e;
+        attention_few_kernel<T, D, PAGED><<<grid, kThreads, bytes, stream>>>(a, p.splits);
+    } else {
+        attention_tile_kernel<T, D, PAGED><<<grid, kThreads, 0, stream>>>(a, p.splits);
+    }
+    if (hipError_t e = hipGetLastError()) return e;
+    if (p.splits == 1) return hipSuccess;
+    const int64_t rows = (int64_t)a.max_q * a.q_heads;
+    attention_join_kernel<T, D><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, p.splits);
+    return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t by_keys(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
+    return a.pages.table ? run<T, D, true>(a, p, stream) : run<T, D, false>(a, p, stream);
+}
+template <typename T>
+hipError_t by_dim(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
+    return a.dim == 64 ? by_keys<T, 64>(a, p, stream) : by_keys<T, 128>(a, p, stream);
+}
+
+}  // namespace
+}  // namespace fa
+
+size_t attention_forward_workspace(const dcn_attention_shape& s) {
+    const fa::Plan p = fa::plan_of(s.sequences, s.kv_heads, s.q_heads / s.kv_heads, s.max_q, s.max_kv, s.frame_tokens, s.back, s.sinks);
+    return p.splits == 1 ? 0 : (size_t)s.q_tokens * s.q_heads * p.splits * (s.head_dim + 4) * sizeof(float);
+}
+
+hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream) {
+    const fa::Plan p = fa::plan_of(a.sequences, a.kv_heads, a.group, a.max_q, a.max_kv, a.frame, a.back, a.sinks);
+    return dtype == DCN_DTYPE_F16 ? fa::by_dim<_Float16>(a, p, stream) : fa::by_dim<fa::bf16>(a, p, stream);
+}
+
+}  // namespace dcn
