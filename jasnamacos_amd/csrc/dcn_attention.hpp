@@ -93,5 +93,7 @@ hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hip
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).
 hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream);
 size_t attention_forward_workspace(const dcn_attention_shape& s);
+hipError_t launch_attention_matrix_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
+size_t attention_backward_workspace(const dcn_attention_shape& s);
 
 }  // namespace dcn

@@ -159,7 +159,8 @@ bool matrix_tensor(const H& h) {
 bool matrix_pool(const dcn_cache* c) { return c->page_tokens >= 8 && (int64_t)c->pages * c->page_tokens <= INT32_MAX; }
 
 size_t attention_workspace(const dcn_attention_shape* s, int pass) {
-    if (pass == DCN_ATTENTION_BACKWARD) return (size_t)s->q_tokens * s->q_heads * sizeof(float);  // delta
+    if (pass == DCN_ATTENTION_BACKWARD)  // the rows' delta at least
+        return matrix_heads(s) ? dcn::attention_backward_workspace(*s) : (size_t)s->q_tokens * s->q_heads * sizeof(float);
     return matrix_heads(s) ? dcn::attention_forward_workspace(*s) : 0;
 }
 
@@ -423,7 +424,11 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
         a.workspace = d_workspace;
         if (!shape->q_tokens) a.max_q = 0;
         if (!shape->kv_tokens) a.max_kv = 0;
-        DCN_HIP(ctx, dcn::launch_attention_rows_backward(shape->dtype, a, (hipStream_t)stream));
+        bool matrix = matrix_heads(shape);
+        for (const dcn::HeadsIn* h : {&a.q, &a.k, &a.v, &a.o, &a.dout}) matrix = matrix && matrix_tensor(*h);
+        for (const dcn::HeadsOut* h : {&a.dq, &a.dk, &a.dv}) matrix = matrix && matrix_tensor(*h);
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix_backward : dcn::launch_attention_rows_backward)(shape->dtype, a,
+                                                                                                          (hipStream_t)stream));
         return DCN_OK;
     });
 }

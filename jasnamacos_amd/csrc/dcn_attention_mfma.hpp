@@ -140,6 +140,211 @@ __device__ __forceinline__ bool clean16(u32x4& v) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+
+// Where one workgroup works.
+struct Place {
+    int seq, kh, split, splits;
+    Run q, kv;
+    int rows;   // packed rows of this (sequence, key head)
+    int row0;   // the workgroup's first
+    int offset; // position of query 0
+};
+
+template <bool PAGED>
+struct Keys {
+    HeadsIn k, v;
+    PagesArgs pages;
+    const char *kp, *vp;  // the head's first row (contiguous: of the sequence)
+    int seq, count;
+
+    __device__ __forceinline__ Keys(const AttentionArgs& a, int s, int kh, const Run& kv) : k(a.k), v(a.v), pages(a.pages) {
+        seq = s;
+        count = kv.count;
+        const int64_t first = PAGED ? 0 : kv.first;
+        kp = (const char*)a.k.p + (first * k.ts + kh * k.hs) * 2;
+        vp = (const char*)a.v.p + (first * v.ts + kh * v.hs) * 2;
+    }
+    // Row of the pool of key j (uniform); -1 where its page is not there. A scalar load: it is not
+    // counted with the copies, so waiting for it does not wait for them.
+    __device__ __forceinline__ int pool_row(int j) const {
+        typedef const __attribute__((address_space(4))) int* scalar;
+        const int page = ((scalar)(uintptr_t)(pages.table + (int64_t)seq * pages.width))[j >> pages.shift];
+        return (unsigned)page >= (unsigned)pages.pages ? -1 : (page << pages.shift) + (j & ((1 << pages.shift) - 1));
+    }
+    __device__ __forceinline__ int end(int t1) const { return t1 < count ? t1 : count; }
+    // Value row of key j, or null.
+    __device__ __forceinline__ const uint16_t* value(int j) const {
+        const int64_t row = PAGED ? pool_row(j) : j;
+        return row < 0 ? nullptr : (const uint16_t*)(vp + row * v.ts * 2);
+    }
+};
+
+// Pages have 8 tokens at least, and every run of 8 keys from a multiple of 8 lies on one. What
+// the copies of a tile of ROWS keys need of the table, looked up a tile ahead: the rows of the
+// pool that copy instructions wave, wave + WAVES, ... start at (past the sequence's end: those
+// of its last run; rows past it are in the pool, and not visible), and a bit per key whose page
+// is not there.
+template <int D, int ROWS, int WAVES, bool PAGED>
+struct TilePages {
+    static constexpr int kCopies = ROWS / Tile<D>::kRowsPerCopy / WAVES;
+    int row[kCopies];
+    unsigned long long holes = 0;
+
+    __device__ __forceinline__ void find(const Keys<PAGED>& keys, int t0, int wave) {
+        if constexpr (PAGED) {
+            const int last = (keys.count - 1) & ~7;
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) {
+                const int in = (n * WAVES + wave) * Tile<D>::kRowsPerCopy, j = t0 + (in & ~7);
+                const int r = keys.pool_row(j < last ? j : last);
+                row[n] = r < 0 ? 0 : r + (in & 7);
+            }
+            holes = 0;
+#pragma unroll
+            for (int g = 0; g < ROWS / 8; ++g) {
+                const int j = t0 + 8 * g;
+                if (keys.pool_row(j < last ? j : last) < 0) holes |= 0xffull << (8 * g);
+            }
+        }
+    }
+};
+
+// Copies the tile of ROWS keys from t0 (below the sequence's end) to `k` and `v`; this wave's
+// part. Contiguous rows past the end are copies of the last one.
+template <int D, int ROWS, int WAVES, bool PAGED>
+__device__ __forceinline__ void copy_tile(const Keys<PAGED>& keys, int t0, const TilePages<D, ROWS, WAVES, PAGED>& pages, char* k,
+                                          char* v, int wave, int lane) {
+    using Ti = Tile<D>;
+    const char* kb = keys.kp + (int64_t)t0 * keys.k.ts * 2;
+    const char* vb = keys.vp + (int64_t)t0 * keys.v.ts * 2;
+    const int last = keys.count - 1 - t0;
+#pragma unroll
+    for (int n = 0; n < pages.kCopies; ++n) {
+        const int i = n * WAVES + wave, r = Ti::copy_row(i, lane), c = Ti::copy_channel(r, lane);
+        if constexpr (PAGED) {
+            const uint32_t in = lane / Ti::kChunks;
+            copy16(keys.kp + (int64_t)pages.row[n] * keys.k.ts * 2, (in * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
+            copy16(keys.vp + (int64_t)pages.row[n] * keys.v.ts * 2, (in * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
+        } else {
+            const uint32_t at = r < last ? r : last;
+            copy16(kb, (at * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
+            copy16(vb, (at * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
+        }
+    }
+}
+
+// Whether a tile holds infinities or NaN in the chunks that a thread looks at.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ bool tile_nonfinite(const char* v, int thread, int threads) {
+    bool bad = false;
+    for (int i = thread; i < ROWS * D / 8; i += threads) {
+        u32x4 x = *(const u32x4*)(v + i * 16);
+        bad |= clean16<T>(x);
+    }
+    return bad;
+}
+// Zeros for the infinities and NaN of a tile, by `threads` threads; whether a thread saw one.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ bool clean_tile(char* v, int thread, int threads) {
+    bool bad = false;
+    for (int i = thread; i < ROWS * D / 8; i += threads) {
+        u32x4 x = *(const u32x4*)(v + i * 16);
+        if (clean16<T>(x)) {
+            *(u32x4*)(v + i * 16) = x;
+            bad = true;
+        }
+    }
+    return bad;
+}
+
+// Infinities and NaN of one row of 16-bit channels, which stand as zeros in LDS, to a lane's sums
+// (o^T: channels 32 i + 8 a + 4 h + b) if `on`.
+template <typename T, int D>
+__device__ __forceinline__ void add_nonfinite(f32x16* o, const uint16_t* row, bool on, int lane) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const u32x2 four = *(const u32x2*)(row + 32 * i + 8 * a + 4 * (lane >> 5));
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint16_t bits = (uint16_t)(four[b >> 1] >> (16 * (b & 1)));
+                if (on && !finite16<T>(bits)) o[i][4 * a + b] += widen(__builtin_bit_cast(T, bits));
+            }
+            asm volatile("" ::: "memory");  // one load at a time: few registers, and this is rare
+        }
+}
+// The same for the rows of a tile of keys, `row(j)` that of key j or null.
+template <typename T, int D, typename Row>
+__device__ __forceinline__ void add_nonfinite(f32x16* o, const Span& sp, int t0, int to, unsigned long long holes, int lane, Row row) {
+    for (int j = t0; j < to; ++j)
+        if (const uint16_t* v = row(j)) add_nonfinite<T, D>(o, v, sees(sp, j) && !(holes >> (j - t0) & 1), lane);
+}
+
+// blockIdx.x = split + splits * row block (the last rows first: they see the most keys).
+template <int ROWS_WG>
+__device__ __forceinline__ bool place_of(const AttentionArgs& a, int splits, Place* pl) {
+    pl->seq = blockIdx.z;
+    pl->kh = blockIdx.y;
+    pl->splits = splits;
+    const int block = gridDim.x / splits - 1 - blockIdx.x / splits;
+    pl->split = blockIdx.x % splits;
+    pl->q = run_of(a.cu_q, pl->seq, a.max_q, a.q_tokens);
+    pl->kv = kv_run_of(a, pl->seq);
+    pl->q.count = uniform(pl->q.count);
+    pl->kv.count = uniform(pl->kv.count);
+    pl->offset = pl->kv.count - pl->q.count;
+    const int64_t rows = (int64_t)(pl->q.count < a.max_q ? pl->q.count : a.max_q) * a.group;
+    pl->rows = (int)rows;
+    pl->row0 = block * ROWS_WG;
+    return pl->row0 < pl->rows;
+}
+
+// The B operand of packed row r (past the end: of the last one): channels 16 i + 8 h .. + 7.
+template <int D>
+__device__ __forceinline__ void load_row(u32x4* to, const HeadsIn& t, const AttentionArgs& a, const Place& pl, const Rows& rw, int r,
+                                         int lane) {
+    r = r < pl.rows ? r : pl.rows - 1;
+    const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+    const char* p = (const char*)t.p + ((pl.q.first + tok) * t.ts + head * t.hs + 8 * (lane >> 5)) * 2;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) to[i] = *(const u32x4*)(p + i * 32);
+}
+
+struct Spread {
+    Span first, last;  // of the first and the last row of a run of rows: all three ends grow with the position
+};
+__device__ __forceinline__ Spread spread_of(const AttentionArgs& a, const Place& pl, const Rows& rw, int from, int to) {
+    Spread s;
+    s.first = span_of(a, pl.offset + rw.token(from), pl.kv.count);
+    s.last = span_of(a, pl.offset + rw.token(to), pl.kv.count);
+    return s;
+}
+// Tiles of ROWS keys that some row of the run sees.
+template <int ROWS>
+struct TileList {
+    int near, first, count;
+    __device__ __forceinline__ TileList(const Spread& s) {
+        const int end = (s.last.hi + ROWS - 1) / ROWS;
+        first = s.first.lo / ROWS;
+        near = (s.last.sink + ROWS - 1) / ROWS;
+        if (near > first) near = first;
+        count = near + (end > first ? end - first : 0);
+    }
+    __device__ __forceinline__ int tile(int i) const { return (i < near ? i : first + (i - near)) * ROWS; }
+};
+template <int ROWS>
+__device__ __forceinline__ bool all_see(const Spread& s, int t0) {
+    const int t1 = t0 + ROWS;
+    return t1 <= s.first.hi && (t0 >= s.last.lo || t1 <= s.first.sink);
+}
+template <int ROWS>
+__device__ __forceinline__ bool none_sees(const Spread& s, int t0) {
+    return t0 >= s.last.hi || (t0 + ROWS <= s.first.lo && t0 >= s.last.sink);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -1,0 +1,537 @@
+// Gradients of windowed attention on the matrix cores: FP16 and BF16 heads of 64 and 128 channels.
+//
+// With P = exp(S - lse) again from q, k and lse, delta = rowsum(dO * O) and dP = dO V^T:
+//   dS = P (dP - delta), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO.
+// Two passes, so that no sum is made with atomics and the same inputs give the same bits: one
+// over query rows (dQ, and delta on the way), one over keys (dK and dV); seven products for
+// the five of a pass that adds dQ up in memory. Both keep a wave's rows (keys) in registers as
+// the B operand and as columns of the sums, as the forward does, and walk tiles of the other
+// side in LDS.
+//
+// FP16 would lose gradients below 2^-24 and overflow above 2^16: dS enters its products
+// times a power of two that follows the largest one seen of its row (first pass) or its key
+// (second), P times 2^10. BF16 has FP32's range and needs neither.
+#include "dcn_attention_mfma.hpp"
+
+namespace dcn {
+namespace fa {
+namespace {
+
+template <typename T>
+constexpr bool kScaled = __is_same(T, _Float16);
+constexpr float kWeightLift = 1024.f;  // FP16: P's factor
+constexpr float kMostScaled = 32768.f;
+
+// The power of two that brings `top` into [2^12, 2^13).
+__device__ __forceinline__ float scale_for(float top) {
+    int e = 12 - ((int)(__builtin_bit_cast(uint32_t, top) >> 23 & 255) - 127);
+    e = e > 100 ? 100 : (e < -100 ? -100 : e);
+    return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
+}
+__device__ __forceinline__ float top_of(const f32x16& v) {
+    float t = fabsf(v[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) t = fmaxf(t, fabsf(v[r]));
+    return t;
+}
+
+// Lowers (or first sets) the factor of a lane's row or key where dS times it would leave FP16,
+// and its sums with it.
+template <int D>
+__device__ __forceinline__ void follow_scale(float top, float* up, f32x16* sum) {
+    top = both_max(top);
+    const bool change = top * *up > kMostScaled || (*up == 0.f && top > 0.f);
+    if (!__any(change)) return;
+    const float next = change ? scale_for(top) : *up, by = *up == 0.f ? 1.f : next / *up;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sum[n][x] *= by;
+    *up = next;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs a) {
+    constexpr int ROWS = 64, BYTES = ROWS * D * 2, MB = ROWS / 32;
+    using Ti = Tile<D>;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    Place pl;
+    if (!place_of<32 * kWaves>(a, 1, &pl)) return;
+    const Rows rw = rows_of(a.group);
+    const int last_row = pl.rows - 1;
+    const int w0 = pl.row0 + 32 * wave, w1 = w0 + 31 < last_row ? w0 + 31 : last_row;
+    const Spread all = spread_of(a, pl, rw, pl.row0, pl.row0 + 32 * kWaves - 1 < last_row ? pl.row0 + 32 * kWaves - 1 : last_row);
+    const bool idle = w0 > last_row;
+    const Spread mine = idle ? all : spread_of(a, pl, rw, w0, w1);
+    const int r = w0 + (lane & 31), rc = r < last_row ? r : last_row;
+    const Span sp = r <= last_row ? span_of(a, pl.offset + rw.token(r), pl.kv.count) : Span{0, 0, 0};
+    const int tok = rw.token(rc), head = pl.kh * a.group + (rc - tok * a.group);
+    const int64_t row = pl.q.first + tok, index = row * a.q_heads + head;
+    const TileList<ROWS> list(all);
+    const Keys<false> keys(a, pl.seq, pl.kh, pl.kv);
+    TilePages<D, ROWS, kWaves, false> none;
+    if (list.count) copy_tile<D, ROWS, kWaves, false>(keys, list.tile(0), none, lds[0][0], lds[0][1], wave, lane);
+    u32x4 q[D / 16], go[D / 16];
+    load_row<D>(q, a.q, a, pl, rw, r, lane);
+    load_row<D>(go, a.dout, a, pl, rw, r, lane);
+    float delta = 0.f;
+    {
+        u32x4 o[D / 16];
+        load_row<D>(o, a.o, a, pl, rw, r, lane);
+        typedef T vec __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const vec x = __builtin_bit_cast(vec, o[i]), y = __builtin_bit_cast(vec, go[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+        }
+        delta = both_sum(delta);
+    }
+    float lse = a.lse_in[index] * kLog2e;
+    if (lane < 32 && r <= last_row) ((float*)a.workspace)[index] = delta;
+    // Loaded: later waits for these registers would wait for the copies too.
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]), "+v"(go[i]));
+    asm volatile("" : "+v"(lse), "+v"(delta));
+    const float c = a.scale * kLog2e;
+    f32x16 sum[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sum[i][x] = 0.f;
+    float up = kScaled<T> ? 0.f : 1.f;  // FP16: dS's factor of this row; 0: no dS seen yet
+    for (int i = 0; i < list.count; ++i) {
+        char(*now)[BYTES] = lds[i & 1], (*other)[BYTES] = lds[(i & 1) ^ 1];
+        const int t0 = list.tile(i);
+        wait_copies<0>();
+        __syncthreads();
+        if (i + 1 < list.count) copy_tile<D, ROWS, kWaves, false>(keys, list.tile(i + 1), none, other[0], other[1], wave, lane);
+        bool bad = false;
+        if (!all_see<ROWS>(all, t0)) bad = __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads));
+        const bool active = !idle && !none_sees<ROWS>(mine, t0), whole = all_see<ROWS>(mine, t0);
+        u32x4 ds[2 * MB];
+        if (active) {
+            f32x16 t[MB];
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                f32x16 s, dp;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(now[0], mb, n, lane), q[n], s);
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(now[1], mb, n, lane), go[n], dp);
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    t[mb][x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - delta);
+                if (!whole) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x)
+                        t[mb][x] = sees(sp, t0 + 4 * (lane >> 5) + 32 * mb + 8 * (x >> 2) + (x & 3)) ? t[mb][x] : 0.f;
+                }
+            }
+            if constexpr (kScaled<T>) {
+                follow_scale<D>(fmaxf(top_of(t[0]), top_of(t[1])), &up, sum);
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) t[mb][x] *= up;
+            }
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                ds[2 * mb] = pack8<T>(t[mb], 0);
+                ds[2 * mb + 1] = pack8<T>(t[mb], 8);
+            }
+        }
+        if (bad) {  // some row does not see all of this tile, and a key in it is not finite
+            __syncthreads();
+            clean_tile<T, D, ROWS>(now[0], threadIdx.x, kThreads);
+            __syncthreads();
+        }
+        if (active) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+#pragma unroll
+                    for (int n = 0; n < D / 32; ++n) sum[n] = mma<T>(Ti::columns(now[0], mb, st, n, lane), ds[2 * mb + st], sum[n]);
+            if (bad)
+                add_nonfinite<T, D>(sum, sp, t0, keys.end(t0 + ROWS), 0, lane,
+                                    [&](int j) { return (const uint16_t*)(keys.kp + (int64_t)j * keys.k.ts * 2); });
+        }
+    }
+    if (r > last_row) return;
+    const float f = up == 0.f ? 0.f : a.scale / up;
+    T* to = (T*)a.dq.p + row * a.dq.ts + head * a.dq.hs + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            typedef T four __attribute__((ext_vector_type(4)));
+            four v;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) v[b] = narrow<T>(sum[i][4 * x + b] * f);
+            *(four*)(to + 32 * i + 8 * x) = v;
+        }
+}
+
+// How the key blocks (128 keys) share out their query tiles: the first `sink_blocks` hold keys
+// that every later query sees, and are cut into more parts than the others.
+struct KeyPlan {
+    int blocks, sink_blocks, parts, sink_parts;
+    __host__ __device__ int items() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * parts; }
+    __host__ __device__ void item(int i, int* block, int* part, int* of) const {
+        if (i < sink_blocks * sink_parts) {
+            *block = i / sink_parts;
+            *part = i % sink_parts;
+            *of = sink_parts;
+        } else {
+            i -= sink_blocks * sink_parts;
+            *block = sink_blocks + i / parts;
+            *part = i % parts;
+            *of = parts;
+        }
+    }
+};
+constexpr int kKeys = 32 * kWaves;
+
+// Positions that see key j: [from, to), and from `from` on without an end for a sink.
+struct Seen {
+    int from, to;
+};
+__device__ __forceinline__ Seen seen_of(const AttentionArgs& a, int j, int n) {
+    const int64_t f = j / a.frame, fr = a.frame;
+    int64_t from = a.ahead < 0 ? 0 : (f - a.ahead) * fr, to = a.back < 0 || f < a.sinks ? n : (f + a.back + 1) * fr;
+    from = from < 0 ? 0 : (from > n ? n : from);
+    to = to > n ? n : to;
+    return Seen{(int)from, (int)to};
+}
+
+// Positions that see all keys j .. to: `from` grows with the key, and so does `to` past the
+// sinks, whose `to` is n.
+__device__ __forceinline__ Seen all_seen_of(const AttentionArgs& a, int j, int to, int n) {
+    const int64_t sinks = (int64_t)a.sinks * a.frame;
+    return Seen{seen_of(a, to, n).from, seen_of(a, j < sinks && sinks <= to ? (int)sinks : j, n).to};
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttentionArgs a, KeyPlan plan, float* parts) {
+    constexpr int ROWS = 64, BYTES = ROWS * D * 2, MB = ROWS / 32;
+    using Ti = Tile<D>;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
+    __shared__ __attribute__((aligned(16))) int row_at[2][ROWS];  // a row's position; -1: no row
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    int block, part, of;
+    plan.item(blockIdx.x, &block, &part, &of);
+    Place pl;
+    pl.seq = blockIdx.z;
+    pl.kh = blockIdx.y;
+    pl.q = run_of(a.cu_q, pl.seq, a.max_q, a.q_tokens);
+    pl.kv = run_of(a.cu_kv, pl.seq, a.max_kv, a.kv_tokens);
+    pl.q.count = uniform(pl.q.count);
+    pl.kv.count = uniform(pl.kv.count);
+    pl.offset = pl.kv.count - pl.q.count;
+    pl.rows = (pl.q.count < a.max_q ? pl.q.count : a.max_q) * a.group;
+    const int k0 = block * kKeys, nk = pl.kv.count;
+    if (k0 >= nk) return;
+    const Rows rw = rows_of(a.group);
+    // The wave's keys, as B operands (past the end: the last key's; their sums are not stored).
+    const int j = k0 + 32 * wave + (lane & 31), jc = j < nk ? j : nk - 1;
+    u32x4 k[D / 16], v[D / 16];
+    {
+        const char* kp = (const char*)a.k.p + ((pl.kv.first + jc) * a.k.ts + pl.kh * a.k.hs + 8 * (lane >> 5)) * 2;
+        const char* vp = (const char*)a.v.p + ((pl.kv.first + jc) * a.v.ts + pl.kh * a.v.hs + 8 * (lane >> 5)) * 2;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            k[i] = *(const u32x4*)(kp + i * 32);
+            v[i] = *(const u32x4*)(vp + i * 32);
+        }
+    }
+    const Seen me = seen_of(a, jc, nk);
+    // Positions that see some key of the block; all of them; all keys of the wave.
+    const int kl = k0 + kKeys - 1 < nk ? k0 + kKeys - 1 : nk - 1;
+    const int wf = k0 + 32 * wave < nk ? k0 + 32 * wave : nk - 1, wl = wf + 31 < nk ? wf + 31 : nk - 1;
+    const Seen first = seen_of(a, k0, nk), last = seen_of(a, kl, nk);
+    const Seen every = all_seen_of(a, k0, kl, nk), wave_every = all_seen_of(a, wf, wl, nk);
+    // A sink's `to` is n: the largest `to` of a run of keys is that of its first or its last.
+    int t_from = first.from - pl.offset, t_to = (first.to > last.to ? first.to : last.to) - pl.offset;
+    t_from = t_from < 0 ? 0 : t_from;
+    const int q_rows = pl.rows;
+    const int64_t r_to = (int64_t)t_to * a.group;
+    const int tile_from = (int)((int64_t)t_from * a.group / ROWS), end = r_to < q_rows ? (int)(r_to < 0 ? 0 : r_to) : q_rows;
+    const int tile_to = (end + ROWS - 1) / ROWS;
+    const int tiles = tile_to > tile_from ? tile_to - tile_from : 0;
+    const int per = (tiles + of - 1) / of;
+    const int begin = tile_from + part * per, stop = begin + per < tile_to ? begin + per : tile_to;
+
+    // Copies of the query tile at packed row r0, and its rows' lse, delta and positions.
+    auto copy = [&](int r0, char* to_q, char* to_do) {
+#pragma unroll
+        for (int n = 0; n < ROWS / Ti::kRowsPerCopy / kWaves; ++n) {
+            const int i = n * kWaves + wave, in = Ti::copy_row(i, lane), c = Ti::copy_channel(in, lane);
+            const int r = r0 + in < q_rows ? r0 + in : q_rows - 1;
+            const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+            const int64_t row = pl.q.first + tok;
+            copy16((const char*)a.q.p + (row * a.q.ts + head * a.q.hs + c) * 2, to_q + i * 1024);
+            copy16((const char*)a.dout.p + (row * a.dout.ts + head * a.dout.hs + c) * 2, to_do + i * 1024);
+        }
+    };
+    float next_lse = 0.f, next_delta = 0.f;
+    int next_at = -1;
+    auto fetch = [&](int r0) {
+        if (threadIdx.x >= ROWS) return;
+        const int r = r0 + (int)threadIdx.x;
+        next_at = -1;
+        if (r >= q_rows) return;
+        const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+        const int64_t index = (pl.q.first + tok) * a.q_heads + head;
+        next_lse = a.lse_in[index] * kLog2e;
+        next_delta = ((const float*)a.workspace)[index];
+        next_at = pl.offset + tok;
+    };
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) dk[i][x] = dv[i][x] = 0.f;
+    const float c = a.scale * kLog2e;
+    float up = kScaled<T> ? 0.f : 1.f;  // FP16: dS's factor of this key; 0: no dS seen yet
+    if (begin < stop) {
+        fetch(begin * ROWS);
+        copy(begin * ROWS, lds[0][0], lds[0][1]);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(k[i]), "+v"(v[i]));
+    for (int i = begin; i < stop; ++i) {
+        const int buf = (i - begin) & 1, r0 = i * ROWS;
+        char *qt = lds[buf][0], *ot = lds[buf][1];
+        if (threadIdx.x < ROWS) {
+            row_lse[buf][threadIdx.x] = next_lse;
+            row_delta[buf][threadIdx.x] = next_delta;
+            row_at[buf][threadIdx.x] = next_at;
+        }
+        wait_copies<0>();
+        __syncthreads();
+        if (i + 1 < stop) {
+            fetch(r0 + ROWS);
+            copy(r0 + ROWS, lds[buf ^ 1][0], lds[buf ^ 1][1]);
+        }
+        // Positions of the tile's first and last row; whether this wave's keys are seen by all of them.
+        const int rl = r0 + ROWS - 1 < q_rows ? r0 + ROWS - 1 : q_rows - 1;
+        const int p0 = pl.offset + rw.token(r0), p1 = pl.offset + rw.token(rl);
+        const bool rows_there = r0 + ROWS <= q_rows && p0 >= 0;
+        const bool whole = rows_there && p0 >= wave_every.from && p1 < wave_every.to;
+        const bool block_whole = rows_there && p0 >= every.from && p1 < every.to;
+        bool bad = false;
+        if (!block_whole)
+            bad = __syncthreads_or((int)tile_nonfinite<T, D, ROWS>(qt, threadIdx.x, kThreads) |
+                                   (int)tile_nonfinite<T, D, ROWS>(ot, threadIdx.x, kThreads));
+        u32x4 p16[2 * MB], ds[2 * MB];
+        f32x16 t[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(qt, mb, n, lane), k[n], s);
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(ot, mb, n, lane), v[n], dp);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * mb + 8 * g + 4 * (lane >> 5);
+                const f32x4 l4 = *(const f32x4*)&row_lse[buf][at], d4 = *(const f32x4*)&row_delta[buf][at];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int x = 4 * g + b;
+                    s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[b]));
+                    t[mb][x] = s[x] * (dp[x] - d4[b]);
+                }
+                if (!whole) {
+                    typedef int i32x4 __attribute__((ext_vector_type(4)));
+                    const i32x4 p4 = *(const i32x4*)&row_at[buf][at];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const bool on = p4[b] >= me.from && p4[b] < me.to && p4[b] >= 0;
+                        s[4 * g + b] = on ? s[4 * g + b] : 0.f;
+                        t[mb][4 * g + b] = on ? t[mb][4 * g + b] : 0.f;
+                    }
+                }
+            }
+            if constexpr (kScaled<T>) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[x] *= kWeightLift;
+            }
+            p16[2 * mb] = pack8<T>(s, 0);
+            p16[2 * mb + 1] = pack8<T>(s, 8);
+        }
+        if constexpr (kScaled<T>) {
+            follow_scale<D>(fmaxf(top_of(t[0]), top_of(t[1])), &up, dk);
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) t[mb][x] *= up;
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            ds[2 * mb] = pack8<T>(t[mb], 0);
+            ds[2 * mb + 1] = pack8<T>(t[mb], 8);
+        }
+        if (bad) {  // some pair of the tile is not visible, and a query or a gradient in it is not finite
+            __syncthreads();
+            clean_tile<T, D, ROWS>(qt, threadIdx.x, kThreads);
+            clean_tile<T, D, ROWS>(ot, threadIdx.x, kThreads);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int n = 0; n < D / 32; ++n) {
+                    dv[n] = mma<T>(Ti::columns(ot, mb, st, n, lane), p16[2 * mb + st], dv[n]);
+                    dk[n] = mma<T>(Ti::columns(qt, mb, st, n, lane), ds[2 * mb + st], dk[n]);
+                }
+        if (bad) {
+            for (int x = 0; x < ROWS; ++x) {
+                const int at = row_at[buf][x];
+                if (at < 0) continue;
+                const bool on = at >= me.from && at < me.to;
+                const int r = r0 + x, tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
+                const int64_t row = pl.q.first + tok;
+                add_nonfinite<T, D>(dk, (const uint16_t*)a.q.p + row * a.q.ts + head * a.q.hs, on, lane);
+                add_nonfinite<T, D>(dv, (const uint16_t*)a.dout.p + row * a.dout.ts + head * a.dout.hs, on, lane);
+            }
+        }
+    }
+    const float fk = up == 0.f ? 0.f : a.scale / up, fv = kScaled<T> ? 1.f / kWeightLift : 1.f;
+    if (of > 1) {
+        // [item][dk, dv][key][D] FP32, in order of the parts
+        const int64_t item = ((int64_t)pl.seq * a.kv_heads + pl.kh) * plan.items() + blockIdx.x;
+        float* to = parts + ((item * 2) * kKeys + 32 * wave + (lane & 31)) * D + 4 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                *(f32x4*)(to + 32 * i + 8 * x) = f32x4{dk[i][4 * x] * fk, dk[i][4 * x + 1] * fk, dk[i][4 * x + 2] * fk, dk[i][4 * x + 3] * fk};
+                *(f32x4*)(to + kKeys * D + 32 * i + 8 * x) =
+                    f32x4{dv[i][4 * x] * fv, dv[i][4 * x + 1] * fv, dv[i][4 * x + 2] * fv, dv[i][4 * x + 3] * fv};
+            }
+        return;
+    }
+    if (j >= nk) return;
+    T* to_k = (T*)a.dk.p + (pl.kv.first + j) * a.dk.ts + pl.kh * a.dk.hs + 4 * (lane >> 5);
+    T* to_v = (T*)a.dv.p + (pl.kv.first + j) * a.dv.ts + pl.kh * a.dv.hs + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            typedef T four __attribute__((ext_vector_type(4)));
+            four vk, vv;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                vk[b] = narrow<T>(dk[i][4 * x + b] * fk);
+                vv[b] = narrow<T>(dv[i][4 * x + b] * fv);
+            }
+            *(four*)(to_k + 32 * i + 8 * x) = vk;
+            *(four*)(to_v + 32 * i + 8 * x) = vv;
+        }
+}
+
+// The parts of one key block's gradients, in order; four channels a thread.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void attention_dkv_join_kernel(AttentionArgs a, KeyPlan plan, const float* parts, int from_block) {
+    const Run kv = run_of(a.cu_kv, blockIdx.z, a.max_kv, a.kv_tokens);
+    constexpr int per = kThreads * 4 / D, groups = kKeys / per;  // keys of one workgroup
+    const int block = from_block + blockIdx.x / groups, key = (blockIdx.x % groups) * per + threadIdx.x / (D / 4);
+    const int j = block * kKeys + key, at = threadIdx.x % (D / 4) * 4;
+    if (j >= kv.count) return;
+    const int of = block < plan.sink_blocks ? plan.sink_parts : plan.parts;
+    const int first = block < plan.sink_blocks ? block * plan.sink_parts
+                                               : plan.sink_blocks * plan.sink_parts + (block - plan.sink_blocks) * plan.parts;
+    const int64_t item = ((int64_t)blockIdx.z * a.kv_heads + blockIdx.y) * plan.items() + first;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < of; ++p) {
+            const f32x4 x = *(const f32x4*)(parts + (((item + p) * 2 + which) * kKeys + key) * D + at);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) sum[b] += x[b];
+        }
+        typedef T four __attribute__((ext_vector_type(4)));
+        four v;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[b] = narrow<T>(sum[b]);
+        const HeadsOut& h = which ? a.dv : a.dk;
+        *(four*)((T*)h.p + (kv.first + j) * h.ts + blockIdx.y * h.hs + at) = v;
+    }
+}
+
+KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, int frame, int back, int ahead, int sinks) {
+    KeyPlan p;
+    p.blocks = (max_kv + kKeys - 1) / kKeys;
+    const int64_t all = ((int64_t)max_q * group + 63) / 64;
+    // Query tiles of a block: those of its window, or all.
+    int64_t tiles = all;
+    p.sink_blocks = 0;
+    if (back >= 0) {
+        const int64_t frames = (int64_t)back + 1 + (ahead < 0 ? 0 : ahead) + (kKeys + frame - 1) / frame;
+        const int64_t window = ahead < 0 ? all : (frames * frame * group + 63) / 64 + 1;
+        tiles = window < all ? window : all;
+        const int64_t keys = (int64_t)sinks * frame < max_kv ? (int64_t)sinks * frame : max_kv;
+        if (tiles < all) p.sink_blocks = (int)((keys + kKeys - 1) / kKeys);
+    }
+    // A workgroup a CU where the blocks alone do not give it, of eight tiles at least.
+    const int64_t groups = (int64_t)p.blocks * kv_heads * sequences;
+    int64_t parts = groups > 0 ? 256 / groups : 1;
+    if (parts > tiles / 8) parts = tiles / 8;
+    p.parts = (int)(parts < 1 ? 1 : parts);
+    // A sink block's parts are about as long as another block's.
+    const int64_t each = (tiles + p.parts - 1) / p.parts;
+    const int64_t sink_parts = each > 0 ? (all + each - 1) / each : 1;
+    p.sink_parts = p.sink_blocks ? (int)(sink_parts < p.parts ? p.parts : (sink_parts > 256 ? 256 : sink_parts)) : p.parts;
+    return p;
+}
+
+template <typename T, int D>
+hipError_t run(const AttentionArgs& a, const KeyPlan& p, hipStream_t stream) {
+    if (a.max_q > 0) {
+        const int64_t rows = (int64_t)a.max_q * a.group;
+        attention_dq_kernel<T, D><<<dim3((unsigned)((rows + 127) / 128), a.kv_heads, a.sequences), kThreads, 0, stream>>>(a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    if (a.max_kv <= 0) return hipSuccess;
+    float* parts = (float*)a.workspace + ((a.q_tokens * a.q_heads + 3) & ~INT64_C(3));
+    attention_dkv_kernel<T, D><<<dim3((unsigned)p.items(), a.kv_heads, a.sequences), kThreads, 0, stream>>>(a, p, parts);
+    if (hipError_t e = hipGetLastError()) return e;
+    const int joined = p.parts > 1 ? p.blocks : (p.sink_parts > 1 ? p.sink_blocks : 0);
+    if (!joined) return hipSuccess;
+    attention_dkv_join_kernel<T, D><<<dim3((unsigned)joined * (kKeys * D / (kThreads * 4)), a.kv_heads, a.sequences), kThreads, 0, stream>>>(a, p, parts, 0);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t by_dim(const AttentionArgs& a, const KeyPlan& p, hipStream_t stream) {
+    return a.dim == 64 ? run<T, 64>(a, p, stream) : run<T, 128>(a, p, stream);
+}
+
+}  // namespace
+}  // namespace fa
+
+size_t attention_backward_workspace(const dcn_attention_shape& s) {
+    const fa::KeyPlan p = fa::key_plan(s.sequences, s.kv_heads, s.q_heads / s.kv_heads, s.max_q, s.max_kv, s.frame_tokens, s.back,
+                                       s.ahead, s.sinks);
+    size_t n = ((size_t)s.q_tokens * s.q_heads + 3) & ~(size_t)3;
+    if (p.parts > 1 || p.sink_parts > 1)
+        n += (size_t)s.sequences * s.kv_heads * p.items() * 2 * fa::kKeys * s.head_dim;
+    return n * sizeof(float);
+}
+
+hipError_t launch_attention_matrix_backward(int dtype, const AttentionArgs& a, hipStream_t stream) {
+    const fa::KeyPlan p = fa::key_plan(a.sequences, a.kv_heads, a.group, a.max_q, a.max_kv, a.frame, a.back, a.ahead, a.sinks);
+    return dtype == DCN_DTYPE_F16 ? fa::by_dim<_Float16>(a, p, stream) : fa::by_dim<fa::bf16>(a, p, stream);
+}
+
+}  // namespace dcn
