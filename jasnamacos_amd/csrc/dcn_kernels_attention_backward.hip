@@ -21,6 +21,7 @@ template <typename T>
 constexpr bool kScaled = __is_same(T, _Float16);
 constexpr float kWeightLift = 1024.f;  // FP16: P's factor
 constexpr float kMostScaled = 32768.f;
+constexpr int kFewKeys = 256;
 
 // The power of two that brings `top` into [2^12, 2^13).
 __device__ __forceinline__ float scale_for(float top) {
@@ -50,9 +51,14 @@ __device__ __forceinline__ void follow_scale(float top, float* up, f32x16* sum) 
     *up = next;
 }
 
+// Keys of a tile of the first pass: with 128 channels a wave's operands and sums leave registers
+// for 32 keys' dS.
+template <int D>
+constexpr int kDqKeys = D == 64 ? 64 : 32;
+
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs a) {
-    constexpr int ROWS = 64, BYTES = ROWS * D * 2, MB = ROWS / 32;
+    constexpr int ROWS = kDqKeys<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -89,7 +95,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
         delta = both_sum(delta);
     }
     float lse = a.lse_in[index] * kLog2e;
-    if (lane < 32 && r <= last_row) ((float*)a.workspace)[index] = delta;
+    // delta from the rounded out is off by a rounding's share of it, 1 / sqrt(keys) of what dS's
+    // own rounding costs. Rows of few keys take it from P and dP instead, in a pass of its own.
+    const bool sum_delta = list.count * ROWS <= kFewKeys;
+    if (!sum_delta && lane < 32 && r <= last_row) ((float*)a.workspace)[index] = delta;
     // Loaded: later waits for these registers would wait for the copies too.
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]), "+v"(go[i]));
@@ -101,14 +110,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
 #pragma unroll
         for (int x = 0; x < 16; ++x) sum[i][x] = 0.f;
     float up = kScaled<T> ? 0.f : 1.f;  // FP16: dS's factor of this row; 0: no dS seen yet
-    for (int i = 0; i < list.count; ++i) {
-        char(*now)[BYTES] = lds[i & 1], (*other)[BYTES] = lds[(i & 1) ^ 1];
+    float exact_delta = 0.f;
+    if (sum_delta) delta = 0.f;
+    const int steps = sum_delta ? 2 * list.count : list.count;
+    for (int step = 0, i = 0; step < steps; ++step, i = i + 1 < list.count ? i + 1 : 0) {
+        char(*now)[BYTES] = lds[step & 1], (*other)[BYTES] = lds[(step & 1) ^ 1];
         const int t0 = list.tile(i);
         wait_copies<0>();
         __syncthreads();
-        if (i + 1 < list.count) copy_tile<D, ROWS, kWaves, false>(keys, list.tile(i + 1), none, other[0], other[1], wave, lane);
+        if (step + 1 < steps)
+            copy_tile<D, ROWS, kWaves, false>(keys, list.tile(i + 1 < list.count ? i + 1 : 0), none, other[0], other[1], wave, lane);
+        const bool delta_step = sum_delta && step < list.count;
         bool bad = false;
-        if (!all_see<ROWS>(all, t0)) bad = __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads));
+        if (!delta_step && !all_see<ROWS>(all, t0))
+            bad = __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads));
         const bool active = !idle && !none_sees<ROWS>(mine, t0), whole = all_see<ROWS>(mine, t0);
         u32x4 ds[2 * MB];
         if (active) {
@@ -131,8 +146,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
                         t[mb][x] = sees(sp, t0 + 4 * (lane >> 5) + 32 * mb + 8 * (x >> 2) + (x & 3)) ? t[mb][x] : 0.f;
                 }
             }
+            if (delta_step) {
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) exact_delta += t[mb][x];
+            } else {
             if constexpr (kScaled<T>) {
-                follow_scale<D>(fmaxf(top_of(t[0]), top_of(t[1])), &up, sum);
+                follow_scale<D>(MB == 1 ? top_of(t[0]) : fmaxf(top_of(t[0]), top_of(t[MB - 1])), &up, sum);
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -143,6 +164,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
                 ds[2 * mb] = pack8<T>(t[mb], 0);
                 ds[2 * mb + 1] = pack8<T>(t[mb], 8);
             }
+            }
+        }
+        if (delta_step) {
+            if (i + 1 == list.count) delta = both_sum(exact_delta);
+            continue;
         }
         if (bad) {  // some row does not see all of this tile, and a key in it is not finite
             __syncthreads();
@@ -162,6 +188,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
         }
     }
     if (r > last_row) return;
+    if (sum_delta && lane < 32) ((float*)a.workspace)[index] = delta;
     const float f = up == 0.f ? 0.f : a.scale / up;
     T* to = (T*)a.dq.p + row * a.dq.ts + head * a.dq.hs + 4 * (lane >> 5);
 #pragma unroll
