@@ -242,9 +242,53 @@ __device__ __forceinline__ Seen all_seen_of(const AttentionArgs& a, int j, int t
     return Seen{seen_of(a, to, n).from, seen_of(a, j < sinks && sinks <= to ? (int)sinks : j, n).to};
 }
 
+template <int D>
+constexpr int kDkvRows = 64;
+
+// P (16 bits, FP16 lifted) and dS of a query tile's rows (registers) and a wave's keys (lanes).
+// MASKED: some row may not see some key.
+template <typename T, int D, int MB, bool MASKED>
+__device__ __forceinline__ void weights_of(const char* qt, const char* ot, const u32x4* k, const u32x4* v, const float* lse,
+                                           const float* delta, const int* at, float c, const Seen& me, int lane, u32x4* p16,
+                                           f32x16* t) {
+    using Ti = Tile<D>;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(qt, mb, n, lane), k[n], s);
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(ot, mb, n, lane), v[n], dp);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const int in = 32 * mb + 8 * g + 4 * (lane >> 5);
+            const f32x4 l4 = *(const f32x4*)(lse + in), d4 = *(const f32x4*)(delta + in);
+            i32x4 p4;
+            if constexpr (MASKED) p4 = *(const i32x4*)(at + in);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int x = 4 * g + b;
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[b]));
+                t[mb][x] = s[x] * (dp[x] - d4[b]);
+                if constexpr (MASKED) {
+                    const bool on = p4[b] >= me.from && p4[b] < me.to && p4[b] >= 0;
+                    s[x] = on ? s[x] : 0.f;
+                    t[mb][x] = on ? t[mb][x] : 0.f;
+                }
+                if constexpr (kScaled<T>) s[x] *= kWeightLift;
+            }
+        }
+        p16[2 * mb] = pack8<T>(s, 0);
+        p16[2 * mb + 1] = pack8<T>(s, 8);
+    }
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttentionArgs a, KeyPlan plan, float* parts) {
-    constexpr int ROWS = 64, BYTES = ROWS * D * 2, MB = ROWS / 32;
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a, KeyPlan plan, float* parts) {
+    constexpr int ROWS = kDkvRows<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
@@ -357,45 +401,12 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttentionArg
                                    (int)tile_nonfinite<T, D, ROWS>(ot, threadIdx.x, kThreads));
         u32x4 p16[2 * MB], ds[2 * MB];
         f32x16 t[MB];
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            f32x16 s, dp;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(qt, mb, n, lane), k[n], s);
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(ot, mb, n, lane), v[n], dp);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = 32 * mb + 8 * g + 4 * (lane >> 5);
-                const f32x4 l4 = *(const f32x4*)&row_lse[buf][at], d4 = *(const f32x4*)&row_delta[buf][at];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int x = 4 * g + b;
-                    s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[b]));
-                    t[mb][x] = s[x] * (dp[x] - d4[b]);
-                }
-                if (!whole) {
-                    typedef int i32x4 __attribute__((ext_vector_type(4)));
-                    const i32x4 p4 = *(const i32x4*)&row_at[buf][at];
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const bool on = p4[b] >= me.from && p4[b] < me.to && p4[b] >= 0;
-                        s[4 * g + b] = on ? s[4 * g + b] : 0.f;
-                        t[mb][4 * g + b] = on ? t[mb][4 * g + b] : 0.f;
-                    }
-                }
-            }
-            if constexpr (kScaled<T>) {
-#pragma unroll
-                for (int x = 0; x < 16; ++x) s[x] *= kWeightLift;
-            }
-            p16[2 * mb] = pack8<T>(s, 0);
-            p16[2 * mb + 1] = pack8<T>(s, 8);
-        }
+        if (whole)
+            weights_of<T, D, MB, false>(qt, ot, k, v, row_lse[buf], row_delta[buf], row_at[buf], c, me, lane, p16, t);
+        else
+            weights_of<T, D, MB, true>(qt, ot, k, v, row_lse[buf], row_delta[buf], row_at[buf], c, me, lane, p16, t);
         if constexpr (kScaled<T>) {
-            follow_scale<D>(fmaxf(top_of(t[0]), top_of(t[1])), &up, dk);
+            follow_scale<D>(MB == 1 ? top_of(t[0]) : fmaxf(top_of(t[0]), top_of(t[MB - 1])), &up, dk);
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb)
 #pragma unroll

@@ -81,19 +81,51 @@ __device__ __forceinline__ float with_low(float rounded, uint16_t low) {
         return fmaf((float)__builtin_bit_cast(_Float16, low), 1.f / 2048.f, rounded);
 }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void add_low(const NormArgs& a, int64_t base, int at, float* v) {
-    const uint16_t* from = (const uint16_t*)((const char*)a.low + norm_low_header(a.tokens)) + base + at;
-    if constexpr (WIDE) {
-        if (at >= a.channels) return;
-        const Pack<uint16_t> p = *(const Pack<uint16_t>*)from;
+// A lane's channels of one row's tensors, as they are stored: loaded a row ahead.
+template <typename T, int NV>
+struct RawRow {
+    Pack<T> dy[NV], x_out[NV], dx_out[NV], h[NV];
+    Pack<uint16_t> low[NV];
+    float r1, r2, low1, low2;
+
+    template <bool WIDE, typename U>
+    static __device__ __forceinline__ void get(const U* from, int at, int channels, Pack<U>* to) {
+        if constexpr (WIDE) {
+            if (at < channels) *to = *(const Pack<U>*)(from + at);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = with_low<T>(v[i], p.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-            if (at + i < a.channels) v[i] = with_low<T>(v[i], from[i]);
+            for (int i = 0; i < kVec; ++i)
+                if (at + i < channels) to->v[i] = from[at + i];
+        }
     }
+    template <int LANES, bool WIDE>
+    __device__ __forceinline__ void load(const NormArgs& a, int64_t row, int lane) {
+        const int64_t base = row * a.channels;
+        const int c = a.channels;
+        r1 = a.rstd[row * 2];
+        r2 = a.rstd[row * 2 + 1];
+        if (sizeof(T) == 2 && a.low) {
+            low1 = ((const float*)a.low)[row * 2];
+            low2 = ((const float*)a.low)[row * 2 + 1];
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int at = (n * LANES + lane) * kVec;
+            if (a.dy) {
+                get<WIDE>((const T*)a.dy + base, at, c, &dy[n]);
+                get<WIDE>((const T*)a.x_out + base, at, c, &x_out[n]);
+                if (sizeof(T) == 2 && a.low)
+                    get<WIDE>((const uint16_t*)((const char*)a.low + norm_low_header(a.tokens)) + base, at, c, &low[n]);
+            }
+            get<WIDE>((const T*)a.dx_out + base, at, c, &dx_out[n]);
+            get<WIDE>((const T*)a.h + base, at, c, &h[n]);
+        }
+    }
+};
+// Channel i of a lane's chunk at `at`, zero past the row's end.
+template <typename T>
+__device__ __forceinline__ float raw(const Pack<T>& p, int i, int at, int channels) {
+    return at + i < channels ? widen(p.v[i]) : 0.f;
 }
 
 // The sum over a row's LANES lanes, in every one of them.
@@ -219,7 +251,21 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a, Cut
     __shared__ float sums[kThreads * kVec];
     constexpr int slots = kThreads / LANES;
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, c = a.channels;
-    float dw1[NV][kVec] = {}, dw2[NV][kVec] = {};
+    // One vector a lane: weights and gates stay in registers; more: they come from the cache each row.
+    constexpr bool keep = NV == 1;
+    float dw1[NV][kVec] = {}, dw2[NV][kVec] = {}, w1[keep ? NV : 1][kVec], w2[keep ? NV : 1][kVec], g[keep ? NV : 1][kVec];
+    auto factor = [&](const T* row, int n, float* to) {
+        if (row) {
+            load_row<T, WIDE>(row, (n * LANES + lane) * kVec, c, 0.f, to);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) to[i] = 1.f;
+        }
+    };
+    if constexpr (keep) {
+        factor((const T*)a.w_post, 0, w1[0]);
+        factor((const T*)a.w_pre, 0, w2[0]);
+    }
     for (int64_t unit = (int64_t)blockIdx.x * slots + slot; unit < cut.units; unit += (int64_t)gridDim.x * slots) {
         const int64_t gate = unit / cut.per_gate, first = gate * a.gate_tokens;
         const int64_t from = first + (unit - gate * cut.per_gate) * cut.rows;
@@ -227,26 +273,35 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a, Cut
         to = to > first + a.gate_tokens ? first + a.gate_tokens : to;
         to = to > a.tokens ? a.tokens : to;
         float dg[NV][kVec] = {};
+        const T* gates = a.gate ? (const T*)a.gate + gate * c : nullptr;
+        if constexpr (keep) factor(gates, 0, g[0]);
+        // Short rows are loaded a row ahead; a long one alone has enough bytes in flight.
+        constexpr bool ahead = NV == 1;
+        RawRow<T, NV> now, next;
+        if (ahead && from < to) next.template load<LANES, WIDE>(a, from, lane);
         for (int64_t row = from; row < to; ++row) {
             const int64_t base = row * c;
-            const float r1 = a.rstd[row * 2], r2 = a.rstd[row * 2 + 1];
+            if constexpr (ahead) {
+                now = next;
+                if (row + 1 < to) next.template load<LANES, WIDE>(a, row + 1, lane);
+            } else {
+                now.template load<LANES, WIDE>(a, row, lane);
+            }
             float t[NV][kVec], m[NV][kVec], sum = 0.f;
-            const float* head = (const float*)a.low + row * 2;
-            const bool whole = sizeof(T) == 2 && a.low && head[0] == r1 && head[1] == r2;
             if (a.dy) {
+                const bool whole = sizeof(T) == 2 && a.low && now.low1 == now.r1 && now.low2 == now.r2;
 #pragma unroll
                 for (int n = 0; n < NV; ++n) {
                     const int at = (n * LANES + lane) * kVec;
-                    float w[kVec];
-                    load_row<T, WIDE>((const T*)a.dy + base, at, c, 0.f, t[n]);
-                    load_row<T, WIDE>((const T*)a.x_out + base, at, c, 0.f, m[n]);
-                    if (whole) add_low<T, WIDE>(a, base, at, m[n]);
-                    if (a.w_pre) load_row<T, WIDE>((const T*)a.w_pre, at, c, 0.f, w);
+                    if constexpr (!keep) factor((const T*)a.w_pre, n, w2[0]);
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) {
-                        m[n][i] *= r2;
+                        t[n][i] = raw(now.dy[n], i, at, c);
+                        float x = raw(now.x_out[n], i, at, c);
+                        if (sizeof(T) == 2 && whole && at + i < c) x = with_low<T>(x, now.low[n].v[i]);
+                        m[n][i] = x * now.r2;
                         dw2[n][i] = fmaf(t[n][i], m[n][i], dw2[n][i]);
-                        if (a.w_pre) t[n][i] *= w[i];
+                        t[n][i] *= w2[keep ? n : 0][i];
                         sum = fmaf(t[n][i], m[n][i], sum);
                     }
                 }
@@ -254,27 +309,30 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a, Cut
 #pragma unroll
                 for (int n = 0; n < NV; ++n)
 #pragma unroll
-                    for (int i = 0; i < kVec; ++i) t[n][i] = r2 * fmaf(-mean, m[n][i], t[n][i]);
+                    for (int i = 0; i < kVec; ++i) t[n][i] = now.r2 * fmaf(-mean, m[n][i], t[n][i]);
             }
             sum = 0.f;
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
                 const int at = (n * LANES + lane) * kVec;
-                float w[kVec], g[kVec], d[kVec];
-                load_row<T, WIDE>((const T*)a.dx_out + base, at, c, 0.f, d);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) t[n][i] = a.dy ? t[n][i] + d[i] : d[i];
-                store_row<T, WIDE>((T*)a.dx + base, at, c, t[n]);
-                load_row<T, WIDE>((const T*)a.h + base, at, c, 0.f, m[n]);
-                if (a.w_post) load_row<T, WIDE>((const T*)a.w_post, at, c, 0.f, w);
-                if (a.gate) load_row<T, WIDE>((const T*)a.gate + gate * c, at, c, 0.f, g);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    m[n][i] *= r1;
-                    const float at_ = a.alpha * t[n][i], wi = a.w_post ? w[i] : 1.f, gi = a.gate ? g[i] : 1.f;
-                    dg[n][i] = fmaf(at_ * wi, m[n][i], dg[n][i]);
-                    dw1[n][i] = fmaf(at_ * gi, m[n][i], dw1[n][i]);
-                    t[n][i] = at_ * gi * wi;
+                    const float d = raw(now.dx_out[n], i, at, c);
+                    t[n][i] = a.dy ? t[n][i] + d : d;
+                }
+                store_row<T, WIDE>((T*)a.dx + base, at, c, t[n]);
+                if constexpr (!keep) {
+                    factor((const T*)a.w_post, n, w1[0]);
+                    factor(gates, n, g[0]);
+                }
+                const float *w = w1[keep ? n : 0], *gt = g[keep ? n : 0];
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    m[n][i] = raw(now.h[n], i, at, c) * now.r1;
+                    const float s = a.alpha * t[n][i];
+                    dg[n][i] = fmaf(s * w[i], m[n][i], dg[n][i]);
+                    dw1[n][i] = fmaf(s * gt[i], m[n][i], dw1[n][i]);
+                    t[n][i] = s * gt[i] * w[i];
                     sum = fmaf(t[n][i], m[n][i], sum);
                 }
             }
@@ -282,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a, Cut
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) t[n][i] = r1 * fmaf(-mean, m[n][i], t[n][i]);
+                for (int i = 0; i < kVec; ++i) t[n][i] = now.r1 * fmaf(-mean, m[n][i], t[n][i]);
                 store_row<T, WIDE>((T*)a.dh + base, (n * LANES + lane) * kVec, c, t[n]);
             }
         }
@@ -319,37 +377,50 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a, Cut
     }
 }
 
-// out[row][channel] = the sum over `count` parts, four partial sums a thread: a workgroup
-// adds 64 channels of one row, its waves taking parts in turn.
+// out[channel] = the sum over `count` parts of a row, for 64 channels a workgroup: 16 threads
+// have four channels each, 64 groups of them take parts in turn and are added in their order.
+constexpr int kJoinThreads = 1024;
 template <typename T>
-__device__ __forceinline__ void add_parts(const float* parts, int64_t count, int c, T* out) {
-    __shared__ float sums[kThreads];
-    const int at = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
-    float s = 0.f;
-    if (at < c)
-        for (int64_t p = wave; p < count; p += kThreads / 64) s += parts[p * c + at];
-    sums[threadIdx.x] = s;
-    __syncthreads();
-    if (wave == 0 && at < c) {
+__device__ __forceinline__ void add_parts(const float* parts, int64_t count, int c, T* out, float* sums) {
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const int at = blockIdx.x * 64 + (threadIdx.x & 15) * 4, group = threadIdx.x >> 4;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (at + 3 < c && c % 4 == 0) {
+#pragma unroll 8
+        for (int64_t p = group; p < count; p += kJoinThreads / 16) {
+            const f32x4 x = *(const f32x4*)(parts + p * c + at);
 #pragma unroll
-        for (int w = 1; w < kThreads / 64; ++w) s += sums[w * 64 + threadIdx.x];
-        out[at] = narrow<T>(s);
+            for (int i = 0; i < 4; ++i) s[i] += x[i];
+        }
+    } else {
+        for (int64_t p = group; p < count; p += kJoinThreads / 16)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += at + i < c ? parts[p * c + at + i] : 0.f;
     }
+    *(f32x4*)(sums + threadIdx.x * 4) = s;
+    __syncthreads();
+    if (threadIdx.x < 64 && blockIdx.x * 64 + (int)threadIdx.x < c) {
+        float t = 0.f;
+#pragma unroll 8
+        for (int g = 0; g < kJoinThreads / 16; ++g) t += sums[g * 64 + threadIdx.x];
+        out[blockIdx.x * 64 + threadIdx.x] = narrow<T>(t);
+    }
+    __syncthreads();
 }
 
 // Rows 0 .. gates - 1: dgate from its units; then dw_post and dw_pre from the workgroups.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_join_kernel(NormArgs a, Cut cut, int gates, const float* gate_parts,
-                                                             const float* w_parts) {
+__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormArgs a, Cut cut, int gates, const float* gate_parts,
+                                                                 const float* w_parts) {
+    __shared__ __attribute__((aligned(16))) float sums[kJoinThreads * 4];
     const int64_t c = a.channels;
     for (int row = blockIdx.y; row < gates + 2; row += gridDim.y) {
-        __syncthreads();
         if (row < gates) {
-            add_parts(gate_parts + (int64_t)row * cut.per_gate * c, cut.per_gate, a.channels, (T*)a.dgate + row * c);
+            add_parts(gate_parts + (int64_t)row * cut.per_gate * c, cut.per_gate, a.channels, (T*)a.dgate + row * c, sums);
         } else {
             const int which = row - gates;
             float* out = which ? a.dw_pre : a.dw_post;
-            if (out) add_parts(w_parts + which * cut.groups * c, cut.groups, a.channels, out);
+            if (out) add_parts(w_parts + which * cut.groups * c, cut.groups, a.channels, out, sums);
         }
     }
 }
@@ -372,7 +443,7 @@ hipError_t run(const NormArgs& a, bool backward, hipStream_t stream) {
     const int64_t gates = a.dgate && cut.per_gate > 1 ? (a.tokens + a.gate_tokens - 1) / a.gate_tokens : 0;
     if (!gates && !a.dw_post && !a.dw_pre) return hipSuccess;
     const int64_t rows = gates + 2;
-    norm_join_kernel<T><<<dim3((a.channels + 63) / 64, (unsigned)(rows < 32768 ? rows : 32768)), kThreads, 0, stream>>>(
+    norm_join_kernel<T><<<dim3((a.channels + 63) / 64, (unsigned)(rows < 32768 ? rows : 32768)), kJoinThreads, 0, stream>>>(
         a, cut, (int)gates, gate_parts, w_parts);
     return hipGetLastError();
 }
