@@ -42,21 +42,40 @@ struct RowState {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
     }
-    // ROWS keys from t0. MASKED: some row may not see some key (holes: bit per key that is not there).
-    template <int ROWS, bool MASKED>
-    __device__ __forceinline__ void add(const char* kt, const char* vt, int t0, float c, unsigned long long holes, int lane) {
+    // ROWS keys from t0. masked: some row may not see some key (holes: bit per key that is not there).
+    template <int ROWS>
+    __device__ __forceinline__ void add(const char* kt, const char* vt, int t0, float c, bool masked, unsigned long long holes,
+                                        int lane) {
         constexpr int MB = ROWS / 32;
         using Ti = Tile<D>;
         f32x16 s[MB];
+        // All reads of a product are in flight before its first step, those of the values before
+        // the softmax: left to itself the compiler keeps two, and each step waits for LDS.
+        {
+            u32x4 kf[MB][D / 16];
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
+            for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
+                for (int i = 0; i < D / 16; ++i) kf[mb][i] = Ti::rows(kt, mb, i, lane);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) s[mb] = mma<T>(Ti::rows(kt, mb, i, lane), q[i], s[mb]);
+            for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) s[mb] = mma<T>(kf[mb][i], q[i], s[mb]);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int early = D == 64 ? MB * 2 : MB;  // steps whose values are read before the softmax
+        u32x4 vf[MB * 2][D / 32];
+#pragma unroll
+        for (int st = 0; st < early; ++st)
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) vf[st][i] = Ti::columns(vt, st >> 1, st & 1, i, lane);
+        __builtin_amdgcn_sched_barrier(0);
         const int base = t0 + 4 * (lane >> 5);
-        if constexpr (MASKED) {
+        if (masked) {
             const unsigned long long gone = holes >> (4 * (lane >> 5));
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb)
@@ -73,7 +92,7 @@ struct RowState {
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[mb][r]);
         top = both_max(top) * c;
-        if (__any(top > m + kSlack)) {
+        if (__builtin_expect(__any(top > m + kSlack), 0)) {
             const float next = fmaxf(m, top);
             const float old = exp2f(m - (next == -INFINITY ? 0.f : next));
             m = next;
@@ -98,11 +117,13 @@ struct RowState {
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+        for (int st = early; st < MB * 2; ++st)
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
+            for (int i = 0; i < D / 32; ++i) vf[st][i] = Ti::columns(vt, st >> 1, st & 1, i, lane);
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] = mma<T>(Ti::columns(vt, mb, st, i, lane), p[2 * mb + st], o[i]);
+        for (int st = 0; st < MB * 2; ++st)
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] = mma<T>(vf[st][i], p[st], o[i]);
     }
 };
 
@@ -176,8 +197,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionAr
         bool bad = false;
         if (holes || !all_see<ROWS>(all, t0)) bad = __syncthreads_or(clean_tile<T, D, ROWS>(now[1], threadIdx.x, kThreads));
         if (!idle && !none_sees<ROWS>(mine, t0)) {
-            if (!holes && all_see<ROWS>(mine, t0)) st.template add<ROWS, false>(now[0], now[1], t0, c, 0, lane);
-            else st.template add<ROWS, true>(now[0], now[1], t0, c, holes, lane);
+            st.template add<ROWS>(now[0], now[1], t0, c, holes || !all_see<ROWS>(mine, t0), holes, lane);
             if (bad) add_nonfinite<T, D>(st.o, st.sp, t0, keys.end(t0 + ROWS), holes, lane, [&](int j) { return keys.value(j); });
         }
         holes = pages.holes;
@@ -240,8 +260,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kerne
         const bool whole = !holes && all_see<ROWS>(all, t0);
         bool bad = false;
         if (!whole) bad = __any(clean_tile<T, D, ROWS>(vt, lane, 64));
-        if (whole) st.template add<ROWS, false>(kt, vt, t0, c, 0, lane);
-        else st.template add<ROWS, true>(kt, vt, t0, c, holes, lane);
+        st.template add<ROWS>(kt, vt, t0, c, !whole, holes, lane);
         if (bad) add_nonfinite<T, D>(st.o, st.sp, t0, keys.end(t0 + ROWS), holes, lane, [&](int j) { return keys.value(j); });
         holes = pages.holes;
         wait_reads();  // the next copies go where this tile was
