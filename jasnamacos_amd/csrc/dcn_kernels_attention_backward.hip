@@ -42,13 +42,29 @@ template <int D>
 __device__ __forceinline__ void follow_scale(float top, float* up, f32x16* sum) {
     top = both_max(top);
     const bool change = top * *up > kMostScaled || (*up == 0.f && top > 0.f);
-    if (!__any(change)) return;
+    if (__builtin_expect(!__any(change), 1)) return;
     const float next = change ? scale_for(top) : *up, by = *up == 0.f ? 1.f : next / *up;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
         for (int x = 0; x < 16; ++x) sum[n][x] *= by;
     *up = next;
+}
+
+// Zeros for a tile's infinities and NaN, by the whole workgroup; a bit for each row that had one.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ unsigned long long clean_rows(char* tile, unsigned long long* mask, int thread) {
+    if (thread == 0) *mask = 0;
+    __syncthreads();
+    for (int i = thread; i < ROWS * D / 8; i += kThreads) {
+        u32x4 x = *(const u32x4*)(tile + i * 16);
+        if (clean16<T>(x)) {
+            *(u32x4*)(tile + i * 16) = x;
+            atomicOr(mask, 1ull << (i / (D / 8)));
+        }
+    }
+    __syncthreads();
+    return *mask;
 }
 
 // Keys of a tile of the first pass: with 128 channels a wave's operands and sums leave registers
@@ -61,6 +77,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
     constexpr int ROWS = kDqKeys<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
+    __shared__ unsigned long long row_mask;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
     if (!place_of<32 * kWaves>(a, 1, &pl)) return;
@@ -121,71 +138,75 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
         if (step + 1 < steps)
             copy_tile<D, ROWS, kWaves, false>(keys, list.tile(i + 1 < list.count ? i + 1 : 0), none, other[0], other[1], wave, lane);
         const bool delta_step = sum_delta && step < list.count;
-        bool bad = false;
-        if (!delta_step && !all_see<ROWS>(all, t0))
-            bad = __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads));
-        const bool active = !idle && !none_sees<ROWS>(mine, t0), whole = all_see<ROWS>(mine, t0);
-        u32x4 ds[2 * MB];
-        if (active) {
-            f32x16 t[MB];
+        // Keys that are not finite, where some row does not see all of the tile: zeros in LDS, and
+        // the scores of the rows that see them are NaN.
+        unsigned long long poison = 0;
+        if (!all_see<ROWS>(all, t0) && __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads)))
+            poison = clean_rows<T, D, ROWS>(now[0], &row_mask, threadIdx.x);
+        if (!idle && !none_sees<ROWS>(mine, t0)) {
+            const bool masked = !all_see<ROWS>(mine, t0) || poison;
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) {
                 f32x16 s, dp;
+                {
+                    u32x4 kr[D / 16], vr[D / 16];
 #pragma unroll
-                for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+                    for (int n = 0; n < D / 16; ++n) kr[n] = Ti::rows(now[0], mb, n, lane);
 #pragma unroll
-                for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(now[0], mb, n, lane), q[n], s);
+                    for (int n = 0; n < D / 16; ++n) vr[n] = Ti::rows(now[1], mb, n, lane);
+                    if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(now[1], mb, n, lane), go[n], dp);
+                    for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
 #pragma unroll
-                for (int x = 0; x < 16; ++x)
-                    t[mb][x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - delta);
-                if (!whole) {
+                    for (int n = 0; n < D / 16; ++n) s = mma<T>(kr[n], q[n], s);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        t[mb][x] = sees(sp, t0 + 4 * (lane >> 5) + 32 * mb + 8 * (x >> 2) + (x & 3)) ? t[mb][x] : 0.f;
+                    for (int n = 0; n < D / 16; ++n) dp = mma<T>(vr[n], go[n], dp);
                 }
-            }
-            if (delta_step) {
+                // 64 channels leave registers to read the next product's keys before the weights are made.
+                u32x4 kc[2][D / 32];
+                auto read_columns = [&] {
 #pragma unroll
-                for (int mb = 0; mb < MB; ++mb)
+                    for (int st = 0; st < 2; ++st)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) exact_delta += t[mb][x];
-            } else {
-            if constexpr (kScaled<T>) {
-                follow_scale<D>(MB == 1 ? top_of(t[0]) : fmaxf(top_of(t[0]), top_of(t[MB - 1])), &up, sum);
+                        for (int n = 0; n < D / 32; ++n) kc[st][n] = Ti::columns(now[0], mb, st, n, lane);
+                };
+                if constexpr (D == 64) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_columns();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
-                for (int mb = 0; mb < MB; ++mb)
+                for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - delta);
+                if (masked) {
+                    const unsigned long long not_finite = poison >> (4 * (lane >> 5));
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) t[mb][x] *= up;
-            }
+                    for (int x = 0; x < 16; ++x) {
+                        const int in = 32 * mb + 8 * (x >> 2) + (x & 3);
+                        if ((uint32_t)(not_finite >> (in & 32)) >> (in & 31) & 1) s[x] = NAN;
+                        s[x] = sees(sp, t0 + 4 * (lane >> 5) + in) ? s[x] : 0.f;
+                    }
+                }
+                if (delta_step) {  // the sums are left as they are by a product with zeros
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-                ds[2 * mb] = pack8<T>(t[mb], 0);
-                ds[2 * mb + 1] = pack8<T>(t[mb], 8);
-            }
-            }
-        }
-        if (delta_step) {
-            if (i + 1 == list.count) delta = both_sum(exact_delta);
-            continue;
-        }
-        if (bad) {  // some row does not see all of this tile, and a key in it is not finite
-            __syncthreads();
-            clean_tile<T, D, ROWS>(now[0], threadIdx.x, kThreads);
-            __syncthreads();
-        }
-        if (active) {
+                    for (int x = 0; x < 16; ++x) {
+                        exact_delta += s[x];
+                        s[x] = 0.f;
+                    }
+                }
+                if constexpr (kScaled<T>) {
+                    follow_scale<D>(top_of(s), &up, sum);
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
+                    for (int x = 0; x < 16; ++x) s[x] *= up;
+                }
+                const u32x4 ds[2] = {pack8<T>(s, 0), pack8<T>(s, 8)};
+                if constexpr (D != 64) read_columns();
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
 #pragma unroll
-                    for (int n = 0; n < D / 32; ++n) sum[n] = mma<T>(Ti::columns(now[0], mb, st, n, lane), ds[2 * mb + st], sum[n]);
-            if (bad)
-                add_nonfinite<T, D>(sum, sp, t0, keys.end(t0 + ROWS), 0, lane,
-                                    [&](int j) { return (const uint16_t*)(keys.kp + (int64_t)j * keys.k.ts * 2); });
+                    for (int n = 0; n < D / 32; ++n) sum[n] = mma<T>(kc[st][n], ds[st], sum[n]);
+            }
         }
+        if (delta_step && i + 1 == list.count) delta = both_sum(exact_delta);
     }
     if (r > last_row) return;
     if (sum_delta && lane < 32) ((float*)a.workspace)[index] = delta;
@@ -245,47 +266,6 @@ __device__ __forceinline__ Seen all_seen_of(const AttentionArgs& a, int j, int t
 template <int D>
 constexpr int kDkvRows = 64;
 
-// P (16 bits, FP16 lifted) and dS of a query tile's rows (registers) and a wave's keys (lanes).
-// MASKED: some row may not see some key.
-template <typename T, int D, int MB, bool MASKED>
-__device__ __forceinline__ void weights_of(const char* qt, const char* ot, const u32x4* k, const u32x4* v, const float* lse,
-                                           const float* delta, const int* at, float c, const Seen& me, int lane, u32x4* p16,
-                                           f32x16* t) {
-    using Ti = Tile<D>;
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-        f32x16 s, dp;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) s = mma<T>(Ti::rows(qt, mb, n, lane), k[n], s);
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) dp = mma<T>(Ti::rows(ot, mb, n, lane), v[n], dp);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            typedef int i32x4 __attribute__((ext_vector_type(4)));
-            const int in = 32 * mb + 8 * g + 4 * (lane >> 5);
-            const f32x4 l4 = *(const f32x4*)(lse + in), d4 = *(const f32x4*)(delta + in);
-            i32x4 p4;
-            if constexpr (MASKED) p4 = *(const i32x4*)(at + in);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int x = 4 * g + b;
-                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[b]));
-                t[mb][x] = s[x] * (dp[x] - d4[b]);
-                if constexpr (MASKED) {
-                    const bool on = p4[b] >= me.from && p4[b] < me.to && p4[b] >= 0;
-                    s[x] = on ? s[x] : 0.f;
-                    t[mb][x] = on ? t[mb][x] : 0.f;
-                }
-                if constexpr (kScaled<T>) s[x] *= kWeightLift;
-            }
-        }
-        p16[2 * mb] = pack8<T>(s, 0);
-        p16[2 * mb + 1] = pack8<T>(s, 8);
-    }
-}
-
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a, KeyPlan plan, float* parts) {
     constexpr int ROWS = kDkvRows<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
@@ -293,6 +273,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
     __shared__ __attribute__((aligned(16))) int row_at[2][ROWS];  // a row's position; -1: no row
+    __shared__ unsigned long long row_mask, row_mask2;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     int block, part, of;
     plan.item(blockIdx.x, &block, &part, &of);
@@ -395,53 +376,82 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
         const bool rows_there = r0 + ROWS <= q_rows && p0 >= 0;
         const bool whole = rows_there && p0 >= wave_every.from && p1 < wave_every.to;
         const bool block_whole = rows_there && p0 >= every.from && p1 < every.to;
-        bool bad = false;
-        if (!block_whole)
-            bad = __syncthreads_or((int)tile_nonfinite<T, D, ROWS>(qt, threadIdx.x, kThreads) |
-                                   (int)tile_nonfinite<T, D, ROWS>(ot, threadIdx.x, kThreads));
-        u32x4 p16[2 * MB], ds[2 * MB];
-        f32x16 t[MB];
-        if (whole)
-            weights_of<T, D, MB, false>(qt, ot, k, v, row_lse[buf], row_delta[buf], row_at[buf], c, me, lane, p16, t);
-        else
-            weights_of<T, D, MB, true>(qt, ot, k, v, row_lse[buf], row_delta[buf], row_at[buf], c, me, lane, p16, t);
-        if constexpr (kScaled<T>) {
-            follow_scale<D>(MB == 1 ? top_of(t[0]) : fmaxf(top_of(t[0]), top_of(t[MB - 1])), &up, dk);
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) t[mb][x] *= up;
+        // Queries and gradients that are not finite, where some pair of the tile is not visible:
+        // zeros in LDS, and the weights of the pairs that are visible are NaN.
+        if (!block_whole && __syncthreads_or((int)tile_nonfinite<T, D, ROWS>(qt, threadIdx.x, kThreads) |
+                                             (int)tile_nonfinite<T, D, ROWS>(ot, threadIdx.x, kThreads))) {
+            const unsigned long long not_finite = clean_rows<T, D, ROWS>(qt, &row_mask, threadIdx.x) |
+                                                  clean_rows<T, D, ROWS>(ot, &row_mask2, threadIdx.x);
+            if (threadIdx.x < ROWS && (not_finite >> threadIdx.x & 1)) row_lse[buf][threadIdx.x] = NAN;
+            __syncthreads();
         }
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-            ds[2 * mb] = pack8<T>(t[mb], 0);
-            ds[2 * mb + 1] = pack8<T>(t[mb], 8);
-        }
-        if (bad) {  // some pair of the tile is not visible, and a query or a gradient in it is not finite
-            __syncthreads();
-            clean_tile<T, D, ROWS>(qt, threadIdx.x, kThreads);
-            clean_tile<T, D, ROWS>(ot, threadIdx.x, kThreads);
-            __syncthreads();
-        }
+            f32x16 s, dp;
+            {
+                u32x4 qr[D / 16], gr[D / 16];
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+                for (int n = 0; n < D / 16; ++n) qr[n] = Ti::rows(qt, mb, n, lane);
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) gr[n] = Ti::rows(ot, mb, n, lane);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) s = mma<T>(qr[n], k[n], s);
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) dp = mma<T>(gr[n], v[n], dp);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 oc[2][D / 32], qc[2][D / 32];
+            f32x4 l4[4], d4[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                l4[g] = *(const f32x4*)&row_lse[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
+                d4[g] = *(const f32x4*)&row_delta[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
+            }
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int n = 0; n < D / 32; ++n) {
-                    dv[n] = mma<T>(Ti::columns(ot, mb, st, n, lane), p16[2 * mb + st], dv[n]);
-                    dk[n] = mma<T>(Ti::columns(qt, mb, st, n, lane), ds[2 * mb + st], dk[n]);
+                    oc[st][n] = Ti::columns(ot, mb, st, n, lane);
+                    qc[st][n] = Ti::columns(qt, mb, st, n, lane);
                 }
-        if (bad) {
-            for (int x = 0; x < ROWS; ++x) {
-                const int at = row_at[buf][x];
-                if (at < 0) continue;
-                const bool on = at >= me.from && at < me.to;
-                const int r = r0 + x, tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
-                const int64_t row = pl.q.first + tok;
-                add_nonfinite<T, D>(dk, (const uint16_t*)a.q.p + row * a.q.ts + head * a.q.hs, on, lane);
-                add_nonfinite<T, D>(dv, (const uint16_t*)a.dout.p + row * a.dout.ts + head * a.dout.hs, on, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[x >> 2][x & 3]));
+                dp[x] = s[x] * (dp[x] - d4[x >> 2][x & 3]);
             }
+            if (!whole) {
+                typedef int i32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const i32x4 at = *(const i32x4*)&row_at[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const bool on = at[b] >= me.from && at[b] < me.to && at[b] >= 0;
+                        s[4 * g + b] = on ? s[4 * g + b] : 0.f;
+                        dp[4 * g + b] = on ? dp[4 * g + b] : 0.f;
+                    }
+                }
+            }
+            if constexpr (kScaled<T>) {
+                follow_scale<D>(top_of(dp), &up, dk);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    s[x] *= kWeightLift;
+                    dp[x] *= up;
+                }
+            }
+            const u32x4 p16[2] = {pack8<T>(s, 0), pack8<T>(s, 8)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 8)};
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int n = 0; n < D / 32; ++n) {
+                    dv[n] = mma<T>(oc[st][n], p16[st], dv[n]);
+                    dk[n] = mma<T>(qc[st][n], ds[st], dk[n]);
+                }
         }
     }
     const float fk = up == 0.f ? 0.f : a.scale / up, fv = kScaled<T> ? 1.f / kWeightLift : 1.f;
