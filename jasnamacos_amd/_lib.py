@@ -255,20 +255,20 @@ SIGNATURES: dict[str, tuple] = {
     "dcn_clip_capture": (C.c_int, [c_void, c_void, c_void, c_void, c_void, C.c_int, C.POINTER(c_void)]),
     "dcn_clip_run_with_fallback_dev": (C.c_int, [c_void, c_void, c_void, c_void, c_void, c_void, ReportFn, c_void,
                                                  C.POINTER(C.c_int)]),
-    # frame attention
-    "dcn_rotary_dev": (C.c_int, [CtxP, C.POINTER(DcnRotary), C.c_int64, C.c_int, c_void, C.c_int64, C.c_int64, c_void,
+    # frame attention (shapes: a ctypes struct by reference, or its packed bytes)
+    "dcn_rotary_dev": (C.c_int, [CtxP, c_void, C.c_int64, C.c_int, c_void, C.c_int64, C.c_int64, c_void,
                                  c_void, C.c_int, c_void, C.c_int64, C.c_int64, c_void]),
-    "dcn_cache_append_dev": (C.c_int, [CtxP, C.POINTER(DcnCache), C.POINTER(DcnAppendShape), C.POINTER(DcnRotary)]
+    "dcn_cache_append_dev": (C.c_int, [CtxP, c_void, c_void, c_void]
                              + [c_void] * 12),
-    "dcn_attention_workspace_bytes": (c_size, [C.POINTER(DcnAttentionShape), C.c_int]),
-    "dcn_attention_forward_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape)] + [c_void] * 8 + [c_size, c_void]),
-    "dcn_attention_paged_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape), C.POINTER(DcnCache)] + [c_void] * 9
+    "dcn_attention_workspace_bytes": (c_size, [c_void, C.c_int]),
+    "dcn_attention_forward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 8 + [c_size, c_void]),
+    "dcn_attention_paged_dev": (C.c_int, [CtxP, c_void, c_void] + [c_void] * 9
                                 + [c_size, c_void]),
-    "dcn_attention_backward_dev": (C.c_int, [CtxP, C.POINTER(DcnAttentionShape)] + [c_void] * 12 + [c_size, c_void]),
-    "dcn_gated_norm_forward_dev": (C.c_int, [CtxP, C.POINTER(DcnNormShape)] + [c_void] * 10),
-    "dcn_gated_norm_low_bytes": (c_size, [C.POINTER(DcnNormShape)]),
-    "dcn_gated_norm_workspace_bytes": (c_size, [C.POINTER(DcnNormShape)]),
-    "dcn_gated_norm_backward_dev": (C.c_int, [CtxP, C.POINTER(DcnNormShape)] + [c_void] * 15 + [c_size, c_void]),
+    "dcn_attention_backward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 12 + [c_size, c_void]),
+    "dcn_gated_norm_forward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 10),
+    "dcn_gated_norm_low_bytes": (c_size, [c_void]),
+    "dcn_gated_norm_workspace_bytes": (c_size, [c_void]),
+    "dcn_gated_norm_backward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 15 + [c_size, c_void]),
 }
 
 _LIB: C.CDLL | None = None

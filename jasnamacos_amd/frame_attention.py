@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -40,25 +41,46 @@ def _need(condition, message: str) -> None:
         raise DeformConvError(INVALID_SHAPE, message)
 
 
-def _heads(name: str, t, dtype, tokens, heads, dim) -> tuple:
-    """The strides of a tensor of heads, after its checks (None: any)."""
-    if t.dim() != 3 or (tokens is not None and t.shape[0] != tokens) or t.shape[1] != heads or t.shape[2] != dim:
-        raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected "
-                                             f"[{'tokens' if tokens is None else tokens}][{heads}][{dim}]")
-    if t.dtype != dtype:
-        raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
-    ts, hs, cs = t.stride()
-    if cs != 1 and dim > 1:
+def _heads(name: str, t, dtype, shape) -> tuple:
+    """The strides of a tensor of heads of this shape (its own row count where that is None)."""
+    if t.shape == shape and t.dtype is dtype:
+        strides = t.stride()
+        if strides[2] == 1 or shape[2] == 1:
+            return strides
         raise DeformConvError(INVALID_SHAPE, f"{name} channels are not adjacent")
-    return ts, hs
-
-
-def _whole(name: str, t, dtype, *shape) -> None:
-    """An adjacent tensor of this type and shape."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}, adjacent")
+    raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}")
+
+
+def _rows(name: str, t) -> int:
+    """The rows of a tensor of heads."""
+    if t.dim() != 3:
+        raise DeformConvError(INVALID_SHAPE, f"{name} has {t.dim()} dimensions; expected [tokens][heads][channels]")
+    return t.shape[0]
+
+
+def _whole(name: str, t, dtype, shape) -> None:
+    """An adjacent tensor of this type and shape."""
+    if t.shape == shape and t.dtype is dtype and t.is_contiguous():
+        return
+    if t.dtype is not dtype:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
+    raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}, adjacent")
+
+
+def _index(name: str, t, count) -> None:
+    """An adjacent int32 array of this length."""
+    if t.dtype is torch.int32 and t.shape == (count,) and t.is_contiguous():
+        return
+    raise DeformConvError(INVALID_SHAPE, f"{name} is not {count} adjacent int32 values")
+
+
+# The C structs' layouts: packing one is several times faster than filling its fields.
+_APPEND = struct.Struct("iiq8q")
+_ATTENTION = struct.Struct("11ifqq16q")
+_NORM = struct.Struct("iiqqff")
+_NO_STRIDES = (0, 0)
 
 
 class _Handle:
@@ -66,9 +88,16 @@ class _Handle:
         self.ctx = ctx
         self._lib = ctx._lib
         self._workspace = None
+        self._sizes = {}  # workspace bytes of the shapes seen
 
-    def _room(self, count: int, like):
-        """(pointer, bytes) of a workspace of `count` bytes that the handle keeps."""
+    def _room(self, key, ask, like):
+        """(pointer, bytes) of the workspace that the handle keeps; ask() says how many bytes calls
+        of the sizes `key` need."""
+        count = self._sizes.get(key)
+        if count is None:
+            if len(self._sizes) > 1024:
+                self._sizes.clear()
+            count = self._sizes[key] = ask()
         if not count:
             return None, 0
         w = self._workspace
@@ -87,6 +116,7 @@ class Rotary(_Handle):
         super().__init__(ctx)
         self.head_dim, self.pairs, self.interleaved = int(head_dim), tuple(int(p) for p in pairs), bool(interleaved)
         _need(len(self.pairs) == 3, "rotary pairs are three numbers (time, height, width)")
+        self._freq_shape = (sum(self.pairs),)
         self._c = {code: _lib.DcnRotary(code, self.head_dim, (C.c_int32 * 3)(*self.pairs), int(self.interleaved))
                    for code in DTYPES.values()}
 
@@ -96,34 +126,32 @@ class Rotary(_Handle):
         return torch.cat(parts).float().to(device)
 
     def _check(self, positions, freq, tokens) -> None:
-        _whole("positions", positions, torch.int32, tokens, 3)
-        _whole("freq", freq, torch.float32, sum(self.pairs))
+        _whole("positions", positions, torch.int32, (tokens, 3))
+        _whole("freq", freq, torch.float32, self._freq_shape)
 
     def run_dev(self, x, positions, freq, out, inverse: bool = False, stream=None) -> None:
         """out = x turned by positions ([tokens][3] int32) times freq; inverse: the gradient."""
-        tokens, heads = x.shape[0], x.shape[1]
-        xs = _heads("x", x, x.dtype, tokens, heads, self.head_dim)
-        os = _heads("out", out, x.dtype, tokens, heads, self.head_dim)
+        tokens, dtype = _rows("x", x), x.dtype
+        heads = x.shape[1]
+        shape = (tokens, heads, self.head_dim)
+        xt, xh, _ = _heads("x", x, dtype, shape)
+        ot, oh, _ = _heads("out", out, dtype, shape)
         self._check(positions, freq, tokens)
         self.ctx._check(self._lib.dcn_rotary_dev(
-            self.ctx.ctx, C.byref(self._c[_dtype(x)]), tokens, heads, x.data_ptr(), xs[0], xs[1], positions.data_ptr(),
-            freq.data_ptr(), int(inverse), out.data_ptr(), os[0], os[1], _stream(stream)))
+            self.ctx.ctx, C.byref(self._c[_dtype(x)]), tokens, heads, x.data_ptr(), xt, xh, positions.data_ptr(),
+            freq.data_ptr(), inverse, out.data_ptr(), ot, oh, _stream(stream)))
 
 
 def _cache(k_pages, v_pages, table) -> _lib.DcnCache:
     if k_pages.dim() != 4 or table.dim() != 2:
         raise DeformConvError(INVALID_SHAPE, "pages are [pages][page_tokens][heads][channels], the table "
                                              "[sequences][width]")
-    _whole("k_pages", k_pages, k_pages.dtype, *k_pages.shape)
-    _whole("v_pages", v_pages, k_pages.dtype, *k_pages.shape)
-    _whole("table", table, torch.int32, *table.shape)
-    pages, page_tokens, heads, dim = k_pages.shape
+    shape, dtype = k_pages.shape, k_pages.dtype
+    _whole("k_pages", k_pages, dtype, shape)
+    _whole("v_pages", v_pages, dtype, shape)
+    _whole("table", table, torch.int32, table.shape)
+    pages, page_tokens, heads, dim = shape
     return _lib.DcnCache(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
-
-
-def _starts(name: str, t, sequences) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != sequences or not t.is_contiguous():
-        raise DeformConvError(INVALID_SHAPE, f"{name} is not {sequences} int32 values")
 
 
 class CacheAppend(_Handle):
@@ -135,24 +163,26 @@ class CacheAppend(_Handle):
         last of its kv_lens[s] tokens. Keys are turned by `rotary` on the way, and so is q into
         q_out where it is given."""
         cache = _cache(k_pages, v_pages, table)
-        tokens, sequences = k.shape[0], table.shape[0]
-        s = _lib.DcnAppendShape(sequences, 0, tokens)
-        s.k_stride[:] = _heads("k", k, k_pages.dtype, tokens, cache.kv_heads, cache.head_dim)
-        s.v_stride[:] = _heads("v", v, k_pages.dtype, tokens, cache.kv_heads, cache.head_dim)
-        _starts("cu_q", cu_q, sequences + 1)
-        _starts("kv_lens", kv_lens, sequences)
+        tokens, sequences, dtype, dim = _rows("k", k), table.shape[0], k_pages.dtype, cache.head_dim
+        shape = (tokens, cache.kv_heads, dim)
+        ks, vs = _heads("k", k, dtype, shape), _heads("v", v, dtype, shape)
+        _index("cu_q", cu_q, sequences + 1)
+        _index("kv_lens", kv_lens, sequences)
+        q_heads, qs, os = 0, _NO_STRIDES, _NO_STRIDES
         if q is not None:
-            s.q_heads = q.shape[1]
-            s.q_stride[:] = _heads("q", q, k_pages.dtype, tokens, q.shape[1], cache.head_dim)
-            s.q_out_stride[:] = _heads("q_out", q_out, k_pages.dtype, tokens, q.shape[1], cache.head_dim)
+            _rows("q", q)
+            q_heads = q.shape[1]
+            shape = (tokens, q_heads, dim)
+            qs, os = _heads("q", q, dtype, shape), _heads("q_out", q_out, dtype, shape)
         r = None
         if rotary is not None:
             rotary._check(positions, freq, tokens)
             r = C.byref(rotary._c[cache.dtype])
+        s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
         self.ctx._check(self._lib.dcn_cache_append_dev(
-            self.ctx.ctx, C.byref(cache), C.byref(s), r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions),
-            _ptr(freq), cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(),
-            v_pages.data_ptr(), _stream(stream)))
+            self.ctx.ctx, C.byref(cache), s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq),
+            cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
+            _stream(stream)))
 
 
 class FrameAttention(_Handle):
@@ -170,60 +200,69 @@ class FrameAttention(_Handle):
         self.frame_tokens, self.back, self.ahead, self.sinks = int(frame_tokens), int(back), int(ahead), int(sinks)
         self.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
 
-    def _shape(self, q, sequences, max_q, max_kv, kv_tokens) -> _lib.DcnAttentionShape:
-        return _lib.DcnAttentionShape(_dtype(q), sequences, self.q_heads, self.kv_heads, self.head_dim,
-                                      self.frame_tokens, self.back, self.ahead, self.sinks, max_q, max_kv, self.scale,
-                                      q.shape[0], kv_tokens)
+    def _pack(self, q, sequences, max_q, max_kv, q_tokens, kv_tokens, *strides) -> bytes:
+        """The packed dcn_attention_shape; strides: (token, head, ...) of q, k, v, out, dout, dq, dk, dv."""
+        flat = [x for s in strides for x in s[:2]]
+        flat += [0] * (16 - len(flat))
+        return _ATTENTION.pack(_dtype(q), sequences, self.q_heads, self.kv_heads, self.head_dim, self.frame_tokens,
+                               self.back, self.ahead, self.sinks, max_q, max_kv, self.scale, q_tokens, kv_tokens, *flat)
 
-    def _runs(self, q, k, cu_q, cu_kv, max_q, max_kv):
+    def _runs(self, q_tokens, kv_tokens, cu_q, cu_kv, max_q, max_kv):
         """(sequences, max_q, max_kv): without index arrays, one sequence of all rows, or the
         rows in equal runs of max_q and max_kv."""
-        max_q = q.shape[0] if max_q is None else int(max_q)
-        max_kv = k.shape[0] if max_kv is None else int(max_kv)
+        max_q = q_tokens if max_q is None else int(max_q)
+        max_kv = kv_tokens if max_kv is None else int(max_kv)
         if cu_q is not None:
             sequences = cu_q.shape[0] - 1
         elif cu_kv is not None:
             sequences = cu_kv.shape[0] - 1
         else:
-            sequences = q.shape[0] // max_q if max_q else (k.shape[0] // max_kv if max_kv else 0)
+            sequences = q_tokens // max_q if max_q else (kv_tokens // max_kv if max_kv else 0)
         if cu_q is not None:
-            _starts("cu_q", cu_q, sequences + 1)
+            _index("cu_q", cu_q, sequences + 1)
         if cu_kv is not None:
-            _starts("cu_kv", cu_kv, sequences + 1)
+            _index("cu_kv", cu_kv, sequences + 1)
         return sequences, max_q, max_kv
 
-    def _forward_shape(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv):
-        sequences, max_q, max_kv = self._runs(q, k, cu_q, cu_kv, max_q, max_kv)
-        s = self._shape(q, sequences, max_q, max_kv, k.shape[0])
-        s.q_stride[:] = _heads("q", q, q.dtype, None, self.q_heads, self.head_dim)
-        s.k_stride[:] = _heads("k", k, q.dtype, None, self.kv_heads, self.head_dim)
-        s.v_stride[:] = _heads("v", v, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
-        s.out_stride[:] = _heads("out", out, q.dtype, q.shape[0], self.q_heads, self.head_dim)
+    def _forward_parts(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv):
+        """What _pack takes, after the checks."""
+        q_tokens, kv_tokens, dtype = _rows("q", q), _rows("k", k), q.dtype
+        runs = self._runs(q_tokens, kv_tokens, cu_q, cu_kv, max_q, max_kv)
+        q_shape, k_shape = (q_tokens, self.q_heads, self.head_dim), (kv_tokens, self.kv_heads, self.head_dim)
+        strides = (_heads("q", q, dtype, q_shape), _heads("k", k, dtype, k_shape), _heads("v", v, dtype, k_shape),
+                   _heads("out", out, dtype, q_shape))
         if lse is not None:
-            _whole("lse", lse, torch.float32, q.shape[0], self.q_heads)
-        return s
+            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads))
+        return (q, *runs, q_tokens, kv_tokens, *strides)
+
+    def _forward_shape(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv) -> _lib.DcnAttentionShape:
+        parts = self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
+        return _lib.DcnAttentionShape.from_buffer_copy(self._pack(*parts))
+
+    def _workspace_of(self, s: bytes, which: int, q):
+        """The workspace of a call of this shape; strides have no part in its size."""
+        return self._room((which, s[:64]), lambda: self._lib.dcn_attention_workspace_bytes(s, which), q)
 
     def forward_dev(self, q, k, v, out, lse=None, cu_q=None, cu_kv=None, max_q=None, max_kv=None, stream=None) -> None:
         """out = softmax(scale q k^T over what is visible) v; lse ([tokens][q_heads] FP32) is what
         backward_dev reads. cu_q, cu_kv: int32 starts of the sequences and the end of the last;
         max_q and max_kv bound their lengths."""
-        s = self._forward_shape(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
-        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_FORWARD), q)
+        s = self._pack(*self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv))
+        w, size = self._workspace_of(s, PASS_FORWARD, q)
         self.ctx._check(self._lib.dcn_attention_forward_dev(
-            self.ctx.ctx, C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_q), _ptr(cu_kv), out.data_ptr(),
+            self.ctx.ctx, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_q), _ptr(cu_kv), out.data_ptr(),
             _ptr(lse), w, size, _stream(stream)))
 
     def backward_dev(self, q, k, v, out, lse, dout, dq, dk, dv, cu_q=None, cu_kv=None, max_q=None, max_kv=None,
                      stream=None) -> None:
         """The gradients of forward_dev's out, from its arguments, out, lse and dout."""
-        s = self._forward_shape(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
-        s.dout_stride[:] = _heads("dout", dout, q.dtype, q.shape[0], self.q_heads, self.head_dim)
-        s.dq_stride[:] = _heads("dq", dq, q.dtype, q.shape[0], self.q_heads, self.head_dim)
-        s.dk_stride[:] = _heads("dk", dk, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
-        s.dv_stride[:] = _heads("dv", dv, q.dtype, k.shape[0], self.kv_heads, self.head_dim)
-        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_BACKWARD), q)
+        parts = self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
+        dtype, q_shape, k_shape = q.dtype, q.shape, k.shape
+        s = self._pack(*parts, _heads("dout", dout, dtype, q_shape), _heads("dq", dq, dtype, q_shape),
+                       _heads("dk", dk, dtype, k_shape), _heads("dv", dv, dtype, k_shape))
+        w, size = self._workspace_of(s, PASS_BACKWARD, q)
         self.ctx._check(self._lib.dcn_attention_backward_dev(
-            self.ctx.ctx, C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            self.ctx.ctx, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             dout.data_ptr(), _ptr(cu_q), _ptr(cu_kv), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), w, size,
             _stream(stream)))
 
@@ -233,22 +272,22 @@ class FrameAttention(_Handle):
         last tokens (one, or a frame's). cu_q None: max_q queries each. max_kv bounds kv_lens
         (default: the table's width)."""
         cache = _cache(k_pages, v_pages, table)
-        sequences = table.shape[0]
+        sequences, q_tokens, dtype = table.shape[0], _rows("q", q), k_pages.dtype
         if cu_q is not None:
-            _starts("cu_q", cu_q, sequences + 1)
-        _starts("kv_lens", kv_lens, sequences)
+            _index("cu_q", cu_q, sequences + 1)
+        _index("kv_lens", kv_lens, sequences)
         if max_q is None:
-            max_q = q.shape[0] if cu_q is not None else (q.shape[0] // sequences if sequences else 0)
+            max_q = q_tokens if cu_q is not None else (q_tokens // sequences if sequences else 0)
         if max_kv is None:
             max_kv = cache.table_width * cache.page_tokens
-        s = self._shape(q, sequences, int(max_q), int(max_kv), 0)
-        s.q_stride[:] = _heads("q", q, k_pages.dtype, None, self.q_heads, self.head_dim)
-        s.out_stride[:] = _heads("out", out, k_pages.dtype, q.shape[0], self.q_heads, self.head_dim)
+        shape = (q_tokens, self.q_heads, self.head_dim)
         if lse is not None:
-            _whole("lse", lse, torch.float32, q.shape[0], self.q_heads)
-        w, size = self._room(self._lib.dcn_attention_workspace_bytes(C.byref(s), PASS_PAGED), q)
+            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads))
+        s = self._pack(q, sequences, int(max_q), int(max_kv), q_tokens, 0, _heads("q", q, dtype, shape), _NO_STRIDES,
+                       _NO_STRIDES, _heads("out", out, dtype, shape))
+        w, size = self._workspace_of(s, PASS_PAGED, q)
         self.ctx._check(self._lib.dcn_attention_paged_dev(
-            self.ctx.ctx, C.byref(s), C.byref(cache), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q),
+            self.ctx.ctx, s, C.byref(cache), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q),
             kv_lens.data_ptr(), table.data_ptr(), out.data_ptr(), _ptr(lse), w, size, _stream(stream)))
 
 
@@ -264,26 +303,36 @@ class GatedNorm(_Handle):
         self._kept = None
         _need(self.channels > 0 and self.gate_tokens > 0, "channels and gate_tokens must be positive")
 
-    def _shape(self, x, gate, vectors, tensors) -> _lib.DcnNormShape:
+    def _pack(self, x) -> bytes:
+        if x.dim() != 2:
+            raise DeformConvError(INVALID_SHAPE, f"the residual stream has {x.dim()} dimensions; expected [tokens][channels]")
+        return _NORM.pack(_dtype(x), self.channels, x.shape[0], self.gate_tokens, self.residual_scale, self.eps)
+
+    def _check_all(self, x, tensors, gates, vectors, sums=()) -> None:
         tokens, dtype = x.shape[0], x.dtype
+        shape = (tokens, self.channels)
         for name, t in tensors:
             if t is not None:
-                _whole(name, t, dtype, tokens, self.channels)
-        for name, t in gate:
+                _whole(name, t, dtype, shape)
+        for name, t in gates:
             if t is not None:
-                _whole(name, t, dtype, -(-tokens // self.gate_tokens), self.channels)
-        for name, t, kind in vectors:
+                _whole(name, t, dtype, (-(-tokens // self.gate_tokens), self.channels))
+        for name, t in vectors:
             if t is not None:
-                _whole(name, t, kind or dtype, self.channels)
-        return _lib.DcnNormShape(_dtype(x), self.channels, tokens, self.gate_tokens, self.residual_scale, self.eps)
+                _whole(name, t, dtype, (self.channels,))
+        for name, t in sums:
+            if t is not None:
+                _whole(name, t, torch.float32, (self.channels,))
 
     def low_bytes(self, x) -> int:
         """Bytes of forward_dev's `low` for a residual stream like x."""
-        return int(self._lib.dcn_gated_norm_low_bytes(C.byref(self._shape(x, [], [], [("x", x)]))))
+        return int(self._lib.dcn_gated_norm_low_bytes(self._pack(x)))
 
     def _low(self, s, low, like, make: bool):
         """The pointer of the caller's low, or of the handle's own."""
-        count = self._lib.dcn_gated_norm_low_bytes(C.byref(s))
+        if like.dtype is torch.float32:
+            return None
+        count = self._lib.dcn_gated_norm_low_bytes(s)
         if not count:
             return None
         if low is not None:
@@ -302,12 +351,13 @@ class GatedNorm(_Handle):
         """gate, w_post, w_pre may be None (ones); y None: no block follows. rstd ([tokens][2]
         FP32) is what backward_dev reads; with it, 16-bit calls keep what rounding takes from
         x_out (low_bytes(x) uint8 values) in `low`, or in the handle for its next backward_dev."""
-        s = self._shape(x, [("gate", gate)], [("w_post", w_post, None), ("w_pre", w_pre, None)],
-                        [("h", h), ("x", x), ("x_out", x_out), ("y", y)])
+        s = self._pack(x)
+        self._check_all(x, (("h", h), ("x", x), ("x_out", x_out), ("y", y)), (("gate", gate),),
+                        (("w_post", w_post), ("w_pre", w_pre)))
         if rstd is not None:
-            _whole("rstd", rstd, torch.float32, x.shape[0], 2)
+            _whole("rstd", rstd, torch.float32, (x.shape[0], 2))
         self.ctx._check(self._lib.dcn_gated_norm_forward_dev(
-            self.ctx.ctx, C.byref(s), h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
+            self.ctx.ctx, s, h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
             x_out.data_ptr(), _ptr(y), _ptr(rstd), None if rstd is None else self._low(s, low, x, True),
             _stream(stream)))
 
@@ -317,13 +367,13 @@ class GatedNorm(_Handle):
         dw_pre (FP32) where they are given. Rows whose low halves are not those of the forward
         that made rstd (the handle ran another one since, and `low` is None) take x_out as it
         was rounded."""
-        s = self._shape(x_out, [("gate", gate), ("dgate", dgate)],
-                        [("w_post", w_post, None), ("w_pre", w_pre, None), ("dw_post", dw_post, torch.float32),
-                         ("dw_pre", dw_pre, torch.float32)],
-                        [("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dy", dy), ("dh", dh), ("dx", dx)])
-        _whole("rstd", rstd, torch.float32, x_out.shape[0], 2)
-        w, size = self._room(self._lib.dcn_gated_norm_workspace_bytes(C.byref(s)), x_out)
+        s = self._pack(x_out)
+        self._check_all(x_out, (("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dy", dy), ("dh", dh), ("dx", dx)),
+                        (("gate", gate), ("dgate", dgate)), (("w_post", w_post), ("w_pre", w_pre)),
+                        (("dw_post", dw_post), ("dw_pre", dw_pre)))
+        _whole("rstd", rstd, torch.float32, (x_out.shape[0], 2))
+        w, size = self._room(s, lambda: self._lib.dcn_gated_norm_workspace_bytes(s), x_out)
         self.ctx._check(self._lib.dcn_gated_norm_backward_dev(
-            self.ctx.ctx, C.byref(s), h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
+            self.ctx.ctx, s, h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
             rstd.data_ptr(), self._low(s, low, x_out, False), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw_post),
             _ptr(dw_pre), w, size, _stream(stream)))
