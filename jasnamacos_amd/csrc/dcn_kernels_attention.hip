@@ -216,8 +216,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionAr
     if (lane < 32) store_sums<D>(a, pl, index, st.m, l, kLift<T>);
 }
 
-template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kernel(AttentionArgs a, int splits) {
+template <typename T, int D, int WAVES, bool PAGED>
+__global__ __launch_bounds__(64 * WAVES, 1) void attention_few_kernel(AttentionArgs a, int splits) {
     constexpr int ROWS = 32, BYTES = ROWS * D * 2, COPIES = 2 * ROWS / Tile<D>::kRowsPerCopy;
     extern __shared__ __attribute__((aligned(1024))) char lds[];  // [wave][2][2][BYTES], then the join
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -244,15 +244,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kerne
         copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(from + wave), pages, own, own + BYTES, 0, lane);
     }
     unsigned long long holes = pages.holes;
-    if (from + wave + kWaves < to) next.find(keys, list.tile(from + wave + kWaves), 0);
+    if (from + wave + WAVES < to) next.find(keys, list.tile(from + wave + WAVES), 0);
     st.settle();
-    for (int i = from + wave; i < to; i += kWaves, ++n) {
+    for (int i = from + wave; i < to; i += WAVES, ++n) {
         char *kt = own + (n & 1) * 2 * BYTES, *vt = kt + BYTES, *other = own + ((n + 1) & 1) * 2 * BYTES;
         const int t0 = list.tile(i);
-        if (i + kWaves < to) {
+        if (i + WAVES < to) {
             pages = next;
-            copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(i + kWaves), pages, other, other + BYTES, 0, lane);
-            if (i + 2 * kWaves < to) next.find(keys, list.tile(i + 2 * kWaves), 0);
+            copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(i + WAVES), pages, other, other + BYTES, 0, lane);
+            if (i + 2 * WAVES < to) next.find(keys, list.tile(i + 2 * WAVES), 0);
             wait_copies<COPIES>();
         } else {
             wait_copies<0>();
@@ -282,14 +282,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kerne
         line[D + 1] = l;
     }
     __syncthreads();
-    // Eight threads a row.
-    const int jr = threadIdx.x >> 3, part = threadIdx.x & 7;
+    // Two threads a row and wave.
+    constexpr int share = 2 * WAVES;
+    const int jr = threadIdx.x / share, part = threadIdx.x % share;
     if (pl.row0 + jr > last_row) return;
-    float m = -INFINITY, sum = 0.f, w[kWaves];
+    float m = -INFINITY, sum = 0.f, w[WAVES];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, mem[(i * 32 + jr) * LINE + D]);
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, mem[(i * 32 + jr) * LINE + D]);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         w[i] = exp2f(mem[(i * 32 + jr) * LINE + D] - (m == -INFINITY ? 0.f : m));
         sum = fmaf(w[i], mem[(i * 32 + jr) * LINE + D + 1], sum);
     }
@@ -297,10 +298,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kerne
     const int64_t row = pl.q.first + tok, index = row * a.q_heads + head;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int at = part * 4; at < D; at += 32) {
+    for (int at = part * 4; at < D; at += 4 * share) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             const f32x4 v = *(const f32x4*)(mem + (i * 32 + jr) * LINE + at);
 #pragma unroll
             for (int b = 0; b < 4; ++b) o[b] = fmaf(w[i], v[b], o[b]);
@@ -311,75 +312,127 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_few_kerne
     if (part == 0) store_sums<D>(a, pl, index, m, sum, kLift<T>);
 }
 
-// One wave a row and head: the parts of all splits, in their order.
-template <typename T, int D>
+// The parts of all splits (32 at most) of a row and head, by PER waves: lane s of each has split
+// s's maximum and sum; the waves take the splits' sums in turn and are added in order.
+template <typename T, int D, int PER>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionArgs a, int splits) {
-    const int lane = threadIdx.x & 63;
+    typedef float vec __attribute__((ext_vector_type(2)));
+    constexpr int N = D / 64;
+    __shared__ vec sums[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const Run q = run_of(a.cu_q, blockIdx.z, a.max_q, a.q_tokens);
-    const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int64_t item = (int64_t)blockIdx.x * (kWaves / PER) + wave / PER;
     const int tok = (int)(item / a.q_heads), head = (int)(item % a.q_heads);
-    if (tok >= q.count || tok >= a.max_q) return;
-    const int64_t row = q.first + tok, index = row * a.q_heads + head;
+    const bool there = tok < q.count && tok < a.max_q;
+    const int64_t row = q.first + (there ? tok : 0), index = row * a.q_heads + head;
     const float* parts = (const float*)a.workspace + index * splits * (D + 4);
-    float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, parts[s * (D + 4) + D]);
-    float sum = 0.f, o[D / 64] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float* p = parts + s * (D + 4);
-        const float w = exp2f(p[D] - (m == -INFINITY ? 0.f : m));
-        sum = fmaf(w, p[D + 1], sum);
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) o[i] = fmaf(w, p[lane + 64 * i], o[i]);
+    float m = -INFINITY, l = 0.f;
+    if (there && lane < splits) {
+        m = parts[lane * (D + 4) + D];
+        l = parts[lane * (D + 4) + D + 1];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = (T*)a.out.p + row * a.out.ts + head * a.out.hs;
+    const float top = wave_max(m);
+    const float w = exp2f(m - (top == -INFINITY ? 0.f : top)), sum = wave_sum(w * l);
+    float o[2] = {};
+    if (there) {
+        const float* at = parts + lane * N;
+        for (int s = wave % PER; s < splits; s += 4 * PER) {
+            // Four splits' loads at once.
+            float v[4][N];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) out[lane + 64 * i] = narrow<T>(o[i] * inv);
-    if (a.lse && lane == 0) a.lse[index] = sum == 0.f ? -INFINITY : (m - kLift<T> + __builtin_amdgcn_logf(sum)) * kLn2;
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[u][i] = s + u * PER < splits ? at[(s + u * PER) * (D + 4) + i] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float ws = __shfl(w, (s + u * PER) & 63);
+#pragma unroll
+                for (int i = 0; i < N; ++i) o[i] = s + u * PER < splits ? fmaf(ws, v[u][i], o[i]) : o[i];
+            }
+        }
+    }
+    if constexpr (PER > 1) {
+        sums[wave][lane] = vec{o[0], o[1]};
+        __syncthreads();
+        if (wave % PER) return;
+#pragma unroll
+        for (int g = 1; g < PER; ++g) {
+            o[0] += sums[wave + g][lane][0];
+            o[1] += sums[wave + g][lane][1];
+        }
+    }
+    if (!there) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)a.out.p + row * a.out.ts + head * a.out.hs + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = narrow<T>(o[i] * inv);
+    if (a.lse && lane == 0) a.lse[index] = sum == 0.f ? -INFINITY : (top - kLift<T> + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // Row blocks, and over how many workgroups each one's key tiles are split.
 struct Plan {
     bool few;
-    int blocks, splits;
+    int waves, blocks, splits;
 };
-Plan plan_of(int sequences, int kv_heads, int group, int max_q, int max_kv, int frame, int back, int sinks) {
+Plan plan_of(int dim, int sequences, int kv_heads, int group, int max_q, int max_kv, int frame, int back, int sinks) {
     Plan p;
-    const int64_t rows = (int64_t)max_q * group;
-    p.few = rows <= 32;
+    const int64_t rows = (int64_t)max_q * group, wide = (rows + 127) / 128 * kv_heads * sequences;
+    // Keys that one block of `block` rows sees at most.
+    const auto keys_of = [&](int block, int tile) {
+        const int64_t window = back < 0 ? max_kv : ((int64_t)back + 1 + sinks) * frame + block / group + 2 * tile;
+        return window < max_kv ? window : (int64_t)max_kv;
+    };
+    const int64_t keys = keys_of(128, 64);
+    // Few rows, or so few workgroups of 128 rows that 32-row ones with four (eight) waves on the keys
+    // are done sooner, though each key tile is read four times as often (256 x 128 rows, 64
+    // channels: 29.9 -> 21.5 us; 64 x 128 rows of 8,000 keys, 128 channels: 59 -> 103).
+    p.few = rows <= 32 || (dim == 64 ? wide <= 256 && keys <= 4096 : wide <= 128 && keys <= 2048);
     const int per_block = p.few ? 32 : 128, tile = p.few ? 32 : 64;
     p.blocks = (int)((rows + per_block - 1) / per_block);
-    // Keys that one row block sees at most.
-    int64_t keys = max_kv;
-    if (back >= 0) {
-        const int64_t window = ((int64_t)back + 1 + sinks) * frame + per_block / group + 2 * tile;
-        keys = window < keys ? window : keys;
+    const int64_t tiles = (keys_of(per_block, tile) + tile - 1) / tile, groups = (int64_t)p.blocks * kv_heads * sequences;
+    p.waves = p.few && dim == 64 && groups <= 256 ? 8 : 4;
+    // Blocks that leave half of the CUs idle or more split their tiles: until every CU has as many
+    // workgroups as its LDS takes (one of the few kernel's with 128 channels, else two), a tile a
+    // wave (tile kernel: four) being the least, and 32 parts the most that the join adds quickly.
+    // Up to four tiles a wave the join would cost more than it saves: one token of 777 keys, 8
+    // heads of 64: 8.9 us in one part, 9.7 in three; of 1,500 keys 12.8 and 10.0.
+    const int64_t least = p.few ? p.waves : 4, room = p.few && dim == 128 ? 256 : 512;
+    int64_t splits = 1;
+    if (groups > 0 && groups <= 128 && tiles > 4 * least) {
+        splits = (room + groups - 1) / groups;
+        splits = splits < tiles / least ? splits : tiles / least;
+        splits = splits < 32 ? splits : 32;
     }
-    const int64_t tiles = (keys + tile - 1) / tile, groups = (int64_t)p.blocks * kv_heads * sequences;
-    // Two workgroups a CU, each with at least four tiles (few: four a wave).
-    const int64_t least = p.few ? 16 : 4;
-    int64_t splits = groups > 0 ? (512 + groups - 1) / groups : 1;
-    if (splits > tiles / least) splits = tiles / least;
-    p.splits = (int)(splits < 1 ? 1 : (splits > 64 ? 64 : splits));
+    p.splits = (int)splits;
     return p;
+}
+
+template <typename T, int D, int WAVES, bool PAGED>
+hipError_t run_few(const AttentionArgs& a, const Plan& p, const dim3& grid, hipStream_t stream) {
+    constexpr int copies = WAVES * 4 * 32 * D * 2, join = WAVES * 32 * (D + 4) * 4;
+    constexpr int bytes = copies > join ? copies : join;
+    if (hipError_t e = allow_dynamic_lds((const void*)attention_few_kernel<T, D, WAVES, PAGED>, bytes)) return e;
+    attention_few_kernel<T, D, WAVES, PAGED><<<grid, 64 * WAVES, bytes, stream>>>(a, p.splits);
+    return hipGetLastError();
 }
 
 template <typename T, int D, bool PAGED>
 hipError_t run(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
     const dim3 grid((unsigned)p.blocks * p.splits, a.kv_heads, a.sequences);
     if (p.few) {
-        constexpr int copies = kWaves * 4 * 32 * D * 2, join = kWaves * 32 * (D + 4) * 4;
-        constexpr int bytes = copies > join ? copies : join;
-        const void* f = (const void*)attention_few_kernel<T, D, PAGED>;
-        if (hipError_t e = allow_dynamic_lds(f, bytes)) return e;
-        attention_few_kernel<T, D, PAGED><<<grid, kThreads, bytes, stream>>>(a, p.splits);
+        if (hipError_t e = p.waves == 8 ? run_few<T, D, D == 64 ? 8 : 4, PAGED>(a, p, grid, stream)
+                                                   : run_few<T, D, 4, PAGED>(a, p, grid, stream))
+            return e;
     } else {
         attention_tile_kernel<T, D, PAGED><<<grid, kThreads, 0, stream>>>(a, p.splits);
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (p.splits == 1) return hipSuccess;
     const int64_t rows = (int64_t)a.max_q * a.q_heads;
-    attention_join_kernel<T, D><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, p.splits);
+    if (p.splits <= 8)
+        attention_join_kernel<T, D, 1><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, p.splits);
+    else
+        attention_join_kernel<T, D, kWaves><<<dim3((unsigned)rows, 1, a.sequences), kThreads, 0, stream>>>(a, p.splits);
     return hipGetLastError();
 }
 
@@ -396,12 +449,12 @@ hipError_t by_dim(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
 }  // namespace fa
 
 size_t attention_forward_workspace(const dcn_attention_shape& s) {
-    const fa::Plan p = fa::plan_of(s.sequences, s.kv_heads, s.q_heads / s.kv_heads, s.max_q, s.max_kv, s.frame_tokens, s.back, s.sinks);
+    const fa::Plan p = fa::plan_of(s.head_dim, s.sequences, s.kv_heads, s.q_heads / s.kv_heads, s.max_q, s.max_kv, s.frame_tokens, s.back, s.sinks);
     return p.splits == 1 ? 0 : (size_t)s.q_tokens * s.q_heads * p.splits * (s.head_dim + 4) * sizeof(float);
 }
 
 hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream) {
-    const fa::Plan p = fa::plan_of(a.sequences, a.kv_heads, a.group, a.max_q, a.max_kv, a.frame, a.back, a.sinks);
+    const fa::Plan p = fa::plan_of(a.dim, a.sequences, a.kv_heads, a.group, a.max_q, a.max_kv, a.frame, a.back, a.sinks);
     return dtype == DCN_DTYPE_F16 ? fa::by_dim<_Float16>(a, p, stream) : fa::by_dim<fa::bf16>(a, p, stream);
 }
 
