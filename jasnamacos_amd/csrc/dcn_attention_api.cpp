@@ -150,10 +150,11 @@ bool matrix_heads(const dcn_attention_shape* s) {
     return s->dtype != DCN_DTYPE_F32 && (s->head_dim == 64 || s->head_dim == 128) && s->scale > 0.f &&
            (int64_t)s->max_q * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
 }
-// 16-byte rows, and rows of one tile within 32-bit offsets.
+// 16-byte rows, and the rows of one tile (64 tokens, the heads of a group) within 32-bit offsets.
 template <typename H>
-bool matrix_tensor(const H& h) {
-    return (uintptr_t)h.p % 16 == 0 && h.ts % 8 == 0 && h.hs % 8 == 0 && h.ts < (INT64_C(1) << 24);
+bool matrix_tensor(const H& h, int group = 1) {
+    return (uintptr_t)h.p % 16 == 0 && h.ts % 8 == 0 && h.hs % 8 == 0 && h.ts < (INT64_C(1) << 24) &&
+           (group - 1) * h.hs < (INT64_C(1) << 29);
 }
 // Pages of whole runs of 8 keys, and rows of the pool that an int counts.
 bool matrix_pool(const dcn_cache* c) { return c->page_tokens >= 8 && (int64_t)c->pages * c->page_tokens <= INT32_MAX; }
@@ -425,7 +426,7 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
         if (!shape->q_tokens) a.max_q = 0;
         if (!shape->kv_tokens) a.max_kv = 0;
         bool matrix = matrix_heads(shape);
-        for (const dcn::HeadsIn* h : {&a.q, &a.k, &a.v, &a.o, &a.dout}) matrix = matrix && matrix_tensor(*h);
+        for (const dcn::HeadsIn* h : {&a.q, &a.k, &a.v, &a.o, &a.dout}) matrix = matrix && matrix_tensor(*h, a.group);
         for (const dcn::HeadsOut* h : {&a.dq, &a.dk, &a.dv}) matrix = matrix && matrix_tensor(*h);
         DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix_backward : dcn::launch_attention_rows_backward)(shape->dtype, a,
                                                                                                           (hipStream_t)stream));

@@ -211,53 +211,94 @@ struct TilePages {
     }
 };
 
-// Copies the tile of ROWS keys from t0 (below the sequence's end) to `k` and `v`; this wave's
-// part. Contiguous rows past the end are copies of the last one.
+// This wave's part of the copies of key tiles: byte offsets of its lanes from the tile's first
+// key (paged: from each instruction's first key), the same for every tile but the last.
 template <int D, int ROWS, int WAVES, bool PAGED>
-__device__ __forceinline__ void copy_tile(const Keys<PAGED>& keys, int t0, const TilePages<D, ROWS, WAVES, PAGED>& pages, char* k,
-                                          char* v, int wave, int lane) {
+struct TileCopy {
     using Ti = Tile<D>;
-    const char* kb = keys.kp + (int64_t)t0 * keys.k.ts * 2;
-    const char* vb = keys.vp + (int64_t)t0 * keys.v.ts * 2;
-    const int last = keys.count - 1 - t0;
-#pragma unroll
-    for (int n = 0; n < pages.kCopies; ++n) {
-        const int i = n * WAVES + wave, r = Ti::copy_row(i, lane), c = Ti::copy_channel(r, lane);
-        if constexpr (PAGED) {
-            const uint32_t in = lane / Ti::kChunks;
-            copy16(keys.kp + (int64_t)pages.row[n] * keys.k.ts * 2, (in * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
-            copy16(keys.vp + (int64_t)pages.row[n] * keys.v.ts * 2, (in * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
-        } else {
-            const uint32_t at = r < last ? r : last;
-            copy16(kb, (at * (uint32_t)keys.k.ts + c) * 2, k + i * 1024);
-            copy16(vb, (at * (uint32_t)keys.v.ts + c) * 2, v + i * 1024);
-        }
-    }
-}
+    static constexpr int kCopies = ROWS / Ti::kRowsPerCopy / WAVES;
+    static constexpr int kOffsets = PAGED ? 1 : kCopies;
+    uint32_t k[kOffsets], v[kOffsets];
 
-// Whether a tile holds infinities or NaN in the chunks that a thread looks at.
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ bool tile_nonfinite(const char* v, int thread, int threads) {
-    bool bad = false;
-    for (int i = thread; i < ROWS * D / 8; i += threads) {
-        u32x4 x = *(const u32x4*)(v + i * 16);
-        bad |= clean16<T>(x);
-    }
-    return bad;
-}
-// Zeros for the infinities and NaN of a tile, by `threads` threads; whether a thread saw one.
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ bool clean_tile(char* v, int thread, int threads) {
-    bool bad = false;
-    for (int i = thread; i < ROWS * D / 8; i += threads) {
-        u32x4 x = *(const u32x4*)(v + i * 16);
-        if (clean16<T>(x)) {
-            *(u32x4*)(v + i * 16) = x;
-            bad = true;
+    // Rows past `last` stand for it (contiguous keys only: a page is there whole).
+    __device__ __forceinline__ void set(const Keys<PAGED>& keys, int last, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < kOffsets; ++n) {
+            const int in = PAGED ? lane / Ti::kChunks : Ti::copy_row(n * WAVES + wave, lane);
+            const uint32_t at = PAGED || in < last ? in : last;
+            k[n] = at * (uint32_t)keys.k.ts * 2;
+            v[n] = at * (uint32_t)keys.v.ts * 2;
+            if (!PAGED) {
+                k[n] += Ti::copy_channel(in, lane) * 2;
+                v[n] += Ti::copy_channel(in, lane) * 2;
+            }
         }
     }
-    return bad;
+    // The tile from key t0 (below the sequence's end) to `kt` and `vt`.
+    __device__ __forceinline__ void copy(const Keys<PAGED>& keys, int t0, const TilePages<D, ROWS, WAVES, PAGED>& pages, char* kt,
+                                         char* vt, int wave, int lane) {
+        if (!PAGED && t0 + ROWS > keys.count) set(keys, keys.count - 1 - t0, wave, lane);
+        const char* kb = keys.kp + (int64_t)t0 * keys.k.ts * 2;
+        const char* vb = keys.vp + (int64_t)t0 * keys.v.ts * 2;
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) {
+            const int i = n * WAVES + wave;
+            if constexpr (PAGED) {
+                const uint32_t c = Ti::copy_channel(Ti::copy_row(i, lane), lane) * 2;
+                copy16(keys.kp + (int64_t)pages.row[n] * keys.k.ts * 2, k[0] + c, kt + i * 1024);
+                copy16(keys.vp + (int64_t)pages.row[n] * keys.v.ts * 2, v[0] + c, vt + i * 1024);
+            } else {
+                copy16(kb, k[n], kt + i * 1024);
+                copy16(vb, v[n], vt + i * 1024);
+            }
+        }
+    }
+};
+
+// Whether any of eight values is infinite or NaN: its exponent's ones carry into the sign's place.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(u32x4 v) {
+    constexpr uint32_t e = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u, one = __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t |= (v[i] & e) + one;
+    return t & 0x80008000u;
 }
+// Zeros for the infinities and NaN of the rows of a tile that this wave has copied (and that
+// have arrived); a bit, in every lane, for each row that had one.
+template <typename T, int D, int ROWS, int WAVES>
+__device__ __forceinline__ unsigned long long clean_own(char* tile, int wave, int lane) {
+    using Ti = Tile<D>;
+    constexpr int n = ROWS / Ti::kRowsPerCopy / WAVES;
+    u32x4 v[n];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+        v[i] = *(const u32x4*)(tile + (i * WAVES + wave) * 1024 + lane * 16);
+        bad |= any_nonfinite<T>(v[i]);
+    }
+    if (__builtin_expect(!__any(bad), 1)) return 0;
+    unsigned long long rows = 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+        if (clean16<T>(v[i])) {
+            *(u32x4*)(tile + (i * WAVES + wave) * 1024 + lane * 16) = v[i];
+            rows |= 1ull << Ti::copy_row(i * WAVES + wave, lane);
+        }
+    for (int d = 32; d; d >>= 1) rows |= __shfl_xor(rows, d);
+    return rows;
+}
+// What the waves of a workgroup found in a tile, exchanged over the barrier that the tile waits
+// for: one slot a wave and buffer.
+struct FoundRows {
+    unsigned long long wave[2][kWaves];
+    __device__ __forceinline__ unsigned long long all(int buf) const {
+        unsigned long long r = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) r |= wave[buf][w];
+        return r;
+    }
+};
 
 // Infinities and NaN of one row of 16-bit channels, which stand as zeros in LDS, to a lane's sums
 // (o^T: channels 32 i + 8 a + 4 h + b) if `on`.
@@ -311,6 +352,22 @@ __device__ __forceinline__ void load_row(u32x4* to, const HeadsIn& t, const Atte
     const char* p = (const char*)t.p + ((pl.q.first + tok) * t.ts + head * t.hs + 8 * (lane >> 5)) * 2;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) to[i] = *(const u32x4*)(p + i * 32);
+}
+
+// Bits [0, n) of 64.
+__device__ __forceinline__ unsigned long long bits_below(int n) {
+    return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
+}
+// A bit for each of 64 keys from t0 that a row sees.
+__device__ __forceinline__ unsigned long long seen_bits(const Span& s, int t0) {
+    return (bits_below(s.hi - t0) & ~bits_below(s.lo - t0)) | bits_below(s.sink - t0);
+}
+// All ones if bit `in` of a lane's 64 is set: a constant `in` makes it one instruction.
+__device__ __forceinline__ uint32_t spread_bit(unsigned long long bits, int in) {
+    return (uint32_t)((int32_t)((uint32_t)(bits >> (in & 32)) << (31 - (in & 31))) >> 31);
+}
+__device__ __forceinline__ float keep_or(float v, uint32_t mask, float other) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & mask) | (__builtin_bit_cast(uint32_t, other) & ~mask));
 }
 
 struct Spread {

@@ -74,17 +74,13 @@ struct RowState {
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) vf[st][i] = Ti::columns(vt, st >> 1, st & 1, i, lane);
         __builtin_amdgcn_sched_barrier(0);
-        const int base = t0 + 4 * (lane >> 5);
         if (masked) {
-            const unsigned long long gone = holes >> (4 * (lane >> 5));
+            const unsigned long long seen = (seen_bits(sp, t0) & ~holes) >> (4 * (lane >> 5));
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int in = 32 * mb + 8 * (r >> 2) + (r & 3), j = base + in;
-                    const bool on = sees(sp, j) && !((uint32_t)(gone >> (in & 32)) >> (in & 31) & 1);
-                    s[mb][r] = on ? s[mb][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)
+                    s[mb][r] = keep_or(s[mb][r], spread_bit(seen, 32 * mb + 8 * (r >> 2) + (r & 3)), -INFINITY);
         }
         float top = s[0][0];
 #pragma unroll
@@ -157,6 +153,7 @@ template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionArgs a, int splits) {
     constexpr int ROWS = 64, BYTES = ROWS * D * 2;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
+    __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
     if (!place_of<32 * kWaves>(a, splits, &pl)) return;
@@ -177,25 +174,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionAr
     const Keys<PAGED> keys(a, pl.seq, pl.kh, pl.kv);
     const float c = a.scale * kLog2e;
     TilePages<D, ROWS, kWaves, PAGED> pages, next;  // of the tile whose copies are next; one further
+    TileCopy<D, ROWS, kWaves, PAGED> copies;
     if (from < to) {
+        copies.set(keys, ROWS, wave, lane);
         pages.find(keys, list.tile(from), wave);
-        copy_tile<D, ROWS, kWaves, PAGED>(keys, list.tile(from), pages, lds[0][0], lds[0][1], wave, lane);
+        copies.copy(keys, list.tile(from), pages, lds[0][0], lds[0][1], wave, lane);
     }
     unsigned long long holes = pages.holes;
     if (from + 1 < to) next.find(keys, list.tile(from + 1), wave);
     st.settle();
     for (int i = from; i < to; ++i) {
-        char(*now)[BYTES] = lds[(i - from) & 1], (*other)[BYTES] = lds[((i - from) & 1) ^ 1];
-        const int t0 = list.tile(i);
+        const int buf = (i - from) & 1, t0 = list.tile(i);
+        char(*now)[BYTES] = lds[buf], (*other)[BYTES] = lds[buf ^ 1];
         wait_copies<0>();
+        // Values that are not finite matter where some row does not see all of the tile: zero times
+        // them is not zero. Each wave looks at what it copied.
+        const bool partial = holes || !all_see<ROWS>(all, t0);
+        if (partial) found.wave[buf][wave] = clean_own<T, D, ROWS, kWaves>(now[1], wave, lane);
         __syncthreads();
         if (i + 1 < to) {
             pages = next;
-            copy_tile<D, ROWS, kWaves, PAGED>(keys, list.tile(i + 1), pages, other[0], other[1], wave, lane);
+            copies.copy(keys, list.tile(i + 1), pages, other[0], other[1], wave, lane);
             if (i + 2 < to) next.find(keys, list.tile(i + 2), wave);
         }
-        bool bad = false;
-        if (holes || !all_see<ROWS>(all, t0)) bad = __syncthreads_or(clean_tile<T, D, ROWS>(now[1], threadIdx.x, kThreads));
+        const bool bad = partial && uniform(found.all(buf) != 0);
         if (!idle && !none_sees<ROWS>(mine, t0)) {
             st.template add<ROWS>(now[0], now[1], t0, c, holes || !all_see<ROWS>(mine, t0), holes, lane);
             if (bad) add_nonfinite<T, D>(st.o, st.sp, t0, keys.end(t0 + ROWS), holes, lane, [&](int j) { return keys.value(j); });
@@ -239,9 +241,11 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_few_kernel(AttentionA
     char* own = lds + wave * 4 * BYTES;
     int n = 0;
     TilePages<D, ROWS, 1, PAGED> pages, next;
+    TileCopy<D, ROWS, 1, PAGED> copies;
     if (from + wave < to) {
+        copies.set(keys, ROWS, 0, lane);
         pages.find(keys, list.tile(from + wave), 0);
-        copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(from + wave), pages, own, own + BYTES, 0, lane);
+        copies.copy(keys, list.tile(from + wave), pages, own, own + BYTES, 0, lane);
     }
     unsigned long long holes = pages.holes;
     if (from + wave + WAVES < to) next.find(keys, list.tile(from + wave + WAVES), 0);
@@ -251,15 +255,14 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_few_kernel(AttentionA
         const int t0 = list.tile(i);
         if (i + WAVES < to) {
             pages = next;
-            copy_tile<D, ROWS, 1, PAGED>(keys, list.tile(i + WAVES), pages, other, other + BYTES, 0, lane);
+            copies.copy(keys, list.tile(i + WAVES), pages, other, other + BYTES, 0, lane);
             if (i + 2 * WAVES < to) next.find(keys, list.tile(i + 2 * WAVES), 0);
             wait_copies<COPIES>();
         } else {
             wait_copies<0>();
         }
         const bool whole = !holes && all_see<ROWS>(all, t0);
-        bool bad = false;
-        if (!whole) bad = __any(clean_tile<T, D, ROWS>(vt, lane, 64));
+        const bool bad = !whole && clean_own<T, D, ROWS, 1>(vt, 0, lane);
         st.template add<ROWS>(kt, vt, t0, c, !whole, holes, lane);
         if (bad) add_nonfinite<T, D>(st.o, st.sp, t0, keys.end(t0 + ROWS), holes, lane, [&](int j) { return keys.value(j); });
         holes = pages.holes;

@@ -51,22 +51,6 @@ __device__ __forceinline__ void follow_scale(float top, float* up, f32x16* sum) 
     *up = next;
 }
 
-// Zeros for a tile's infinities and NaN, by the whole workgroup; a bit for each row that had one.
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ unsigned long long clean_rows(char* tile, unsigned long long* mask, int thread) {
-    if (thread == 0) *mask = 0;
-    __syncthreads();
-    for (int i = thread; i < ROWS * D / 8; i += kThreads) {
-        u32x4 x = *(const u32x4*)(tile + i * 16);
-        if (clean16<T>(x)) {
-            *(u32x4*)(tile + i * 16) = x;
-            atomicOr(mask, 1ull << (i / (D / 8)));
-        }
-    }
-    __syncthreads();
-    return *mask;
-}
-
 // Keys of a tile of the first pass: with 128 channels a wave's operands and sums leave registers
 // for 32 keys' dS.
 template <int D>
@@ -77,7 +61,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
     constexpr int ROWS = kDqKeys<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
-    __shared__ unsigned long long row_mask;
+    __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
     if (!place_of<32 * kWaves>(a, 1, &pl)) return;
@@ -94,7 +78,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
     const TileList<ROWS> list(all);
     const Keys<false> keys(a, pl.seq, pl.kh, pl.kv);
     TilePages<D, ROWS, kWaves, false> none;
-    if (list.count) copy_tile<D, ROWS, kWaves, false>(keys, list.tile(0), none, lds[0][0], lds[0][1], wave, lane);
+    TileCopy<D, ROWS, kWaves, false> copies;
+    copies.set(keys, ROWS, wave, lane);
+    if (list.count) copies.copy(keys, list.tile(0), none, lds[0][0], lds[0][1], wave, lane);
     u32x4 q[D / 16], go[D / 16];
     load_row<D>(q, a.q, a, pl, rw, r, lane);
     load_row<D>(go, a.dout, a, pl, rw, r, lane);
@@ -131,18 +117,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
     if (sum_delta) delta = 0.f;
     const int steps = sum_delta ? 2 * list.count : list.count;
     for (int step = 0, i = 0; step < steps; ++step, i = i + 1 < list.count ? i + 1 : 0) {
-        char(*now)[BYTES] = lds[step & 1], (*other)[BYTES] = lds[(step & 1) ^ 1];
-        const int t0 = list.tile(i);
+        const int buf = step & 1, t0 = list.tile(i);
+        char(*now)[BYTES] = lds[buf], (*other)[BYTES] = lds[buf ^ 1];
         wait_copies<0>();
-        __syncthreads();
-        if (step + 1 < steps)
-            copy_tile<D, ROWS, kWaves, false>(keys, list.tile(i + 1 < list.count ? i + 1 : 0), none, other[0], other[1], wave, lane);
-        const bool delta_step = sum_delta && step < list.count;
         // Keys that are not finite, where some row does not see all of the tile: zeros in LDS, and
-        // the scores of the rows that see them are NaN.
-        unsigned long long poison = 0;
-        if (!all_see<ROWS>(all, t0) && __syncthreads_or(tile_nonfinite<T, D, ROWS>(now[0], threadIdx.x, kThreads)))
-            poison = clean_rows<T, D, ROWS>(now[0], &row_mask, threadIdx.x);
+        // the scores of the rows that see them are NaN. Each wave looks at what it copied.
+        const bool partial = !all_see<ROWS>(all, t0);
+        if (partial) found.wave[buf][wave] = clean_own<T, D, ROWS, kWaves>(now[0], wave, lane);
+        __syncthreads();
+        if (step + 1 < steps) {
+            const int next = i + 1 < list.count ? i + 1 : 0;
+            if (!next) copies.set(keys, ROWS, wave, lane);
+            copies.copy(keys, list.tile(next), none, other[0], other[1], wave, lane);
+        }
+        const bool delta_step = sum_delta && step < list.count;
+        const unsigned long long poison = partial ? found.all(buf) : 0;
         if (!idle && !none_sees<ROWS>(mine, t0)) {
             const bool masked = !all_see<ROWS>(mine, t0) || poison;
 #pragma unroll
@@ -178,13 +167,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -lse)) * (dp[x] - delta);
                 if (masked) {
-                    const unsigned long long not_finite = poison >> (4 * (lane >> 5));
+                    if (__builtin_expect(poison != 0, 0)) {
+                        const unsigned long long not_finite = poison >> (4 * (lane >> 5));
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const int in = 32 * mb + 8 * (x >> 2) + (x & 3);
-                        if ((uint32_t)(not_finite >> (in & 32)) >> (in & 31) & 1) s[x] = NAN;
-                        s[x] = sees(sp, t0 + 4 * (lane >> 5) + in) ? s[x] : 0.f;
+                        for (int x = 0; x < 16; ++x)
+                            if (spread_bit(not_finite, 32 * mb + 8 * (x >> 2) + (x & 3))) s[x] = NAN;
                     }
+                    const unsigned long long seen = seen_bits(sp, t0) >> (4 * (lane >> 5));
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[x] = keep_or(s[x], spread_bit(seen, 32 * mb + 8 * (x >> 2) + (x & 3)), 0.f);
                 }
                 if (delta_step) {  // the sums are left as they are by a product with zeros
 #pragma unroll
@@ -272,8 +263,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
-    __shared__ __attribute__((aligned(16))) int row_at[2][ROWS];  // a row's position; -1: no row
-    __shared__ unsigned long long row_mask, row_mask2;
+    __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     int block, part, of;
     plan.item(blockIdx.x, &block, &part, &of);
@@ -318,30 +308,40 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     const int per = (tiles + of - 1) / of;
     const int begin = tile_from + part * per, stop = begin + per < tile_to ? begin + per : tile_to;
 
-    // Copies of the query tile at packed row r0, and its rows' lse, delta and positions.
-    auto copy = [&](int r0, char* to_q, char* to_do) {
+    // Copies of the query tile at packed row r0: byte offsets from the token of its first row, the
+    // same for every tile where the group divides 64, but for the last.
+    constexpr int kCopies = ROWS / Ti::kRowsPerCopy / kWaves;
+    uint32_t q_at[kCopies], o_at[kCopies];
+    const bool steady = ROWS % a.group == 0;
+    auto offsets = [&](int r0) {
+        const int rem = r0 - rw.token(r0) * a.group, last = q_rows - 1 - r0;
 #pragma unroll
-        for (int n = 0; n < ROWS / Ti::kRowsPerCopy / kWaves; ++n) {
-            const int i = n * kWaves + wave, in = Ti::copy_row(i, lane), c = Ti::copy_channel(in, lane);
-            const int r = r0 + in < q_rows ? r0 + in : q_rows - 1;
-            const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
-            const int64_t row = pl.q.first + tok;
-            copy16((const char*)a.q.p + (row * a.q.ts + head * a.q.hs + c) * 2, to_q + i * 1024);
-            copy16((const char*)a.dout.p + (row * a.dout.ts + head * a.dout.hs + c) * 2, to_do + i * 1024);
+        for (int n = 0; n < kCopies; ++n) {
+            const int in = Ti::copy_row(n * kWaves + wave, lane), c = Ti::copy_channel(in, lane), r = rem + (in < last ? in : last);
+            const int tok = rw.token(r), g = r - tok * a.group;
+            q_at[n] = (tok * (uint32_t)a.q.ts + g * (uint32_t)a.q.hs + c) * 2;
+            o_at[n] = (tok * (uint32_t)a.dout.ts + g * (uint32_t)a.dout.hs + c) * 2;
+        }
+    };
+    auto copy = [&](int r0, char* to_q, char* to_do) {
+        if (!steady || r0 + ROWS > q_rows) offsets(r0);
+        const int64_t row = pl.q.first + uniform(rw.token(r0)), head = pl.kh * a.group;
+        const char* qb = (const char*)a.q.p + (row * a.q.ts + head * a.q.hs) * 2;
+        const char* ob = (const char*)a.dout.p + (row * a.dout.ts + head * a.dout.hs) * 2;
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) {
+            copy16(qb, q_at[n], to_q + (n * kWaves + wave) * 1024);
+            copy16(ob, o_at[n], to_do + (n * kWaves + wave) * 1024);
         }
     };
     float next_lse = 0.f, next_delta = 0.f;
-    int next_at = -1;
     auto fetch = [&](int r0) {
-        if (threadIdx.x >= ROWS) return;
         const int r = r0 + (int)threadIdx.x;
-        next_at = -1;
-        if (r >= q_rows) return;
+        if (threadIdx.x >= ROWS || r >= q_rows) return;
         const int tok = rw.token(r), head = pl.kh * a.group + (r - tok * a.group);
         const int64_t index = (pl.q.first + tok) * a.q_heads + head;
         next_lse = a.lse_in[index] * kLog2e;
         next_delta = ((const float*)a.workspace)[index];
-        next_at = pl.offset + tok;
     };
     f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -352,6 +352,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     float up = kScaled<T> ? 0.f : 1.f;  // FP16: dS's factor of this key; 0: no dS seen yet
     if (begin < stop) {
         fetch(begin * ROWS);
+        offsets(begin * ROWS);
         copy(begin * ROWS, lds[0][0], lds[0][1]);
     }
 #pragma unroll
@@ -362,28 +363,34 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
         if (threadIdx.x < ROWS) {
             row_lse[buf][threadIdx.x] = next_lse;
             row_delta[buf][threadIdx.x] = next_delta;
-            row_at[buf][threadIdx.x] = next_at;
         }
+        // Positions of the tile's first and last row; whether this wave's keys (all of the block's)
+        // are seen by all of them.
+        const int rl = r0 + ROWS - 1 < q_rows ? r0 + ROWS - 1 : q_rows - 1;
+        const int t0 = rw.token(r0), p0 = pl.offset + t0, p1 = pl.offset + rw.token(rl);
+        const bool rows_there = r0 + ROWS <= q_rows && p0 >= 0;
+        const bool whole = rows_there && p0 >= wave_every.from && p1 < wave_every.to;
+        const bool partial = !(rows_there && p0 >= every.from && p1 < every.to);
         wait_copies<0>();
+        // Queries and gradients that are not finite, where some pair of the tile is not visible:
+        // zeros in LDS, and the weights of the pairs that are visible are NaN.
+        if (partial)
+            found.wave[buf][wave] = clean_own<T, D, ROWS, kWaves>(qt, wave, lane) | clean_own<T, D, ROWS, kWaves>(ot, wave, lane);
         __syncthreads();
         if (i + 1 < stop) {
             fetch(r0 + ROWS);
             copy(r0 + ROWS, lds[buf ^ 1][0], lds[buf ^ 1][1]);
         }
-        // Positions of the tile's first and last row; whether this wave's keys are seen by all of them.
-        const int rl = r0 + ROWS - 1 < q_rows ? r0 + ROWS - 1 : q_rows - 1;
-        const int p0 = pl.offset + rw.token(r0), p1 = pl.offset + rw.token(rl);
-        const bool rows_there = r0 + ROWS <= q_rows && p0 >= 0;
-        const bool whole = rows_there && p0 >= wave_every.from && p1 < wave_every.to;
-        const bool block_whole = rows_there && p0 >= every.from && p1 < every.to;
-        // Queries and gradients that are not finite, where some pair of the tile is not visible:
-        // zeros in LDS, and the weights of the pairs that are visible are NaN.
-        if (!block_whole && __syncthreads_or((int)tile_nonfinite<T, D, ROWS>(qt, threadIdx.x, kThreads) |
-                                             (int)tile_nonfinite<T, D, ROWS>(ot, threadIdx.x, kThreads))) {
-            const unsigned long long not_finite = clean_rows<T, D, ROWS>(qt, &row_mask, threadIdx.x) |
-                                                  clean_rows<T, D, ROWS>(ot, &row_mask2, threadIdx.x);
-            if (threadIdx.x < ROWS && (not_finite >> threadIdx.x & 1)) row_lse[buf][threadIdx.x] = NAN;
-            __syncthreads();
+        const unsigned long long poison = partial ? found.all(buf) : 0;
+        // A bit for each of the tile's rows that sees this lane's key: positions grow with the rows.
+        const bool masked = !whole || poison;
+        unsigned long long seen = 0;
+        if (masked) {
+            const int64_t rem = r0 - (int64_t)t0 * a.group;
+            const int64_t lo = ((int64_t)me.from - p0) * a.group - rem, hi = ((int64_t)me.to - p0) * a.group - rem;
+            const int64_t there = q_rows - r0, top = hi < there ? hi : there;
+            seen = bits_below((int)(top < 64 ? (top < 0 ? 0 : top) : 64)) & ~bits_below((int)(lo < 64 ? (lo < 0 ? 0 : lo) : 64));
+            seen >>= 4 * (lane >> 5);
         }
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
@@ -423,17 +430,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
                 s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[x >> 2][x & 3]));
                 dp[x] = s[x] * (dp[x] - d4[x >> 2][x & 3]);
             }
-            if (!whole) {
-                typedef int i32x4 __attribute__((ext_vector_type(4)));
+            if (masked) {
+                if (__builtin_expect(poison != 0, 0)) {
+                    const unsigned long long not_finite = poison >> (4 * (lane >> 5));
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const i32x4 at = *(const i32x4*)&row_at[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
+                    for (int x = 0; x < 16; ++x)
+                        if (spread_bit(not_finite, 32 * mb + 8 * (x >> 2) + (x & 3))) s[x] = dp[x] = NAN;
+                }
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const bool on = at[b] >= me.from && at[b] < me.to && at[b] >= 0;
-                        s[4 * g + b] = on ? s[4 * g + b] : 0.f;
-                        dp[4 * g + b] = on ? dp[4 * g + b] : 0.f;
-                    }
+                for (int x = 0; x < 16; ++x) {
+                    const uint32_t on = spread_bit(seen, 32 * mb + 8 * (x >> 2) + (x & 3));
+                    s[x] = keep_or(s[x], on, 0.f);
+                    dp[x] = keep_or(dp[x], on, 0.f);
                 }
             }
             if constexpr (kScaled<T>) {
