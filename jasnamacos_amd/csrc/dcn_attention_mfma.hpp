@@ -143,6 +143,32 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
+// Workgroups on the card's eight XCDs, each with an L2 of its own: workgroup i runs on XCD i % 8.
+// The blocks of one (sequence, key head) read the same keys, so they stay on one XCD where the
+// number of pairs is a multiple of 8, or else share as few XCDs as spread the work evenly, taking
+// blocks in turn. `x` blocks a pair.
+struct BlockMap {
+    int x, heads, pairs, classes;  // classes: the greatest common divisor of pairs and 8
+    unsigned grid;
+};
+inline bool block_map(int64_t x, int64_t heads, int64_t sequences, BlockMap* m) {
+    const int64_t pairs = heads * sequences, classes = pairs % 8 == 0 ? 8 : (pairs % 4 == 0 ? 4 : (pairs % 2 == 0 ? 2 : 1));
+    const int64_t share = 8 / classes, each = (pairs / classes * x + share - 1) / share;
+    *m = BlockMap{(int)x, (int)heads, (int)pairs, (int)classes, (unsigned)(8 * each)};
+    return 8 * each < INT32_MAX && x < INT32_MAX;
+}
+// Block, key head and sequence of this workgroup; false for the padding.
+__device__ __forceinline__ bool block_of(const BlockMap& m, int* block, int* head, int* sequence) {
+    const int xcd = blockIdx.x & 7, share = 8 / m.classes;
+    const int item = (int)(blockIdx.x >> 3) * share + xcd / m.classes;
+    const int nth = item / m.x, pair = xcd % m.classes + m.classes * nth;
+    if (pair >= m.pairs) return false;
+    *block = item - nth * m.x;
+    *head = pair % m.heads;
+    *sequence = pair / m.heads;
+    return true;
+}
+
 // Where one workgroup works.
 struct Place {
     int seq, kh, split, splits;
@@ -324,14 +350,14 @@ __device__ __forceinline__ void add_nonfinite(f32x16* o, const Span& sp, int t0,
         if (const uint16_t* v = row(j)) add_nonfinite<T, D>(o, v, sees(sp, j) && !(holes >> (j - t0) & 1), lane);
 }
 
-// blockIdx.x = split + splits * row block (the last rows first: they see the most keys).
+// A pair's blocks are split + splits * row block, the last rows first: they see the most keys.
 template <int ROWS_WG>
-__device__ __forceinline__ bool place_of(const AttentionArgs& a, int splits, Place* pl) {
-    pl->seq = blockIdx.z;
-    pl->kh = blockIdx.y;
+__device__ __forceinline__ bool place_of(const AttentionArgs& a, const BlockMap& map, int splits, Place* pl) {
+    int at;
+    if (!block_of(map, &at, &pl->kh, &pl->seq)) return false;
     pl->splits = splits;
-    const int block = gridDim.x / splits - 1 - blockIdx.x / splits;
-    pl->split = blockIdx.x % splits;
+    const int block = map.x / splits - 1 - at / splits;
+    pl->split = at % splits;
     pl->q = run_of(a.cu_q, pl->seq, a.max_q, a.q_tokens);
     pl->kv = kv_run_of(a, pl->seq);
     pl->q.count = uniform(pl->q.count);

@@ -150,13 +150,13 @@ __device__ __forceinline__ void store_sums(const AttentionArgs& a, const Place& 
 }
 
 template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionArgs a, int splits) {
+__global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionArgs a, BlockMap map, int splits) {
     constexpr int ROWS = 64, BYTES = ROWS * D * 2;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
-    if (!place_of<32 * kWaves>(a, splits, &pl)) return;
+    if (!place_of<32 * kWaves>(a, map, splits, &pl)) return;
     const Rows rw = rows_of(a.group);
     const int last_row = pl.rows - 1;
     const int w0 = pl.row0 + 32 * wave, w1 = w0 + 31 < last_row ? w0 + 31 : last_row;
@@ -219,12 +219,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_tile_kernel(AttentionAr
 }
 
 template <typename T, int D, int WAVES, bool PAGED>
-__global__ __launch_bounds__(64 * WAVES, 1) void attention_few_kernel(AttentionArgs a, int splits) {
+__global__ __launch_bounds__(64 * WAVES, 1) void attention_few_kernel(AttentionArgs a, BlockMap map, int splits) {
     constexpr int ROWS = 32, BYTES = ROWS * D * 2, COPIES = 2 * ROWS / Tile<D>::kRowsPerCopy;
     extern __shared__ __attribute__((aligned(1024))) char lds[];  // [wave][2][2][BYTES], then the join
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
-    if (!place_of<32>(a, splits, &pl)) return;
+    if (!place_of<32>(a, map, splits, &pl)) return;
     const Rows rw = rows_of(a.group);
     const int last_row = pl.rows - 1;
     const Spread all = spread_of(a, pl, rw, pl.row0, pl.row0 + 31 < last_row ? pl.row0 + 31 : last_row);
@@ -411,23 +411,24 @@ Plan plan_of(int dim, int sequences, int kv_heads, int group, int max_q, int max
 }
 
 template <typename T, int D, int WAVES, bool PAGED>
-hipError_t run_few(const AttentionArgs& a, const Plan& p, const dim3& grid, hipStream_t stream) {
+hipError_t run_few(const AttentionArgs& a, const Plan& p, const BlockMap& map, hipStream_t stream) {
     constexpr int copies = WAVES * 4 * 32 * D * 2, join = WAVES * 32 * (D + 4) * 4;
     constexpr int bytes = copies > join ? copies : join;
     if (hipError_t e = allow_dynamic_lds((const void*)attention_few_kernel<T, D, WAVES, PAGED>, bytes)) return e;
-    attention_few_kernel<T, D, WAVES, PAGED><<<grid, 64 * WAVES, bytes, stream>>>(a, p.splits);
+    attention_few_kernel<T, D, WAVES, PAGED><<<map.grid, 64 * WAVES, bytes, stream>>>(a, map, p.splits);
     return hipGetLastError();
 }
 
 template <typename T, int D, bool PAGED>
 hipError_t run(const AttentionArgs& a, const Plan& p, hipStream_t stream) {
-    const dim3 grid((unsigned)p.blocks * p.splits, a.kv_heads, a.sequences);
+    BlockMap map;
+    if (!block_map((int64_t)p.blocks * p.splits, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
     if (p.few) {
-        if (hipError_t e = p.waves == 8 ? run_few<T, D, D == 64 ? 8 : 4, PAGED>(a, p, grid, stream)
-                                                   : run_few<T, D, 4, PAGED>(a, p, grid, stream))
+        if (hipError_t e = p.waves == 8 ? run_few<T, D, D == 64 ? 8 : 4, PAGED>(a, p, map, stream)
+                                                   : run_few<T, D, 4, PAGED>(a, p, map, stream))
             return e;
     } else {
-        attention_tile_kernel<T, D, PAGED><<<grid, kThreads, 0, stream>>>(a, p.splits);
+        attention_tile_kernel<T, D, PAGED><<<map.grid, kThreads, 0, stream>>>(a, map, p.splits);
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (p.splits == 1) return hipSuccess;

@@ -57,14 +57,14 @@ template <int D>
 constexpr int kDqKeys = D == 64 ? 64 : 32;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs a, BlockMap map) {
     constexpr int ROWS = kDqKeys<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     Place pl;
-    if (!place_of<32 * kWaves>(a, 1, &pl)) return;
+    if (!place_of<32 * kWaves>(a, map, 1, &pl)) return;
     const Rows rw = rows_of(a.group);
     const int last_row = pl.rows - 1;
     const int w0 = pl.row0 + 32 * wave, w1 = w0 + 31 < last_row ? w0 + 31 : last_row;
@@ -258,18 +258,17 @@ template <int D>
 constexpr int kDkvRows = 64;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a, KeyPlan plan, float* parts) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a, BlockMap map, KeyPlan plan, float* parts) {
     constexpr int ROWS = kDkvRows<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
     __shared__ FoundRows found;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    int block, part, of;
-    plan.item(blockIdx.x, &block, &part, &of);
+    int at, block, part, of;
     Place pl;
-    pl.seq = blockIdx.z;
-    pl.kh = blockIdx.y;
+    if (!block_of(map, &at, &pl.kh, &pl.seq)) return;
+    plan.item(at, &block, &part, &of);
     pl.q = run_of(a.cu_q, pl.seq, a.max_q, a.q_tokens);
     pl.kv = run_of(a.cu_kv, pl.seq, a.max_kv, a.kv_tokens);
     pl.q.count = uniform(pl.q.count);
@@ -465,7 +464,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     const float fk = up == 0.f ? 0.f : a.scale / up, fv = kScaled<T> ? 1.f / kWeightLift : 1.f;
     if (of > 1) {
         // [item][dk, dv][key][D] FP32, in order of the parts
-        const int64_t item = ((int64_t)pl.seq * a.kv_heads + pl.kh) * plan.items() + blockIdx.x;
+        const int64_t item = ((int64_t)pl.seq * a.kv_heads + pl.kh) * plan.items() + at;
         float* to = parts + ((item * 2) * kKeys + 32 * wave + (lane & 31)) * D + 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -553,14 +552,17 @@ KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, 
 
 template <typename T, int D>
 hipError_t run(const AttentionArgs& a, const KeyPlan& p, hipStream_t stream) {
+    BlockMap map;
     if (a.max_q > 0) {
         const int64_t rows = (int64_t)a.max_q * a.group;
-        attention_dq_kernel<T, D><<<dim3((unsigned)((rows + 127) / 128), a.kv_heads, a.sequences), kThreads, 0, stream>>>(a);
+        if (!block_map((rows + 127) / 128, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
+        attention_dq_kernel<T, D><<<map.grid, kThreads, 0, stream>>>(a, map);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (a.max_kv <= 0) return hipSuccess;
     float* parts = (float*)a.workspace + ((a.q_tokens * a.q_heads + 3) & ~INT64_C(3));
-    attention_dkv_kernel<T, D><<<dim3((unsigned)p.items(), a.kv_heads, a.sequences), kThreads, 0, stream>>>(a, p, parts);
+    if (!block_map(p.items(), a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
+    attention_dkv_kernel<T, D><<<map.grid, kThreads, 0, stream>>>(a, map, p, parts);
     if (hipError_t e = hipGetLastError()) return e;
     const int joined = p.parts > 1 ? p.blocks : (p.sink_parts > 1 ? p.sink_blocks : 0);
     if (!joined) return hipSuccess;
