@@ -8,6 +8,7 @@ namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 4;  // heads whose loads are in flight at once
 
 // N adjacent elements (16 bytes, or one element).
 template <typename T, int N>
@@ -81,28 +82,30 @@ struct Chunk {
         for (int i = 0; i < N; ++i)
             if (i < n) turn(r, pos, first + i, &c[i], &s[i]);
     }
-    __device__ __forceinline__ void copy(const T* from, T* to) const {
-        T a[N];
-        Vec<T, N>::load(from + at, a);
-        Vec<T, N>::store(to + at, a);
-        if (partner) {
-            Vec<T, N>::load(from + at + partner, a);
-            Vec<T, N>::store(to + at + partner, a);
-        }
-    }
-    __device__ __forceinline__ void apply(const T* from, T* to) const {
-        T a[N], b[N];
-        Vec<T, N>::load(from + at, a);
-        if (partner) {
-            Vec<T, N>::load(from + at + partner, b);
+    // The chunk of up to U heads, turned or copied: their loads are all in flight before the first
+    // is used. from(u), to(u): the head's row, null where there is none.
+    template <int U, typename From, typename To>
+    __device__ __forceinline__ void apply_all(From from, To to, bool turn_them) const {
+        T a[U][N], b[U][N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) rotate(a[i], b[i], c[i], s[i]);
-            Vec<T, N>::store(to + at + partner, b);
-        } else if (inside) {
+        for (int u = 0; u < U; ++u)
+            if (const T* f = from(u)) {
+                Vec<T, N>::load(f + at, a[u]);
+                if (partner) Vec<T, N>::load(f + at + partner, b[u]);
+            }
 #pragma unroll
-            for (int i = 0; i + 1 < N; i += 2) rotate(a[i], a[i + 1], c[i / 2], s[i / 2]);
-        }
-        Vec<T, N>::store(to + at, a);
+        for (int u = 0; u < U; ++u)
+            if (T* t = to(u)) {
+                if (turn_them && partner) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) rotate(a[u][i], b[u][i], c[i], s[i]);
+                } else if (turn_them && inside) {
+#pragma unroll
+                    for (int i = 0; i + 1 < N; i += 2) rotate(a[u][i], a[u][i + 1], c[i / 2], s[i / 2]);
+                }
+                Vec<T, N>::store(t + at, a[u]);
+                if (partner) Vec<T, N>::store(t + at + partner, b[u]);
+            }
     }
     static __device__ __forceinline__ void rotate(T& a, T& b, float c, float s) {
         const float x = widen(a), y = widen(b);
@@ -123,7 +126,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs r, int64_t 
     c.set(r, (int)(item - token * chunks), r.positions + token * 3);
     const T* from = (const T*)x.p + token * x.ts;
     T* to = (T*)out.p + token * out.ts;
-    for (int h = blockIdx.y; h < heads; h += gridDim.y) c.apply(from + h * x.hs, to + h * out.hs);
+    const int step = gridDim.y;
+    for (int h = blockIdx.y; h < heads; h += kBatch * step)
+        c.template apply_all<kBatch>([&](int u) { return h + u * step < heads ? from + (h + u * step) * x.hs : nullptr; },
+                                     [&](int u) { return h + u * step < heads ? to + (h + u * step) * out.hs : nullptr; }, true);
 }
 
 // One thread: one chunk of one new token; heads as above, q's, then k's, then v's.
@@ -150,18 +156,27 @@ __global__ __launch_bounds__(kThreads) void append_kernel(RotaryArgs r, AppendAr
     if ((int)blockIdx.y >= heads) return;
     Chunk<T, N> c;
     c.set(r, (int)(item - token * chunks), r.positions + token * 3);
-    for (int h = blockIdx.y; h < heads; h += gridDim.y) {
-        if (h < nq) {
-            c.apply((const T*)a.q.p + token * a.q.ts + h * a.q.hs, (T*)a.q_out.p + token * a.q_out.ts + h * a.q_out.hs);
-            continue;
-        }
-        const int k = h - nq;
-        if (k < a.kv_heads)
-            c.apply((const T*)a.k.p + token * a.k.ts + k * a.k.hs, (T*)a.k_pages.p + row * a.k_pages.ts + k * a.k_pages.hs);
-        else
-            c.copy((const T*)a.v.p + token * a.v.ts + (k - a.kv_heads) * a.v.hs,
-                   (T*)a.v_pages.p + row * a.v_pages.ts + (k - a.kv_heads) * a.v_pages.hs);
-    }
+    // q's and k's heads turn, v's do not: two runs.
+    const int step = gridDim.y, turned = row < 0 ? nq : nq + a.kv_heads;
+    auto from_of = [&](int h) -> const T* {
+        if (h < nq) return (const T*)a.q.p + token * a.q.ts + h * a.q.hs;
+        if (h < turned) return (const T*)a.k.p + token * a.k.ts + (h - nq) * a.k.hs;
+        return (const T*)a.v.p + token * a.v.ts + (h - turned) * a.v.hs;
+    };
+    auto to_of = [&](int h) -> T* {
+        if (h < nq) return (T*)a.q_out.p + token * a.q_out.ts + h * a.q_out.hs;
+        if (h < turned) return (T*)a.k_pages.p + row * a.k_pages.ts + (h - nq) * a.k_pages.hs;
+        return (T*)a.v_pages.p + row * a.v_pages.ts + (h - turned) * a.v_pages.hs;
+    };
+    int h = blockIdx.y;
+    for (; h < turned; h += kBatch * step)
+        c.template apply_all<kBatch>([&](int u) { return h + u * step < turned ? from_of(h + u * step) : nullptr; },
+                                     [&](int u) { return h + u * step < turned ? to_of(h + u * step) : nullptr; }, true);
+    // v's first head of this slice: the next of blockIdx.y, blockIdx.y + step, ... past the turned ones.
+    h = blockIdx.y + (turned > (int)blockIdx.y ? (turned - (int)blockIdx.y + step - 1) / step * step : 0);
+    for (; h < heads; h += kBatch * step)
+        c.template apply_all<kBatch>([&](int u) { return h + u * step < heads ? from_of(h + u * step) : nullptr; },
+                                     [&](int u) { return h + u * step < heads ? to_of(h + u * step) : nullptr; }, false);
 }
 
 bool aligned(const void* p, int64_t ts, int64_t hs, int size) {

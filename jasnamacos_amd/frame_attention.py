@@ -77,6 +77,8 @@ def _index(name: str, t, count) -> None:
 
 
 # The C structs' layouts: packing one is several times faster than filling its fields.
+_ROTARY = struct.Struct("6i")
+_CACHE = struct.Struct("6i")
 _APPEND = struct.Struct("iiq8q")
 _ATTENTION = struct.Struct("11ifqq16q")
 _NORM = struct.Struct("iiqqff")
@@ -86,6 +88,7 @@ _NO_STRIDES = (0, 0)
 class _Handle:
     def __init__(self, ctx: HipDeformConv):
         self.ctx = ctx
+        self._ctx = ctx.ctx
         self._lib = ctx._lib
         self._workspace = None
         self._sizes = {}  # workspace bytes of the shapes seen
@@ -117,8 +120,7 @@ class Rotary(_Handle):
         self.head_dim, self.pairs, self.interleaved = int(head_dim), tuple(int(p) for p in pairs), bool(interleaved)
         _need(len(self.pairs) == 3, "rotary pairs are three numbers (time, height, width)")
         self._freq_shape = (sum(self.pairs),)
-        self._c = {code: _lib.DcnRotary(code, self.head_dim, (C.c_int32 * 3)(*self.pairs), int(self.interleaved))
-                   for code in DTYPES.values()}
+        self._c = {t: _ROTARY.pack(code, self.head_dim, *self.pairs, self.interleaved) for t, code in DTYPES.items()}
 
     def frequencies(self, base: float = 10000.0, device="cuda"):
         """A usual choice of freq: each axis from 1 down to 1 / base."""
@@ -137,12 +139,16 @@ class Rotary(_Handle):
         xt, xh, _ = _heads("x", x, dtype, shape)
         ot, oh, _ = _heads("out", out, dtype, shape)
         self._check(positions, freq, tokens)
-        self.ctx._check(self._lib.dcn_rotary_dev(
-            self.ctx.ctx, C.byref(self._c[_dtype(x)]), tokens, heads, x.data_ptr(), xt, xh, positions.data_ptr(),
-            freq.data_ptr(), inverse, out.data_ptr(), ot, oh, _stream(stream)))
+        _dtype(x)
+        status = self._lib.dcn_rotary_dev(
+            self._ctx, self._c[dtype], tokens, heads, x.data_ptr(), xt, xh, positions.data_ptr(), freq.data_ptr(),
+            inverse, out.data_ptr(), ot, oh, stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
 
 
-def _cache(k_pages, v_pages, table) -> _lib.DcnCache:
+def _cache(k_pages, v_pages, table) -> bytes:
+    """The packed dcn_cache."""
     if k_pages.dim() != 4 or table.dim() != 2:
         raise DeformConvError(INVALID_SHAPE, "pages are [pages][page_tokens][heads][channels], the table "
                                              "[sequences][width]")
@@ -151,7 +157,7 @@ def _cache(k_pages, v_pages, table) -> _lib.DcnCache:
     _whole("v_pages", v_pages, dtype, shape)
     _whole("table", table, torch.int32, table.shape)
     pages, page_tokens, heads, dim = shape
-    return _lib.DcnCache(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
+    return _CACHE.pack(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
 
 
 class CacheAppend(_Handle):
@@ -163,8 +169,9 @@ class CacheAppend(_Handle):
         last of its kv_lens[s] tokens. Keys are turned by `rotary` on the way, and so is q into
         q_out where it is given."""
         cache = _cache(k_pages, v_pages, table)
-        tokens, sequences, dtype, dim = _rows("k", k), table.shape[0], k_pages.dtype, cache.head_dim
-        shape = (tokens, cache.kv_heads, dim)
+        tokens, sequences, dtype = _rows("k", k), table.shape[0], k_pages.dtype
+        _, _, kv_heads, dim = k_pages.shape
+        shape = (tokens, kv_heads, dim)
         ks, vs = _heads("k", k, dtype, shape), _heads("v", v, dtype, shape)
         _index("cu_q", cu_q, sequences + 1)
         _index("kv_lens", kv_lens, sequences)
@@ -177,12 +184,14 @@ class CacheAppend(_Handle):
         r = None
         if rotary is not None:
             rotary._check(positions, freq, tokens)
-            r = C.byref(rotary._c[cache.dtype])
+            r = rotary._c[dtype]
         s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
-        self.ctx._check(self._lib.dcn_cache_append_dev(
-            self.ctx.ctx, C.byref(cache), s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq),
-            cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
-            _stream(stream)))
+        status = self._lib.dcn_cache_append_dev(
+            self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
+            kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
+            stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
 
 
 class FrameAttention(_Handle):
@@ -249,9 +258,11 @@ class FrameAttention(_Handle):
         max_q and max_kv bound their lengths."""
         s = self._pack(*self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv))
         w, size = self._workspace_of(s, PASS_FORWARD, q)
-        self.ctx._check(self._lib.dcn_attention_forward_dev(
-            self.ctx.ctx, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_q), _ptr(cu_kv), out.data_ptr(),
-            _ptr(lse), w, size, _stream(stream)))
+        status = self._lib.dcn_attention_forward_dev(
+            self._ctx, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_q), _ptr(cu_kv), out.data_ptr(), _ptr(lse), w,
+            size, stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
 
     def backward_dev(self, q, k, v, out, lse, dout, dq, dk, dv, cu_q=None, cu_kv=None, max_q=None, max_kv=None,
                      stream=None) -> None:
@@ -279,16 +290,18 @@ class FrameAttention(_Handle):
         if max_q is None:
             max_q = q_tokens if cu_q is not None else (q_tokens // sequences if sequences else 0)
         if max_kv is None:
-            max_kv = cache.table_width * cache.page_tokens
+            max_kv = table.shape[1] * k_pages.shape[1]
         shape = (q_tokens, self.q_heads, self.head_dim)
         if lse is not None:
             _whole("lse", lse, torch.float32, (q_tokens, self.q_heads))
         s = self._pack(q, sequences, int(max_q), int(max_kv), q_tokens, 0, _heads("q", q, dtype, shape), _NO_STRIDES,
                        _NO_STRIDES, _heads("out", out, dtype, shape))
         w, size = self._workspace_of(s, PASS_PAGED, q)
-        self.ctx._check(self._lib.dcn_attention_paged_dev(
-            self.ctx.ctx, s, C.byref(cache), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q),
-            kv_lens.data_ptr(), table.data_ptr(), out.data_ptr(), _ptr(lse), w, size, _stream(stream)))
+        status = self._lib.dcn_attention_paged_dev(
+            self._ctx, s, cache, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q), kv_lens.data_ptr(),
+            table.data_ptr(), out.data_ptr(), _ptr(lse), w, size, stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
 
 
 class GatedNorm(_Handle):
@@ -309,20 +322,13 @@ class GatedNorm(_Handle):
         return _NORM.pack(_dtype(x), self.channels, x.shape[0], self.gate_tokens, self.residual_scale, self.eps)
 
     def _check_all(self, x, tensors, gates, vectors, sums=()) -> None:
-        tokens, dtype = x.shape[0], x.dtype
-        shape = (tokens, self.channels)
-        for name, t in tensors:
-            if t is not None:
-                _whole(name, t, dtype, shape)
-        for name, t in gates:
-            if t is not None:
-                _whole(name, t, dtype, (-(-tokens // self.gate_tokens), self.channels))
-        for name, t in vectors:
-            if t is not None:
-                _whole(name, t, dtype, (self.channels,))
-        for name, t in sums:
-            if t is not None:
-                _whole(name, t, torch.float32, (self.channels,))
+        tokens, dtype, channels = x.shape[0], x.dtype, self.channels
+        for shape, kind, group in (((tokens, channels), dtype, tensors),
+                                   ((-(-tokens // self.gate_tokens), channels), dtype, gates),
+                                   ((channels,), dtype, vectors), ((channels,), torch.float32, sums)):
+            for name, t in group:
+                if t is not None and not (t.shape == shape and t.dtype is kind and t.is_contiguous()):
+                    _whole(name, t, kind, shape)
 
     def low_bytes(self, x) -> int:
         """Bytes of forward_dev's `low` for a residual stream like x."""
@@ -356,10 +362,11 @@ class GatedNorm(_Handle):
                         (("w_post", w_post), ("w_pre", w_pre)))
         if rstd is not None:
             _whole("rstd", rstd, torch.float32, (x.shape[0], 2))
-        self.ctx._check(self._lib.dcn_gated_norm_forward_dev(
-            self.ctx.ctx, s, h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
-            x_out.data_ptr(), _ptr(y), _ptr(rstd), None if rstd is None else self._low(s, low, x, True),
-            _stream(stream)))
+        status = self._lib.dcn_gated_norm_forward_dev(
+            self._ctx, s, h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre), x_out.data_ptr(), _ptr(y),
+            _ptr(rstd), None if rstd is None else self._low(s, low, x, True), stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
 
     def backward_dev(self, h, x_out, gate, w_post, w_pre, rstd, dx_out, dy, dh, dx, dgate=None, dw_post=None,
                      dw_pre=None, low=None, stream=None) -> None:
