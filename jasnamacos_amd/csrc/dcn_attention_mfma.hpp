@@ -108,11 +108,6 @@ __device__ __forceinline__ void copy16(const char* base, uint32_t at, char* dst)
     const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory");
 }
-// The same from an address per lane.
-__device__ __forceinline__ void copy16(const char* from, char* dst) {
-    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
-}
 // All but the last LEFT of this wave's copies have arrived.
 template <int LEFT>
 __device__ __forceinline__ void wait_copies() {

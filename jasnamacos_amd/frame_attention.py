@@ -13,7 +13,8 @@ packed projection is taken as it is. As elsewhere in this package outputs are th
 calls are asynchronous on `stream` (None: the default stream), and errors are
 DeformConvError. A FrameAttention or GatedNorm keeps the workspace of its calls: calls that
 may run at the same time need a handle each, and a handle sizes its workspace in its first
-call of a size (reserve it before a graph capture by running that call once)."""
+call of a size (reserve it before a graph capture by running that call once). Keep a handle
+until its calls on streams other than torch's current one have ended."""
 from __future__ import annotations
 
 import ctypes as C
@@ -85,6 +86,15 @@ _NORM = struct.Struct("iiqqff")
 _NO_STRIDES = (0, 0)
 
 
+def _fresh(count: int, like):
+    """Memory for a handle. The allocator may hand out what work on the current stream still
+    reads; the handle's calls may be on another one."""
+    t = torch.empty(count, dtype=torch.uint8, device=like.device)
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(like.device).synchronize()
+    return t
+
+
 class _Handle:
     def __init__(self, ctx: HipDeformConv):
         self.ctx = ctx
@@ -107,7 +117,7 @@ class _Handle:
         if w is None or w.numel() < count:
             if w is not None:
                 torch.cuda.synchronize(w.device)  # calls in flight still use the old one
-            self._workspace = w = torch.empty(count, dtype=torch.uint8, device=like.device)
+            self._workspace = w = _fresh(count, like)
         return w.data_ptr(), w.numel()
 
 
@@ -350,7 +360,7 @@ class GatedNorm(_Handle):
                 return None
             if self._kept is not None:
                 torch.cuda.synchronize(like.device)
-            self._kept = torch.empty(count, dtype=torch.uint8, device=like.device)
+            self._kept = _fresh(count, like)
         return self._kept.data_ptr()
 
     def forward_dev(self, h, x, gate, w_post, w_pre, x_out, y=None, rstd=None, low=None, stream=None) -> None:
@@ -382,5 +392,5 @@ class GatedNorm(_Handle):
         w, size = self._room(s, lambda: self._lib.dcn_gated_norm_workspace_bytes(s), x_out)
         self.ctx._check(self._lib.dcn_gated_norm_backward_dev(
             self.ctx.ctx, s, h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
-            rstd.data_ptr(), self._low(s, low, x_out, False), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw_post),
-            _ptr(dw_pre), w, size, _stream(stream)))
+            rstd.data_ptr(), self._low(s, low, x_out, False), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(),
+            dx.data_ptr(), _ptr(dgate), _ptr(dw_post), _ptr(dw_pre), w, size, _stream(stream)))
