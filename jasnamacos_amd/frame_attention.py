@@ -42,13 +42,21 @@ def _need(condition, message: str) -> None:
         raise DeformConvError(INVALID_SHAPE, message)
 
 
+def _on_device(name: str, t) -> None:
+    if t is None:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
+    if not t.is_cuda:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is not on a device")
+
+
 def _heads(name: str, t, dtype, shape) -> tuple:
-    """The strides of a tensor of heads of this shape (its own row count where that is None)."""
-    if t.shape == shape and t.dtype is dtype:
+    """The strides of a tensor of heads of this shape."""
+    if t is not None and t.shape == shape and t.dtype is dtype and t.is_cuda:
         strides = t.stride()
         if strides[2] == 1 or shape[2] == 1:
             return strides
         raise DeformConvError(INVALID_SHAPE, f"{name} channels are not adjacent")
+    _on_device(name, t)
     if t.dtype is not dtype:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
     raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}")
@@ -56,6 +64,8 @@ def _heads(name: str, t, dtype, shape) -> tuple:
 
 def _rows(name: str, t) -> int:
     """The rows of a tensor of heads."""
+    if t is None:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
     if t.dim() != 3:
         raise DeformConvError(INVALID_SHAPE, f"{name} has {t.dim()} dimensions; expected [tokens][heads][channels]")
     return t.shape[0]
@@ -63,8 +73,9 @@ def _rows(name: str, t) -> int:
 
 def _whole(name: str, t, dtype, shape) -> None:
     """An adjacent tensor of this type and shape."""
-    if t.shape == shape and t.dtype is dtype and t.is_contiguous():
+    if t is not None and t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.is_cuda:
         return
+    _on_device(name, t)
     if t.dtype is not dtype:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
     raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}, adjacent")
@@ -72,8 +83,9 @@ def _whole(name: str, t, dtype, shape) -> None:
 
 def _index(name: str, t, count) -> None:
     """An adjacent int32 array of this length."""
-    if t.dtype is torch.int32 and t.shape == (count,) and t.is_contiguous():
+    if t is not None and t.dtype is torch.int32 and t.shape == (count,) and t.is_contiguous() and t.is_cuda:
         return
+    _on_device(name, t)
     raise DeformConvError(INVALID_SHAPE, f"{name} is not {count} adjacent int32 values")
 
 
@@ -159,6 +171,8 @@ class Rotary(_Handle):
 
 def _cache(k_pages, v_pages, table) -> bytes:
     """The packed dcn_cache."""
+    if k_pages is None or table is None:
+        raise DeformConvError(INVALID_ARGUMENT, "k_pages or table is missing")
     if k_pages.dim() != 4 or table.dim() != 2:
         raise DeformConvError(INVALID_SHAPE, "pages are [pages][page_tokens][heads][channels], the table "
                                              "[sequences][width]")
@@ -190,6 +204,7 @@ class CacheAppend(_Handle):
             _rows("q", q)
             q_heads = q.shape[1]
             shape = (tokens, q_heads, dim)
+            _rows("q_out", q_out)
             qs, os = _heads("q", q, dtype, shape), _heads("q_out", q_out, dtype, shape)
         r = None
         if rotary is not None:
@@ -278,6 +293,8 @@ class FrameAttention(_Handle):
                      stream=None) -> None:
         """The gradients of forward_dev's out, from its arguments, out, lse and dout."""
         parts = self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
+        if lse is None:
+            raise DeformConvError(INVALID_ARGUMENT, "lse is missing")
         dtype, q_shape, k_shape = q.dtype, q.shape, k.shape
         s = self._pack(*parts, _heads("dout", dout, dtype, q_shape), _heads("dq", dq, dtype, q_shape),
                        _heads("dk", dk, dtype, k_shape), _heads("dv", dv, dtype, k_shape))
@@ -327,17 +344,22 @@ class GatedNorm(_Handle):
         _need(self.channels > 0 and self.gate_tokens > 0, "channels and gate_tokens must be positive")
 
     def _pack(self, x) -> bytes:
+        if x is None:
+            raise DeformConvError(INVALID_ARGUMENT, "the residual stream is missing")
         if x.dim() != 2:
             raise DeformConvError(INVALID_SHAPE, f"the residual stream has {x.dim()} dimensions; expected [tokens][channels]")
         return _NORM.pack(_dtype(x), self.channels, x.shape[0], self.gate_tokens, self.residual_scale, self.eps)
 
-    def _check_all(self, x, tensors, gates, vectors, sums=()) -> None:
+    def _check_all(self, x, needed, tensors, gates, vectors, sums=()) -> None:
+        for name, t in needed:
+            if t is None:
+                raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
         tokens, dtype, channels = x.shape[0], x.dtype, self.channels
-        for shape, kind, group in (((tokens, channels), dtype, tensors),
+        for shape, kind, group in (((tokens, channels), dtype, needed), ((tokens, channels), dtype, tensors),
                                    ((-(-tokens // self.gate_tokens), channels), dtype, gates),
                                    ((channels,), dtype, vectors), ((channels,), torch.float32, sums)):
             for name, t in group:
-                if t is not None and not (t.shape == shape and t.dtype is kind and t.is_contiguous()):
+                if t is not None and not (t.shape == shape and t.dtype is kind and t.is_contiguous() and t.is_cuda):
                     _whole(name, t, kind, shape)
 
     def low_bytes(self, x) -> int:
@@ -352,6 +374,7 @@ class GatedNorm(_Handle):
         if not count:
             return None
         if low is not None:
+            _on_device("low", low)
             if low.dtype != torch.uint8 or low.numel() < count or not low.is_contiguous():
                 raise DeformConvError(INVALID_SHAPE, f"low is not {count} adjacent uint8 values")
             return low.data_ptr()
@@ -368,7 +391,7 @@ class GatedNorm(_Handle):
         FP32) is what backward_dev reads; with it, 16-bit calls keep what rounding takes from
         x_out (low_bytes(x) uint8 values) in `low`, or in the handle for its next backward_dev."""
         s = self._pack(x)
-        self._check_all(x, (("h", h), ("x", x), ("x_out", x_out), ("y", y)), (("gate", gate),),
+        self._check_all(x, (("h", h), ("x", x), ("x_out", x_out)), (("y", y),), (("gate", gate),),
                         (("w_post", w_post), ("w_pre", w_pre)))
         if rstd is not None:
             _whole("rstd", rstd, torch.float32, (x.shape[0], 2))
@@ -385,8 +408,8 @@ class GatedNorm(_Handle):
         that made rstd (the handle ran another one since, and `low` is None) take x_out as it
         was rounded."""
         s = self._pack(x_out)
-        self._check_all(x_out, (("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dy", dy), ("dh", dh), ("dx", dx)),
-                        (("gate", gate), ("dgate", dgate)), (("w_post", w_post), ("w_pre", w_pre)),
+        self._check_all(x_out, (("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dh", dh), ("dx", dx)),
+                        (("dy", dy),), (("gate", gate), ("dgate", dgate)), (("w_post", w_post), ("w_pre", w_pre)),
                         (("dw_post", dw_post), ("dw_pre", dw_pre)))
         _whole("rstd", rstd, torch.float32, (x_out.shape[0], 2))
         w, size = self._room(s, lambda: self._lib.dcn_gated_norm_workspace_bytes(s), x_out)
