@@ -254,12 +254,11 @@ __device__ __forceinline__ Seen all_seen_of(const AttentionArgs& a, int j, int t
     return Seen{seen_of(a, to, n).from, seen_of(a, j < sinks && sinks <= to ? (int)sinks : j, n).to};
 }
 
-template <int D>
-constexpr int kDkvRows = 64;
+constexpr int kDkvRows = 64;  // query rows of a tile of the second pass
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a, BlockMap map, KeyPlan plan, float* parts) {
-    constexpr int ROWS = kDkvRows<D>, BYTES = ROWS * D * 2, MB = ROWS / 32;
+    constexpr int ROWS = kDkvRows, BYTES = ROWS * D * 2, MB = ROWS / 32;
     using Ti = Tile<D>;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS], row_delta[2][ROWS];
@@ -380,85 +379,125 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
             fetch(r0 + ROWS);
             copy(r0 + ROWS, lds[buf ^ 1][0], lds[buf ^ 1][1]);
         }
-        const unsigned long long poison = partial ? found.all(buf) : 0;
+        if (partial)
+            if (const unsigned long long poison = found.all(buf); __builtin_expect(poison != 0, 0)) {
+                if (threadIdx.x < ROWS && poison >> threadIdx.x & 1) row_lse[buf][threadIdx.x] = NAN;
+                __syncthreads();
+            }
         // A bit for each of the tile's rows that sees this lane's key: positions grow with the rows.
-        const bool masked = !whole || poison;
-        unsigned long long seen = 0;
-        if (masked) {
+        unsigned long long seen = ~0ull;
+        if (!whole) {
             const int64_t rem = r0 - (int64_t)t0 * a.group;
             const int64_t lo = ((int64_t)me.from - p0) * a.group - rem, hi = ((int64_t)me.to - p0) * a.group - rem;
             const int64_t there = q_rows - r0, top = hi < there ? hi : there;
             seen = bits_below((int)(top < 64 ? (top < 0 ? 0 : top) : 64)) & ~bits_below((int)(lo < 64 ? (lo < 0 ? 0 : lo) : 64));
             seen >>= 4 * (lane >> 5);
         }
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            f32x16 s, dp;
-            {
-                u32x4 qr[D / 16], gr[D / 16];
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) qr[n] = Ti::rows(qt, mb, n, lane);
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) gr[n] = Ti::rows(ot, mb, n, lane);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) s = mma<T>(qr[n], k[n], s);
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) dp = mma<T>(gr[n], v[n], dp);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            u32x4 oc[2][D / 32], qc[2][D / 32];
+        struct Half {  // 32 rows of the tile against the wave's keys
+            int mb;
+            u32x4 qr[D / 16], gr[D / 16], oc[2][D / 32], qc[2][D / 32];
             f32x4 l4[4], d4[4];
+            f32x16 s, dp;
+        };
+        auto read_rows = [&](Half& h, int mb) {
+            h.mb = mb;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) h.qr[n] = Ti::rows(qt, mb, n, lane);
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) h.gr[n] = Ti::rows(ot, mb, n, lane);
+        };
+        auto scores = [&](Half& h) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) h.s[x] = h.dp[x] = 0.f;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) h.s = mma<T>(h.qr[n], k[n], h.s);
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) h.dp = mma<T>(h.gr[n], v[n], h.dp);
+        };
+        auto read_stats = [&](Half& h) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                l4[g] = *(const f32x4*)&row_lse[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
-                d4[g] = *(const f32x4*)&row_delta[buf][32 * mb + 8 * g + 4 * (lane >> 5)];
+                h.l4[g] = *(const f32x4*)&row_lse[buf][32 * h.mb + 8 * g + 4 * (lane >> 5)];
+                h.d4[g] = *(const f32x4*)&row_delta[buf][32 * h.mb + 8 * g + 4 * (lane >> 5)];
             }
+        };
+        auto read_columns = [&](Half& h) {
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int n = 0; n < D / 32; ++n) {
-                    oc[st][n] = Ti::columns(ot, mb, st, n, lane);
-                    qc[st][n] = Ti::columns(qt, mb, st, n, lane);
+                    h.oc[st][n] = Ti::columns(ot, h.mb, st, n, lane);
+                    h.qc[st][n] = Ti::columns(qt, h.mb, st, n, lane);
                 }
-            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto weights = [&](Half& h) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -l4[x >> 2][x & 3]));
-                dp[x] = s[x] * (dp[x] - d4[x >> 2][x & 3]);
+                h.s[x] = __builtin_amdgcn_exp2f(fmaf(h.s[x], c, -h.l4[x >> 2][x & 3]));
+                h.dp[x] = h.s[x] * (h.dp[x] - h.d4[x >> 2][x & 3]);
             }
-            if (masked) {
-                if (__builtin_expect(poison != 0, 0)) {
-                    const unsigned long long not_finite = poison >> (4 * (lane >> 5));
-#pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        if (spread_bit(not_finite, 32 * mb + 8 * (x >> 2) + (x & 3))) s[x] = dp[x] = NAN;
-                }
+            if (!whole) {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const uint32_t on = spread_bit(seen, 32 * mb + 8 * (x >> 2) + (x & 3));
-                    s[x] = keep_or(s[x], on, 0.f);
-                    dp[x] = keep_or(dp[x], on, 0.f);
+                    const uint32_t on = spread_bit(seen, 32 * h.mb + 8 * (x >> 2) + (x & 3));
+                    h.s[x] = keep_or(h.s[x], on, 0.f);
+                    h.dp[x] = keep_or(h.dp[x], on, 0.f);
                 }
             }
+        };
+        auto add = [&](Half& h) {
             if constexpr (kScaled<T>) {
-                follow_scale<D>(top_of(dp), &up, dk);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    s[x] *= kWeightLift;
-                    dp[x] *= up;
+                    h.s[x] *= kWeightLift;
+                    h.dp[x] *= up;
                 }
             }
-            const u32x4 p16[2] = {pack8<T>(s, 0), pack8<T>(s, 8)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 8)};
+            const u32x4 p16[2] = {pack8<T>(h.s, 0), pack8<T>(h.s, 8)}, ds[2] = {pack8<T>(h.dp, 0), pack8<T>(h.dp, 8)};
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int n = 0; n < D / 32; ++n) {
-                    dv[n] = mma<T>(oc[st][n], p16[st], dv[n]);
-                    dk[n] = mma<T>(qc[st][n], ds[st], dk[n]);
+                    dv[n] = mma<T>(h.oc[st][n], p16[st], dv[n]);
+                    dk[n] = mma<T>(h.qc[st][n], ds[st], dk[n]);
                 }
+        };
+        if constexpr (D == 64 || !kScaled<T>) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                Half h;
+                read_rows(h, mb);
+                __builtin_amdgcn_sched_barrier(0);
+                scores(h);
+                __builtin_amdgcn_sched_barrier(0);
+                read_stats(h);
+                read_columns(h);
+                __builtin_amdgcn_sched_barrier(0);
+                weights(h);
+                if constexpr (kScaled<T>) follow_scale<D>(top_of(h.dp), &up, dk);
+                add(h);
+            }
+        } else {
+            // FP16 of 128 channels looks at its factors once a tile: joining the sums after that
+            // branch costs a copy of each (a training step of four sequences of up to 1021 tokens, two
+            // key heads of four: 100 us with a look for each half, 97 so).
+            Half h0, h1;
+            read_rows(h0, 0);
+            read_stats(h0);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(h0);
+            read_rows(h1, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(h1);
+            weights(h0);
+            __builtin_amdgcn_sched_barrier(0);
+            read_stats(h1);
+            weights(h1);
+            follow_scale<D>(fmaxf(top_of(h0.dp), top_of(h1.dp)), &up, dk);
+            read_columns(h0);
+            add(h0);
+            read_columns(h1);
+            add(h1);
         }
     }
     const float fk = up == 0.f ? 0.f : a.scale / up, fv = kScaled<T> ? 1.f / kWeightLift : 1.f;
