@@ -63,14 +63,20 @@ __device__ __forceinline__ Rows rows_of(int group) {
 }
 
 // A tile: ROWS rows of D 16-bit channels, row-major, the 16-byte chunks of row r at chunk ^
-// swizzle(r). Eight adjacent rows put one chunk in eight places, and four adjacent rows
-// (4n .. 4n + 3) one 32-byte pair in four, so that both kinds of read are free of bank conflicts.
-__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
-
+// swizzle(r). LDS gives 256 bytes a cycle from 64 banks: a read of rows takes sixteen lanes (one
+// chunk of sixteen adjacent rows) at a time, a transposing one thirty-two (64 bytes of four
+// adjacent rows). With 128 channels, a row on all banks, both lie in different banks. With 64 they
+// meet in pairs: the swizzle without that has more addresses to hold, and a training step of
+// 4 x 2560 tokens took 174 us with it, 170 so (128 channels, forward of 2 x 4096 tokens: 185 us
+// without conflicts, 190 in pairs).
 template <int D>
 struct Tile {
     static constexpr int kChunks = D / 8;           // 16-byte chunks a row
     static constexpr int kRowsPerCopy = 64 / kChunks;  // rows that one wave's copy instruction fills
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        return D == 64 ? ((row & 3) << 1) | (row >> 2 & 1) : ((row & 3) << 2) | (row >> 2 & 3);
+    }
 
     // A operand with M = rows: row 32 mb + l % 32, channels 16 s + 8 h .. + 7.
     static __device__ __forceinline__ u32x4 rows(const char* tile, int mb, int s, int lane) {
