@@ -86,8 +86,8 @@ hipError_t launch_norm_backward(int dtype, const NormArgs& a, hipStream_t stream
 constexpr size_t norm_low_header(int64_t tokens) { return ((size_t)tokens * 8 + 15) / 16 * 16; }
 size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 
-// Row kernels: any head size and type (dcn_kernels_attention_rows.hip).
-hipError_t launch_attention_rows(int dtype, const AttentionArgs& a, hipStream_t stream);
+// Any head size, type, stride and alignment (dcn_kernels_attention_any.hip, _rows.hip).
+hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).

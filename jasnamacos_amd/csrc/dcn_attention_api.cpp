@@ -110,6 +110,9 @@ dcn_status check_attention(dcn_context* ctx, const dcn_attention_shape* s, bool 
     REQUIRE_SHAPE(s->max_q >= 0 && s->max_kv >= 0, "max_q and max_kv must not be negative");
     REQUIRE_SHAPE(s->q_tokens >= 0 && s->kv_tokens >= 0, "q_tokens and kv_tokens must not be negative");
     REQUIRE_SHAPE(s->scale == s->scale, "scale is not a number");
+    // Packed rows are counted by an int.
+    REQUIRE_SHAPE((int64_t)s->max_q * (s->q_heads / s->kv_heads) < INT32_MAX - 256,
+                  "max_q times the heads that share a key head must be below 2^31 - 256");
     a->sequences = s->sequences;
     a->q_heads = s->q_heads;
     a->kv_heads = s->kv_heads;
@@ -143,12 +146,11 @@ dcn_status check_even(dcn_context* ctx, const dcn_attention_shape* s, const void
     return DCN_OK;
 }
 
-// Whether the matrix kernels take heads of this kind: 16 bits, 64 or 128 channels, a scale that
-// keeps the order of the scores, and packed rows that an int counts. The rest runs a row at a
-// time, as do tensors that are not aligned to 16 bytes.
+// Whether the 16-bit matrix kernels take heads of this kind: 64 or 128 channels, and a scale that
+// keeps the order of the scores. The kernels of any type take the rest, and tensors that are not
+// aligned to 16 bytes.
 bool matrix_heads(const dcn_attention_shape* s) {
-    return s->dtype != DCN_DTYPE_F32 && (s->head_dim == 64 || s->head_dim == 128) && s->scale > 0.f &&
-           (int64_t)s->max_q * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
+    return s->dtype != DCN_DTYPE_F32 && (s->head_dim == 64 || s->head_dim == 128) && s->scale > 0.f;
 }
 // 16-byte rows, and the rows of one tile (64 tokens, the heads of a group) within 32-bit offsets.
 template <typename H>
@@ -333,7 +335,7 @@ dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape
         a.cu_kv = d_cu_kv;
         a.workspace = d_workspace;
         const bool matrix = matrix_heads(shape) && matrix_tensor(a.q) && matrix_tensor(a.k) && matrix_tensor(a.v) && matrix_tensor(a.out);
-        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_rows)(shape->dtype, a, (hipStream_t)stream));
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_any)(shape->dtype, a, (hipStream_t)stream));
         return DCN_OK;
     });
 }
@@ -375,7 +377,7 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
         a.workspace = d_workspace;
         const bool matrix = matrix_heads(shape) && matrix_pool(cache) && matrix_tensor(a.q) && matrix_tensor(a.k) &&
                             matrix_tensor(a.v) && matrix_tensor(a.out);
-        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_rows)(shape->dtype, a, (hipStream_t)stream));
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_any)(shape->dtype, a, (hipStream_t)stream));
         return DCN_OK;
     });
 }

@@ -1,0 +1,258 @@
+// Frame attention forward of any type, head size up to 256, stride and alignment, contiguous or
+// paged: FP32 products on v_mfma_f32_32x32x2_f32. The 16-bit heads of 64 and 128 channels have
+// kernels of their own where they are aligned; this takes the rest.
+//
+// As there, S^T = K Q^T has keys as rows and packed query rows as columns: a lane holds one
+// query row and, of 32 keys, the keys 8a + 4h + b (h = lane / 32) in register 4a + b. Register r
+// is then the second product's B operand of the pair of keys 8a + b and 8a + 4 + b as it is, and
+// softmax stays in a lane and lane ^ 32. Channels 8s + 4h + e are step 4s + e of the first product,
+// so that a lane loads four adjacent ones. Operands come straight from memory, widened on the way:
+// a lane its key's channels, 32 lanes one value row's, which whole lines serve in both cases.
+//
+// A workgroup has 32 rows; its four waves take the key tiles in turn, without a barrier until
+// their sums are joined through LDS. Bound: the FP32 products, a sixteenth of the 16-bit rate, and
+// for few rows the loads' latency. 2,048 causal tokens, 8 FP32 heads of 64: 110 us (39 of the
+// 157 TFLOP/s), of 128: 172 us; FP16 heads of 96: 165 us.
+#include "dcn_attention_mfma.hpp"
+
+namespace dcn {
+namespace fa {
+namespace {
+
+constexpr float kSlack = 8.f;
+constexpr int kRowsWg = 32, kTile = 32;
+
+// Channels at .. at + 3 of a row, as FP32; zeros past its end. Loads without a branch around
+// them, which would wait for each before the next.
+template <typename T, bool VEC>
+__device__ __forceinline__ f32x4 load4(const T* row, int at, int dim) {
+    f32x4 v;
+    if constexpr (VEC) {
+        typedef T four __attribute__((ext_vector_type(4)));
+        const four t = *(const four*)(row + (at < dim ? at : dim - 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = at < dim ? widen((T)t[i]) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float t = widen(row[at + i < dim ? at + i : dim - 1]);
+            v[i] = at + i < dim ? t : 0.f;
+        }
+    }
+    return v;
+}
+__device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ bool finite32(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) != 0x7f800000u; }
+
+// VEC: rows of four-element alignment and heads of whole fours. NB: blocks of 32 channels.
+template <typename T, int NB, bool PAGED, bool VEC, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void attention_any_kernel(AttentionArgs a, BlockMap map) {
+    constexpr int LINE = NB * 32 + 4;
+    __shared__ __attribute__((aligned(16))) float sums[kRowsWg][LINE];
+    __shared__ float top_of[WAVES][kRowsWg], sum_of[WAVES][kRowsWg], inverse[kRowsWg];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+    Place pl;
+    if (!place_of<kRowsWg>(a, map, 1, &pl)) return;
+    const Rows rw = rows_of(a.group);
+    const int last_row = pl.rows - 1 < pl.row0 + kRowsWg - 1 ? pl.rows - 1 : pl.row0 + kRowsWg - 1;
+    const Spread all = spread_of(a, pl, rw, pl.row0, last_row);
+    const int r = pl.row0 + n, rc = r < last_row ? r : last_row;
+    const int tok = rw.token(rc), head = pl.kh * a.group + (rc - tok * a.group);
+    const Span sp = r <= last_row ? span_of(a, pl.offset + tok, pl.kv.count) : Span{0, 0, 0};
+    f32x4 q[NB * 4];
+    {
+        const T* qp = (const T*)a.q.p + (pl.q.first + tok) * a.q.ts + head * a.q.hs;
+#pragma unroll
+        for (int i = 0; i < NB * 4; ++i) q[i] = load4<T, VEC>(qp, 8 * i + 4 * h, a.dim);
+    }
+    const T* kp = (const T*)a.k.p + pl.kh * a.k.hs;
+    const T* vp = (const T*)a.v.p + pl.kh * a.v.hs;
+    const float c = a.scale * 1.44269504088896340736f;
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const TileList<kTile> list(all);
+    for (int i = wave; i < list.count; i += WAVES) {
+        const int t0 = list.tile(i), j = t0 + n;
+        // Row of this lane's key in memory; keys that are not there stand in for the last one, unseen.
+        int64_t at = pl.kv.first + (j < pl.kv.count ? j : pl.kv.count - 1);
+        uint32_t holes = 0;
+        if constexpr (PAGED) {
+            at = paged_row(a.pages, pl.seq, j < pl.kv.count ? j : pl.kv.count - 1);
+            holes = (uint32_t)__ballot(at < 0);
+            at = at < 0 ? 0 : at;
+        }
+        const bool partial = !all_see<kTile>(all, t0) || holes;
+        f32x16 s;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] = 0.f;
+        const T* key = kp + at * a.k.ts;
+        // Values of 32 channels: register x is the pair of keys 8a + b (h = 0) and 8a + 4 + b (h = 1).
+        const int64_t value = at * a.v.ts;
+        auto load_values = [&](float* v, int b) {
+            const int ch = 32 * b + n, in = ch < a.dim ? ch : a.dim - 1;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const float t = widen(vp[__shfl(value, 8 * (x >> 2) + 4 * h + (x & 3)) + in]);
+                v[x] = ch < a.dim ? t : 0.f;
+            }
+        };
+        float v[2][16];
+        load_values(v[0], 0);
+#pragma unroll
+        for (int b = 0; b < NB * 4; b += 8) {
+            f32x4 k[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) k[e] = load4<T, VEC>(key, 8 * (b + e) + 4 * h, a.dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s = mma32(k[e][x], q[b + e][x], s);
+        }
+        if (partial) {
+            const unsigned long long seen = (seen_bits(sp, t0) & ~(unsigned long long)holes) >> (4 * h);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] = keep_or(s[x] * c, spread_bit(seen, 8 * (x >> 2) + (x & 3)), -INFINITY);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] *= c;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int x = 1; x < 16; ++x) top = fmaxf(top, s[x]);
+        top = both_max(top);
+        if (__any(top > m + kSlack)) {
+            const float next = fmaxf(m, top), old = exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= old;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[b][x] *= old;
+        }
+        // fmaxf drops NaN: a NaN score keeps m and makes its own weight, and the row, NaN.
+        const float ref = m == -INFINITY ? 0.f : m;
+        float part = 0.f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            s[x] = __builtin_amdgcn_exp2f(s[x] - ref);
+            part += s[x];
+        }
+        l += part;
+        bool bad = false;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float* now = v[b & 1];
+            if (b + 1 < NB) load_values(v[b + 1 & 1], b + 1);
+            // A value that is not finite would reach rows that do not see it (0 x NaN): zero here, and
+            // added below where it is seen.
+            if (partial) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const bool fine = finite32(now[x]);
+                    bad |= !fine;
+                    now[x] = fine ? now[x] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[b] = mma32(now[x], s[x], o[b]);
+        }
+        if (__builtin_expect(__any(bad), 0)) {
+            for (int in = 0; in < kTile; ++in) {
+                const bool on = sees(sp, t0 + in) && !(holes >> in & 1);
+                const int64_t row = __shfl(at, in);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int ch = 32 * b + 8 * (x >> 2) + 4 * h + (x & 3);
+                        const float one = on && ch < a.dim ? widen(vp[row * a.v.ts + ch]) : 0.f;
+                        if (!finite32(one)) o[b][x] += one;
+                    }
+            }
+        }
+    }
+    // The waves' sums, in order.
+    l = both_sum(l);
+    if (lane < 32) {
+        top_of[wave][n] = m;
+        sum_of[wave][n] = l;
+    }
+    __syncthreads();
+    float mt = top_of[0][n], lt = 0.f;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) mt = fmaxf(mt, top_of[w][n]);
+    const float ref = mt == -INFINITY ? 0.f : mt, f = exp2f(m - ref);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) lt += sum_of[w][n] * exp2f(top_of[w][n] - ref);
+    for (int w = 0; w < WAVES; ++w) {
+        if (wave == w)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    f32x4* to = (f32x4*)&sums[n][32 * b + 8 * x + 4 * h];
+                    const f32x4 mine = {o[b][4 * x] * f, o[b][4 * x + 1] * f, o[b][4 * x + 2] * f, o[b][4 * x + 3] * f};
+                    *to = w ? *to + mine : mine;
+                }
+        __syncthreads();
+    }
+    const bool empty = mt == -INFINITY && lt == 0.f;
+    if (wave == 0 && lane < 32) {
+        inverse[n] = empty ? 0.f : 1.f / lt;
+        if (a.lse && r <= last_row)
+            a.lse[(pl.q.first + tok) * a.q_heads + head] = empty ? -INFINITY : (mt + log2f(lt)) * 0.69314718055994530942f;
+    }
+    __syncthreads();
+    for (int in = wave; in <= last_row - pl.row0; in += WAVES) {
+        const int row = pl.row0 + in, t = rw.token(row), g = pl.kh * a.group + (row - t * a.group);
+        T* to = (T*)a.out.p + (pl.q.first + t) * a.out.ts + g * a.out.hs;
+        for (int ch = lane; ch < a.dim; ch += 64) to[ch] = narrow<T>(sums[in][ch] * inverse[in]);
+    }
+}
+
+// Whether rows of a tensor lie on multiples of four elements.
+template <typename T>
+bool fours(const HeadsIn& h) {
+    return (uintptr_t)h.p % (4 * sizeof(T)) == 0 && h.ts % 4 == 0 && h.hs % 4 == 0;
+}
+
+template <typename T, int NB, bool PAGED, bool VEC>
+hipError_t run(const AttentionArgs& a, hipStream_t stream) {
+    BlockMap map;
+    const int64_t blocks = ((int64_t)a.max_q * a.group + kRowsWg - 1) / kRowsWg;
+    if (!block_map(blocks, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
+    // Where there is no workgroup for every CU eight waves share the keys (8 sequences of 8,000 keys,
+    // 32 FP32 heads of 128 on 8 key heads: 721 us with four, 487 so).
+    if (NB <= 4 && blocks * a.kv_heads * a.sequences <= 256)
+        attention_any_kernel<T, NB, PAGED, VEC, NB <= 4 ? 8 : 4><<<map.grid, 512, 0, stream>>>(a, map);
+    else
+        attention_any_kernel<T, NB, PAGED, VEC, 4><<<map.grid, 256, 0, stream>>>(a, map);
+    return hipGetLastError();
+}
+template <typename T, int NB, bool PAGED>
+hipError_t by_rows(const AttentionArgs& a, hipStream_t stream) {
+    return a.dim % 4 == 0 && fours<T>(a.q) && fours<T>(a.k) ? run<T, NB, PAGED, true>(a, stream) : run<T, NB, PAGED, false>(a, stream);
+}
+template <typename T, bool PAGED>
+hipError_t by_dim(const AttentionArgs& a, hipStream_t stream) {
+    return a.dim <= 64 ? by_rows<T, 2, PAGED>(a, stream) : (a.dim <= 128 ? by_rows<T, 4, PAGED>(a, stream) : by_rows<T, 8, PAGED>(a, stream));
+}
+template <typename T>
+hipError_t by_keys(const AttentionArgs& a, hipStream_t stream) {
+    return a.pages.table ? by_dim<T, true>(a, stream) : by_dim<T, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace fa
+
+hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream) {
+    if (dtype == DCN_DTYPE_F16) return fa::by_keys<_Float16>(a, stream);
+    if (dtype == DCN_DTYPE_BF16) return fa::by_keys<fa::bf16>(a, stream);
+    return fa::by_keys<float>(a, stream);
+}
+
+}  // namespace dcn
