@@ -88,6 +88,7 @@ size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 
 // Any head size, type, stride and alignment (dcn_kernels_attention_any.hip, _rows.hip).
 hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream);
+hipError_t launch_attention_any_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).

@@ -430,7 +430,7 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
         bool matrix = matrix_heads(shape);
         for (const dcn::HeadsIn* h : {&a.q, &a.k, &a.v, &a.o, &a.dout}) matrix = matrix && matrix_tensor(*h, a.group);
         for (const dcn::HeadsOut* h : {&a.dq, &a.dk, &a.dv}) matrix = matrix && matrix_tensor(*h);
-        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix_backward : dcn::launch_attention_rows_backward)(shape->dtype, a,
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix_backward : dcn::launch_attention_any_backward)(shape->dtype, a,
                                                                                                           (hipStream_t)stream));
         return DCN_OK;
     });

@@ -62,6 +62,18 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int p, int n) {
 }
 __device__ __forceinline__ bool sees(const Span& s, int j) { return j < s.hi && (j >= s.lo || j < s.sink); }
 
+// Positions that see key j: [from, to), and from `from` on without an end for a sink.
+struct Seen {
+    int from, to;
+};
+__device__ __forceinline__ Seen seen_of(const AttentionArgs& a, int j, int n) {
+    const int64_t f = j / a.frame, fr = a.frame;
+    int64_t from = a.ahead < 0 ? 0 : (f - a.ahead) * fr, to = a.back < 0 || f < a.sinks ? n : (f + a.back + 1) * fr;
+    from = from < 0 ? 0 : (from > n ? n : from);
+    to = to > n ? n : to;
+    return Seen{(int)from, (int)to};
+}
+
 // Row of token j of sequence s in the paged cache, in tokens of the pool, or -1.
 __device__ __forceinline__ int64_t paged_row(const PagesArgs& pg, int s, int j) {
     const int page = pg.table[(int64_t)s * pg.width + (j >> pg.shift)];

@@ -1,6 +1,6 @@
-// Gradients of frame attention one row at a time: any head size up to 256, FP16, BF16 and FP32,
-// any stride and alignment. The matrix kernels take the aligned 16-bit heads of 64 and 128
-// channels; these take the rest, and are the plain statement of what those compute.
+// Gradients of frame attention one row at a time, for heads of 129 to 256 channels: FP16, BF16 and
+// FP32, any stride and alignment. Smaller heads have tiled kernels, of whose sums these are the
+// plain statement.
 //
 // One wave per query row, or per key row for the gradients of keys and values. A pass handles
 // 64 rows of the other side: lane = row for the dot products (the wave's own vector is in LDS as

