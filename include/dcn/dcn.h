@@ -770,13 +770,13 @@ dcn_status dcn_cache_append_dev(dcn_context* ctx, const dcn_cache* cache, const 
  * Softmax statistics and sums are FP32. Sequence s holds rows cu_q[s] .. cu_q[s + 1] of the
  * queries and cu_kv[s] .. cu_kv[s + 1] of the keys; null: rows s * max_q .. of max_q each
  * (keys: max_kv). max_q and max_kv are at least the longest sequence's lengths: they size
- * the launch. Rows of no sequence are not written. */
+ * the launch (max_q times the heads that share a key head is below 2^31 - 256). Rows of no sequence are not written. */
 typedef struct dcn_attention_shape {
     int32_t dtype; /* dcn_dtype */
     int32_t sequences;
     int32_t q_heads;
     int32_t kv_heads;
-    int32_t head_dim; /* 1 .. DCN_ATTENTION_MAX_HEAD_DIM; 64 and 128 in 16 bits run on the matrix cores */
+    int32_t head_dim; /* 1 .. DCN_ATTENTION_MAX_HEAD_DIM; 64 and 128 in 16 bits are fastest, others run in FP32 */
     int32_t frame_tokens;
     int32_t back;
     int32_t ahead;

@@ -12,8 +12,8 @@
 // Both may split the key tiles over workgroups; a second kernel then joins the parts.
 //
 // What bounds them. Tile kernel: the issue of vector and matrix instructions and the waits between
-// them at two waves a SIMD (128 channels: MFMA about a third of the cycles, vector instructions
-// another); 7,680 tokens in windows of nine frames of 256, 16 heads of 128 on 4: 140 to 150 us, 840 to
+// them at two waves a SIMD (128 channels: MFMA 44 % of the cycles, vector instructions about as many,
+// which overlap in part); 7,680 tokens in windows of nine frames of 256, 16 heads of 128 on 4: 140 to 150 us, 840 to
 // 890 TFLOP/s of the 1,220 that a large product reaches; 2 x 4,096 causal tokens, 16 heads of 64: 116 us,
 // of 128: 184 us. Few kernel: HBM where histories are long (32 tokens on 16,384 of 20,011 keys, 32 heads of 128
 // on 8: 314 us, 5.5 TB/s), else the chain of launch, first tile and join (one token on 777 keys, 8 heads of 64:
