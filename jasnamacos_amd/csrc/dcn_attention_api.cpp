@@ -1,6 +1,7 @@
 // C-ABI host layer of the frame-attention operators: rotary positions, the paged cache's
 // append, windowed attention and the gated norms. Checks every size, stride and pointer that
 // a kernel relies on, then launches; nothing here allocates or synchronises.
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -109,7 +110,7 @@ dcn_status check_attention(dcn_context* ctx, const dcn_attention_shape* s, bool 
     REQUIRE_SHAPE(s->sinks >= 0, "sinks must not be negative");
     REQUIRE_SHAPE(s->max_q >= 0 && s->max_kv >= 0, "max_q and max_kv must not be negative");
     REQUIRE_SHAPE(s->q_tokens >= 0 && s->kv_tokens >= 0, "q_tokens and kv_tokens must not be negative");
-    REQUIRE_SHAPE(s->scale == s->scale, "scale is not a number");
+    REQUIRE_SHAPE(std::isfinite(s->scale), "scale must be finite");
     // Packed rows are counted by an int.
     REQUIRE_SHAPE((int64_t)s->max_q * (s->q_heads / s->kv_heads) < INT32_MAX - 256,
                   "max_q times the heads that share a key head must be below 2^31 - 256");
@@ -187,7 +188,8 @@ dcn_status check_norm(dcn_context* ctx, const dcn_norm_shape* s, dcn::NormArgs* 
     REQUIRE_SHAPE(s->channels >= 1 && s->channels <= DCN_NORM_MAX_CHANNELS, "norm channels must be 1..8192");
     REQUIRE_SHAPE(s->tokens >= 0 && s->tokens <= INT32_MAX, "norm tokens must be 0..2^31-1");
     REQUIRE_SHAPE(s->gate_tokens >= 1, "gate_tokens must be positive");
-    REQUIRE_SHAPE(s->eps >= 0.f, "eps must not be negative");
+    REQUIRE_SHAPE(s->eps >= 0.f && std::isfinite(s->eps) && std::isfinite(s->residual_scale),
+                  "eps must be finite and not negative, residual_scale finite");
     *a = dcn::NormArgs{};
     a->channels = s->channels;
     a->tokens = s->tokens;

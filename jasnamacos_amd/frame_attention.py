@@ -98,6 +98,18 @@ _NORM = struct.Struct("iiqqff")
 _NO_STRIDES = (0, 0)
 
 
+def _outside() -> DeformConvError:
+    """For a size that its C type does not hold (struct.error of a layout above)."""
+    return DeformConvError(INVALID_SHAPE, "a size is outside its C type")
+
+
+def _factor(name: str, value) -> float:
+    """A number that FP32 holds (packing one that it does not gives an infinity)."""
+    value = float(value)
+    _need(abs(value) <= torch.finfo(torch.float32).max, f"{name} is not a finite FP32 number")
+    return value
+
+
 def _fresh(count: int, like):
     """Memory for a handle. The allocator may hand out what work on the current stream still
     reads; the handle's calls may be on another one."""
@@ -142,7 +154,10 @@ class Rotary(_Handle):
         self.head_dim, self.pairs, self.interleaved = int(head_dim), tuple(int(p) for p in pairs), bool(interleaved)
         _need(len(self.pairs) == 3, "rotary pairs are three numbers (time, height, width)")
         self._freq_shape = (sum(self.pairs),)
-        self._c = {t: _ROTARY.pack(code, self.head_dim, *self.pairs, self.interleaved) for t, code in DTYPES.items()}
+        try:
+            self._c = {t: _ROTARY.pack(code, self.head_dim, *self.pairs, self.interleaved) for t, code in DTYPES.items()}
+        except struct.error:
+            raise _outside() from None
 
     def frequencies(self, base: float = 10000.0, device="cuda"):
         """A usual choice of freq: each axis from 1 down to 1 / base."""
@@ -181,7 +196,10 @@ def _cache(k_pages, v_pages, table) -> bytes:
     _whole("v_pages", v_pages, dtype, shape)
     _whole("table", table, torch.int32, table.shape)
     pages, page_tokens, heads, dim = shape
-    return _CACHE.pack(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
+    try:
+        return _CACHE.pack(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
+    except struct.error:
+        raise _outside() from None
 
 
 class CacheAppend(_Handle):
@@ -210,7 +228,10 @@ class CacheAppend(_Handle):
         if rotary is not None:
             rotary._check(positions, freq, tokens)
             r = rotary._c[dtype]
-        s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
+        try:
+            s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
+        except struct.error:
+            raise _outside() from None
         status = self._lib.dcn_cache_append_dev(
             self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
             kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
@@ -232,14 +253,17 @@ class FrameAttention(_Handle):
               "q_heads must be a positive multiple of kv_heads")
         _need(self.head_dim > 0, "head_dim must be positive")
         self.frame_tokens, self.back, self.ahead, self.sinks = int(frame_tokens), int(back), int(ahead), int(sinks)
-        self.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        self.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else _factor("scale", scale)
 
     def _pack(self, q, sequences, max_q, max_kv, q_tokens, kv_tokens, *strides) -> bytes:
         """The packed dcn_attention_shape; strides: (token, head, ...) of q, k, v, out, dout, dq, dk, dv."""
         flat = [x for s in strides for x in s[:2]]
         flat += [0] * (16 - len(flat))
-        return _ATTENTION.pack(_dtype(q), sequences, self.q_heads, self.kv_heads, self.head_dim, self.frame_tokens,
-                               self.back, self.ahead, self.sinks, max_q, max_kv, self.scale, q_tokens, kv_tokens, *flat)
+        try:
+            return _ATTENTION.pack(_dtype(q), sequences, self.q_heads, self.kv_heads, self.head_dim, self.frame_tokens,
+                                   self.back, self.ahead, self.sinks, max_q, max_kv, self.scale, q_tokens, kv_tokens, *flat)
+        except struct.error:
+            raise _outside() from None
 
     def _runs(self, q_tokens, kv_tokens, cu_q, cu_kv, max_q, max_kv):
         """(sequences, max_q, max_kv): without index arrays, one sequence of all rows, or the
@@ -339,7 +363,7 @@ class GatedNorm(_Handle):
                  eps: float = 1e-6):
         super().__init__(ctx)
         self.channels, self.gate_tokens = int(channels), int(gate_tokens)
-        self.residual_scale, self.eps = float(residual_scale), float(eps)
+        self.residual_scale, self.eps = _factor("residual_scale", residual_scale), _factor("eps", eps)
         self._kept = None
         _need(self.channels > 0 and self.gate_tokens > 0, "channels and gate_tokens must be positive")
 
@@ -348,7 +372,10 @@ class GatedNorm(_Handle):
             raise DeformConvError(INVALID_ARGUMENT, "the residual stream is missing")
         if x.dim() != 2:
             raise DeformConvError(INVALID_SHAPE, f"the residual stream has {x.dim()} dimensions; expected [tokens][channels]")
-        return _NORM.pack(_dtype(x), self.channels, x.shape[0], self.gate_tokens, self.residual_scale, self.eps)
+        try:
+            return _NORM.pack(_dtype(x), self.channels, x.shape[0], self.gate_tokens, self.residual_scale, self.eps)
+        except struct.error:
+            raise _outside() from None
 
     def _check_all(self, x, needed, tensors, gates, vectors, sums=()) -> None:
         for name, t in needed:
