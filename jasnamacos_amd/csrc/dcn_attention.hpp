@@ -50,7 +50,16 @@ struct AttentionArgs {
     HeadsOut dq, dk, dv;
     const float* lse_in;
     void* workspace;
+    int any_splits;  // launch_attention_any: workgroups that share a row block's keys
 };
+
+// Keys that `tokens` adjacent queries see at most, in tiles of `tile`.
+inline int64_t attention_keys(int max_kv, int frame, int back, int sinks, int64_t tokens, int tile) {
+    const int64_t frames = (int64_t)back + 1 + sinks;
+    if (back < 0 || frames > max_kv / frame) return max_kv;
+    const int64_t window = frames * frame + tokens + 2 * tile;
+    return window < max_kv ? window : (int64_t)max_kv;
+}
 
 hipError_t launch_rotary(int dtype, int64_t tokens, int heads, const HeadsIn& x, const HeadsOut& out,
                          const RotaryArgs& r, hipStream_t stream);
@@ -88,6 +97,8 @@ size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 
 // Any head size, type, stride and alignment (dcn_kernels_attention_any.hip, _rows.hip).
 hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream);
+int attention_any_splits(const dcn_attention_shape& s);
+size_t attention_any_workspace(const dcn_attention_shape& s);
 hipError_t launch_attention_any_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 

@@ -165,8 +165,11 @@ bool matrix_pool(const dcn_cache* c) { return c->page_tokens >= 8 && (int64_t)c-
 size_t attention_workspace(const dcn_attention_shape* s, int pass) {
     if (pass == DCN_ATTENTION_BACKWARD)  // the rows' delta at least
         return matrix_heads(s) ? dcn::attention_backward_workspace(*s) : (size_t)s->q_tokens * s->q_heads * sizeof(float);
-    return matrix_heads(s) ? dcn::attention_forward_workspace(*s) : 0;
+    return matrix_heads(s) ? dcn::attention_forward_workspace(*s) : dcn::attention_any_workspace(*s);
 }
+
+// The workspace of heads that the matrix kernels take is for their parts, whichever kernel runs.
+int any_splits(const dcn_attention_shape* s) { return matrix_heads(s) ? 1 : dcn::attention_any_splits(*s); }
 
 dcn_status check_workspace(dcn_context* ctx, const void* p, size_t have, size_t need) {
     if (!need) return DCN_OK;
@@ -336,6 +339,7 @@ dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape
         a.cu_q = d_cu_q;
         a.cu_kv = d_cu_kv;
         a.workspace = d_workspace;
+        a.any_splits = any_splits(shape);
         const bool matrix = matrix_heads(shape) && matrix_tensor(a.q) && matrix_tensor(a.k) && matrix_tensor(a.v) && matrix_tensor(a.out);
         DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_any)(shape->dtype, a, (hipStream_t)stream));
         return DCN_OK;
@@ -377,6 +381,7 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
         a.cu_kv = d_kv_lens;
         a.pages.table = d_table;
         a.workspace = d_workspace;
+        a.any_splits = any_splits(shape);
         const bool matrix = matrix_heads(shape) && matrix_pool(cache) && matrix_tensor(a.q) && matrix_tensor(a.k) &&
                             matrix_tensor(a.v) && matrix_tensor(a.out);
         DCN_HIP(ctx, (matrix ? dcn::launch_attention_matrix : dcn::launch_attention_any)(shape->dtype, a, (hipStream_t)stream));

@@ -389,10 +389,7 @@ Plan plan_of(int dim, int sequences, int kv_heads, int group, int max_q, int max
     Plan p;
     const int64_t rows = (int64_t)max_q * group, wide = (rows + 127) / 128 * kv_heads * sequences;
     // Keys that one block of `block` rows sees at most.
-    const auto keys_of = [&](int block, int tile) {
-        const int64_t window = back < 0 ? max_kv : ((int64_t)back + 1 + sinks) * frame + block / group + 2 * tile;
-        return window < max_kv ? window : (int64_t)max_kv;
-    };
+    const auto keys_of = [&](int block, int tile) { return attention_keys(max_kv, frame, back, sinks, block / group, tile); };
     const int64_t keys = keys_of(128, 64);
     // Few rows, or so few workgroups of 128 rows that 32-row ones with four (eight) waves on the keys
     // are done sooner, though each key tile is read four times as often (256 x 128 rows, 64

@@ -9,10 +9,12 @@
 // so that a lane loads four adjacent ones. Operands come straight from memory, widened on the way:
 // a lane its key's channels, 32 lanes one value row's, which whole lines serve in both cases.
 //
-// A workgroup has 32 rows; its four waves take the key tiles in turn, without a barrier until
-// their sums are joined through LDS. Bound: the FP32 products, a sixteenth of the 16-bit rate, and
+// A workgroup has 32 rows; its four (or eight) waves take the key tiles in turn, without a barrier
+// until their sums are joined through LDS. Where rows are few, workgroups share the key tiles of a
+// block of rows, and a second kernel joins their parts. Bound: the FP32 products, a sixteenth of the 16-bit rate, and
 // for few rows the loads' latency. 2,048 causal tokens, 8 FP32 heads of 64: 110 us (39 of the
-// 157 TFLOP/s), of 128: 172 us; FP16 heads of 96: 165 us.
+// 157 TFLOP/s), of 128: 172 us; FP16 heads of 96: 165 us. One FP32 token on 8,000 paged keys, 8
+// sequences of 32 heads of 128 on 8: 170 us (3.1 TB/s).
 #include "dcn_attention_mfma.hpp"
 
 namespace dcn {
@@ -44,15 +46,18 @@ __device__ __forceinline__ f32x4 load4(const T* row, int at, int dim) {
 __device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ bool finite32(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) != 0x7f800000u; }
 
+// FP32 values of a part: the channels, then maximum and sum.
+__device__ __host__ inline int part_line(int dim) { return (dim + 3) / 4 * 4 + 4; }
+
 // VEC: rows of four-element alignment and heads of whole fours. NB: blocks of 32 channels.
 template <typename T, int NB, bool PAGED, bool VEC, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void attention_any_kernel(AttentionArgs a, BlockMap map) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void attention_any_kernel(AttentionArgs a, BlockMap map, int splits) {
     constexpr int LINE = NB * 32 + 4;
     __shared__ __attribute__((aligned(16))) float sums[kRowsWg][LINE];
     __shared__ float top_of[WAVES][kRowsWg], sum_of[WAVES][kRowsWg], inverse[kRowsWg];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
     Place pl;
-    if (!place_of<kRowsWg>(a, map, 1, &pl)) return;
+    if (!place_of<kRowsWg>(a, map, splits, &pl)) return;
     const Rows rw = rows_of(a.group);
     const int last_row = pl.rows - 1 < pl.row0 + kRowsWg - 1 ? pl.rows - 1 : pl.row0 + kRowsWg - 1;
     const Spread all = spread_of(a, pl, rw, pl.row0, last_row);
@@ -75,7 +80,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void att
         for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
     float m = -INFINITY, l = 0.f;
     const TileList<kTile> list(all);
-    for (int i = wave; i < list.count; i += WAVES) {
+    const int per = (list.count + splits - 1) / splits, from = pl.split * per;
+    const int stop = from + per < list.count ? from + per : list.count;
+    for (int i = from + wave; i < stop; i += WAVES) {
         const int t0 = list.tile(i), j = t0 + n;
         // Row of this lane's key in memory; keys that are not there stand in for the last one, unseen.
         int64_t at = pl.kv.first + (j < pl.kv.count ? j : pl.kv.count - 1);
@@ -201,6 +208,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void att
         __syncthreads();
     }
     const bool empty = mt == -INFINITY && lt == 0.f;
+    if (splits > 1) {  // this part's sums, their reference and weight
+        const int line = part_line(a.dim);
+        if (wave == 0 && lane < 32 && r <= last_row) {
+            float* w = (float*)a.workspace + (((pl.q.first + tok) * a.q_heads + head) * splits + pl.split) * line + line - 4;
+            w[0] = mt;
+            w[1] = lt;
+        }
+        for (int in = wave; in <= last_row - pl.row0; in += WAVES) {
+            const int row = pl.row0 + in, t = rw.token(row), g = pl.kh * a.group + (row - t * a.group);
+            float* to = (float*)a.workspace + (((pl.q.first + t) * a.q_heads + g) * splits + pl.split) * line;
+            for (int ch = lane; ch < a.dim; ch += 64) to[ch] = sums[in][ch];
+        }
+        return;
+    }
     if (wave == 0 && lane < 32) {
         inverse[n] = empty ? 0.f : 1.f / lt;
         if (a.lse && r <= last_row)
@@ -212,6 +233,39 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void att
         T* to = (T*)a.out.p + (pl.q.first + t) * a.out.ts + g * a.out.hs;
         for (int ch = lane; ch < a.dim; ch += 64) to[ch] = narrow<T>(sums[in][ch] * inverse[in]);
     }
+}
+
+// The parts of all splits (32 at most) of a row and head, by a wave: lane s has split s's maximum
+// and sum; the sums are added in order of the splits.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_any_join_kernel(AttentionArgs a, int splits) {
+    const int lane = threadIdx.x & 63, line = part_line(a.dim);
+    const Run q = run_of(a.cu_q, blockIdx.z, a.max_q, a.q_tokens);
+    const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int64_t tok = item / a.q_heads;
+    const int head = (int)(item - tok * a.q_heads);
+    if (tok >= q.count || tok >= a.max_q) return;
+    const int64_t row = q.first + tok, index = row * a.q_heads + head;
+    const float* parts = (const float*)a.workspace + index * splits * line;
+    const float m = lane < splits ? parts[lane * line + line - 4] : -INFINITY;
+    const float l = lane < splits ? parts[lane * line + line - 3] : 0.f;
+    const float top = wave_max(m), w = exp2f(m - (top == -INFINITY ? 0.f : top)), sum = wave_sum(w * l);
+    const bool empty = top == -INFINITY && sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    T* out = (T*)a.out.p + row * a.out.ts + head * a.out.hs;
+    for (int first = 0; first < a.dim; first += 64) {
+        const int ch = first + lane, at = ch < a.dim ? ch : a.dim - 1;
+        float o = 0.f;
+        for (int s = 0; s < splits; s += 8) {  // eight loads at once; w is 0 past the last split
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = s + u < splits ? parts[(s + u) * line + at] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) o = fmaf(__shfl(w, s + u), v[u], o);
+        }
+        if (ch < a.dim) out[ch] = narrow<T>(o * inv);
+    }
+    if (a.lse && lane == 0) a.lse[index] = empty ? -INFINITY : (top + log2f(sum)) * 0.69314718055994530942f;
 }
 
 // Gradients, of heads of up to 128 channels: one pass over query rows (dQ and delta) and one over
@@ -416,14 +470,19 @@ bool fours(const HeadsIn& h) {
 template <typename T, int NB, bool PAGED, bool VEC>
 hipError_t run(const AttentionArgs& a, hipStream_t stream) {
     BlockMap map;
+    const int splits = a.any_splits;
     const int64_t blocks = ((int64_t)a.max_q * a.group + kRowsWg - 1) / kRowsWg;
-    if (!block_map(blocks, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
+    if (!block_map(blocks * splits, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
     // Where there is no workgroup for every CU eight waves share the keys (8 sequences of 8,000 keys,
     // 32 FP32 heads of 128 on 8 key heads: 721 us with four, 487 so).
     if (NB <= 4 && blocks * a.kv_heads * a.sequences <= 256)
-        attention_any_kernel<T, NB, PAGED, VEC, NB <= 4 ? 8 : 4><<<map.grid, 512, 0, stream>>>(a, map);
+        attention_any_kernel<T, NB, PAGED, VEC, NB <= 4 ? 8 : 4><<<map.grid, 512, 0, stream>>>(a, map, splits);
     else
-        attention_any_kernel<T, NB, PAGED, VEC, 4><<<map.grid, 256, 0, stream>>>(a, map);
+        attention_any_kernel<T, NB, PAGED, VEC, 4><<<map.grid, 256, 0, stream>>>(a, map, splits);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (splits == 1) return hipSuccess;
+    const int64_t rows = (int64_t)a.max_q * a.q_heads;
+    attention_any_join_kernel<T><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, splits);
     return hipGetLastError();
 }
 template <typename T, int NB, bool PAGED>
@@ -469,6 +528,26 @@ hipError_t launch_attention_any_backward(int dtype, const AttentionArgs& a, hipS
     if (dtype == DCN_DTYPE_F16) return fa::grad<_Float16>(a, stream);
     if (dtype == DCN_DTYPE_BF16) return fa::grad<fa::bf16>(a, stream);
     return fa::grad<float>(a, stream);
+}
+
+int attention_any_splits(const dcn_attention_shape& s) {
+    const int group = s.q_heads / s.kv_heads;
+    const int64_t blocks = ((int64_t)s.max_q * group + fa::kRowsWg - 1) / fa::kRowsWg, groups = blocks * s.kv_heads * s.sequences;
+    const int64_t keys = attention_keys(s.max_kv, s.frame_tokens, s.back, s.sinks, fa::kRowsWg / group, fa::kTile);
+    const int64_t tiles = (keys + fa::kTile - 1) / fa::kTile, waves = s.head_dim <= 128 ? 8 : 4;
+    // Row blocks that leave half of the CUs idle or more: a workgroup a CU, of a tile a wave at least,
+    // and 32 parts the most that the join adds quickly. Up to two tiles a wave the join costs what it
+    // saves. One FP32 token, whole and in parts: 540 keys of 8 heads of 64: 23.9 and 20.4 us; 8,000:
+    // 224 and 24; for 8 sequences of 32 heads of 128 on 8, 488 and 170; 16 of 8 heads of 64, 309 and 174.
+    if (groups < 1 || groups > 128 || tiles <= 2 * waves) return 1;
+    int64_t splits = 256 / groups;
+    splits = splits < tiles / waves ? splits : tiles / waves;
+    return (int)(splits < 32 ? splits : 32);
+}
+
+size_t attention_any_workspace(const dcn_attention_shape& s) {
+    const int splits = attention_any_splits(s);
+    return splits == 1 ? 0 : (size_t)s.q_tokens * s.q_heads * splits * fa::part_line(s.head_dim) * sizeof(float);
 }
 
 hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream) {
