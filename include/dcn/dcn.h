@@ -827,7 +827,8 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
  * rstd ([tokens][2] FP32: r1, r2) may be null where no backward follows. x_out may be x.
  * low, where it is given, receives what rounding takes from x_out in 16 bits (with each
  * row's r1 and r2), so that the backward has x_out in FP32 even where x is overwritten;
- * dcn_gated_norm_low_bytes of it, 16-byte aligned (0: FP32, none is kept). */
+ * dcn_gated_norm_low_bytes of it, 16-byte aligned (0: FP32, none is kept). It is for the
+ * backward of this forward: two forwards whose backwards follow later need two. */
 #define DCN_NORM_MAX_CHANNELS 8192
 typedef struct dcn_norm_shape {
     int32_t dtype; /* dcn_dtype of every tensor but rstd, dw_post and dw_pre (FP32) */
@@ -843,8 +844,8 @@ dcn_status dcn_gated_norm_forward_dev(dcn_context* ctx, const dcn_norm_shape* sh
 size_t dcn_gated_norm_low_bytes(const dcn_norm_shape* shape);
 /* Gradients from those of x_out and of y (dy null: y was not made): dh, dx, and where their
  * pointers are given dgate, dw_post, dw_pre. Sums over tokens are FP32 in a fixed order.
- * low may be null: x_out is then taken as it was rounded. A row of low that was left by
- * another forward (its r1 or r2 differs from rstd's) counts as zeros. */
+ * low is what the forward that made rstd wrote, or null: x_out is then taken as it was
+ * rounded. A row of low whose r1 or r2 differs from rstd's counts as zeros. */
 size_t dcn_gated_norm_workspace_bytes(const dcn_norm_shape* shape);
 dcn_status dcn_gated_norm_backward_dev(dcn_context* ctx, const dcn_norm_shape* shape, const void* d_h,
                                        const void* d_x_out, const void* d_gate, const void* d_w_post,

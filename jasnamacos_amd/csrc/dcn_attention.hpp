@@ -82,7 +82,7 @@ struct NormArgs {
     const void *h, *x, *gate, *w_post, *w_pre;
     void *x_out, *y;
     float* rstd;
-    void* low;  // [tokens][2] FP32 (r1, r2), then [tokens][channels] of 16 bits; may be null
+    void* low;  // rounded-off halves of x_out (norm_low_bytes); may be null
     // backward
     const void *dx_out, *dy;
     void *dh, *dx, *dgate;
@@ -91,8 +91,13 @@ struct NormArgs {
 };
 hipError_t launch_norm_forward(int dtype, const NormArgs& a, hipStream_t stream);
 hipError_t launch_norm_backward(int dtype, const NormArgs& a, hipStream_t stream);
-// Bytes before the rounded-off halves in `low`.
-constexpr size_t norm_low_header(int64_t tokens) { return ((size_t)tokens * 8 + 15) / 16 * 16; }
+// `low` in blocks of 16 rows: r1 and r2 (FP32) of each, then [16][channels] of 16 bits. A row's place
+// does not depend on how many there are, so its statistics and its halves are always of one forward.
+constexpr int kLowRows = 16;
+constexpr int64_t norm_low_block(int channels) { return kLowRows * (8 + 2 * (int64_t)channels); }
+constexpr size_t norm_low_bytes(int64_t tokens, int channels) {
+    return (size_t)((tokens + kLowRows - 1) / kLowRows * norm_low_block(channels));
+}
 size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 
 // Any head size, type, stride and alignment (dcn_kernels_attention_any.hip, _rows.hip).

@@ -473,7 +473,7 @@ size_t dcn_gated_norm_low_bytes(const dcn_norm_shape* shape) {
     dcn::NormArgs a;
     try {
         if (!shape || check_norm(nullptr, shape, &a) != DCN_OK || shape->dtype == DCN_DTYPE_F32) return 0;
-        return dcn::norm_low_header(a.tokens) + (size_t)a.tokens * a.channels * 2;
+        return dcn::norm_low_bytes(a.tokens, a.channels);
     } catch (const std::exception&) {
         return 0;
     }

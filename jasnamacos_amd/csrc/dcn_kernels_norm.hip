@@ -83,6 +83,14 @@ __device__ __forceinline__ float with_low(float rounded, uint16_t low) {
         return fmaf((float)__builtin_bit_cast(_Float16, low), 1.f / 2048.f, rounded);
 }
 
+// A row's r1 and r2 in `low`, and its halves.
+__device__ __forceinline__ float* low_stats(const NormArgs& a, int64_t row) {
+    return (float*)((char*)a.low + row / kLowRows * norm_low_block(a.channels)) + row % kLowRows * 2;
+}
+__device__ __forceinline__ uint16_t* low_row(const NormArgs& a, int64_t row) {
+    return (uint16_t*)((char*)a.low + row / kLowRows * norm_low_block(a.channels) + kLowRows * 8) + row % kLowRows * a.channels;
+}
+
 // A lane's channels of one row's tensors, as they are stored: loaded a row ahead.
 template <typename T, int NV>
 struct RawRow {
@@ -107,8 +115,8 @@ struct RawRow {
         r1 = a.rstd[row * 2];
         r2 = a.rstd[row * 2 + 1];
         if (sizeof(T) == 2 && a.low) {
-            low1 = ((const float*)a.low)[row * 2];
-            low2 = ((const float*)a.low)[row * 2 + 1];
+            low1 = low_stats(a, row)[0];
+            low2 = low_stats(a, row)[1];
         }
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
@@ -117,7 +125,7 @@ struct RawRow {
                 get<WIDE>((const T*)a.dy + base, at, c, &dy[n]);
                 get<WIDE>((const T*)a.x_out + base, at, c, &x_out[n]);
                 if (sizeof(T) == 2 && a.low)
-                    get<WIDE>((const uint16_t*)((const char*)a.low + norm_low_header(a.tokens)) + base, at, c, &low[n]);
+                    get<WIDE>((const uint16_t*)low_row(a, row), at, c, &low[n]);
             }
             get<WIDE>((const T*)a.dx_out + base, at, c, &dx_out[n]);
             get<WIDE>((const T*)a.h + base, at, c, &h[n]);
@@ -180,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
         }
         store_row<T, WIDE>((T*)a.x_out + base, at, c, h[n]);
         if (a.low) {
-            uint16_t* to = (uint16_t*)((char*)a.low + norm_low_header(a.tokens)) + base;
+            uint16_t* to = low_row(a, row);
             if constexpr (WIDE) {
                 if (at < c) {
                     Pack<uint16_t> p;
@@ -214,8 +222,8 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
         a.rstd[row * 2 + 1] = r2;
     }
     if (a.low && lane == 0) {
-        ((float*)a.low)[row * 2] = r1;
-        ((float*)a.low)[row * 2 + 1] = r2;
+        low_stats(a, row)[0] = r1;
+        low_stats(a, row)[1] = r2;
     }
 }
 

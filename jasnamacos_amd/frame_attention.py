@@ -365,6 +365,7 @@ class GatedNorm(_Handle):
         self.channels, self.gate_tokens = int(channels), int(gate_tokens)
         self.residual_scale, self.eps = _factor("residual_scale", residual_scale), _factor("eps", eps)
         self._kept = None
+        self._kept_for = None  # (rstd, packed shape) of the forward that wrote it
         _need(self.channels > 0 and self.gate_tokens > 0, "channels and gate_tokens must be positive")
 
     def _pack(self, x) -> bytes:
@@ -393,30 +394,50 @@ class GatedNorm(_Handle):
         """Bytes of forward_dev's `low` for a residual stream like x."""
         return int(self._lib.dcn_gated_norm_low_bytes(self._pack(x)))
 
-    def _low(self, s, low, like, make: bool):
-        """The pointer of the caller's low, or of the handle's own."""
+    def _low_of(self, s, low, like):
+        """The pointer of the caller's low, checked."""
         if like.dtype is torch.float32:
             return None
         count = self._lib.dcn_gated_norm_low_bytes(s)
         if not count:
             return None
-        if low is not None:
-            _on_device("low", low)
-            if low.dtype != torch.uint8 or low.numel() < count or not low.is_contiguous():
-                raise DeformConvError(INVALID_SHAPE, f"low is not {count} adjacent uint8 values")
-            return low.data_ptr()
+        _on_device("low", low)
+        if low.dtype != torch.uint8 or low.numel() < count or not low.is_contiguous():
+            raise DeformConvError(INVALID_SHAPE, f"low is not {count} adjacent uint8 values")
+        return low.data_ptr()
+
+    def _low_to_write(self, s, low, like, rstd):
+        """Where a forward that makes rstd writes: the caller's low, or the handle's own."""
+        own = self._kept_for
+        if low is not None or like.dtype is torch.float32:
+            if own is not None and own[0].data_ptr() == rstd.data_ptr():
+                self._kept_for = None  # rstd has another forward's now
+            return self._low_of(s, low, like)
+        self._kept_for = None
+        count = self._lib.dcn_gated_norm_low_bytes(s)
+        if not count:
+            return None
         if self._kept is None or self._kept.numel() < count:
-            if not make:
-                return None
             if self._kept is not None:
                 torch.cuda.synchronize(like.device)
             self._kept = _fresh(count, like)
+        self._kept_for = (rstd, s)
+        return self._kept.data_ptr()
+
+    def _low_to_read(self, s, low, like, rstd):
+        """What a backward reads: the caller's low, or the handle's own where the forward that made
+        rstd was its last one (the tensor is held, so nothing else can lie there)."""
+        if low is not None:
+            return self._low_of(s, low, like)
+        own = self._kept_for
+        if own is None or own[1] != s or own[0].data_ptr() != rstd.data_ptr():
+            return None
         return self._kept.data_ptr()
 
     def forward_dev(self, h, x, gate, w_post, w_pre, x_out, y=None, rstd=None, low=None, stream=None) -> None:
         """gate, w_post, w_pre may be None (ones); y None: no block follows. rstd ([tokens][2]
         FP32) is what backward_dev reads; with it, 16-bit calls keep what rounding takes from
-        x_out (low_bytes(x) uint8 values) in `low`, or in the handle for its next backward_dev."""
+        x_out (low_bytes(x) uint8 values) in `low`, or in the handle until its next such call."""
         s = self._pack(x)
         self._check_all(x, (("h", h), ("x", x), ("x_out", x_out)), (("y", y),), (("gate", gate),),
                         (("w_post", w_post), ("w_pre", w_pre)))
@@ -424,16 +445,16 @@ class GatedNorm(_Handle):
             _whole("rstd", rstd, torch.float32, (x.shape[0], 2))
         status = self._lib.dcn_gated_norm_forward_dev(
             self._ctx, s, h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre), x_out.data_ptr(), _ptr(y),
-            _ptr(rstd), None if rstd is None else self._low(s, low, x, True), stream and _stream(stream))
+            _ptr(rstd), None if rstd is None else self._low_to_write(s, low, x, rstd), stream and _stream(stream))
         if status:
             self.ctx._check(status)
 
     def backward_dev(self, h, x_out, gate, w_post, w_pre, rstd, dx_out, dy, dh, dx, dgate=None, dw_post=None,
                      dw_pre=None, low=None, stream=None) -> None:
         """Gradients from those of x_out and y (dy None where y was not made); dgate, dw_post and
-        dw_pre (FP32) where they are given. Rows whose low halves are not those of the forward
-        that made rstd (the handle ran another one since, and `low` is None) take x_out as it
-        was rounded."""
+        dw_pre (FP32) where they are given. low: that of the forward that made rstd; None: the
+        handle's own if that forward was its last with rstd and kept it there, else x_out is
+        taken as it was rounded."""
         s = self._pack(x_out)
         self._check_all(x_out, (("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dh", dh), ("dx", dx)),
                         (("dy", dy),), (("gate", gate), ("dgate", dgate)), (("w_post", w_post), ("w_pre", w_pre)),
@@ -442,5 +463,5 @@ class GatedNorm(_Handle):
         w, size = self._room(s, lambda: self._lib.dcn_gated_norm_workspace_bytes(s), x_out)
         self.ctx._check(self._lib.dcn_gated_norm_backward_dev(
             self.ctx.ctx, s, h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
-            rstd.data_ptr(), self._low(s, low, x_out, False), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(),
+            rstd.data_ptr(), self._low_to_read(s, low, x_out, rstd), dx_out.data_ptr(), _ptr(dy), dh.data_ptr(),
             dx.data_ptr(), _ptr(dgate), _ptr(dw_post), _ptr(dw_pre), w, size, _stream(stream)))
