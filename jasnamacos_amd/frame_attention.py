@@ -13,8 +13,10 @@ packed projection is taken as it is. As elsewhere in this package outputs are th
 calls are asynchronous on `stream` (None: the default stream), and errors are
 DeformConvError. A FrameAttention or GatedNorm keeps the workspace of its calls: calls that
 may run at the same time need a handle each, and a handle sizes its workspace in its first
-call of a size (reserve it before a graph capture by running that call once). Keep a handle
-until its calls on streams other than torch's current one have ended."""
+call of a size (reserve it before a graph capture by running that call once). A workspace that
+a larger call has replaced stays with the handle, since a captured graph may still use it. Keep
+a handle as long as the graphs captured with it, and until its calls on streams other than
+torch's current one have ended."""
 from __future__ import annotations
 
 import ctypes as C
@@ -125,6 +127,7 @@ class _Handle:
         self._ctx = ctx.ctx
         self._lib = ctx._lib
         self._workspace = None
+        self._replaced = []  # memory that larger calls have outgrown: graphs may hold its address
         self._sizes = {}  # workspace bytes of the shapes seen
 
     def _room(self, key, ask, like):
@@ -139,10 +142,17 @@ class _Handle:
             return None, 0
         w = self._workspace
         if w is None or w.numel() < count:
-            if w is not None:
-                torch.cuda.synchronize(w.device)  # calls in flight still use the old one
-            self._workspace = w = _fresh(count, like)
+            self._workspace = w = self._grown(w, count, like)
         return w.data_ptr(), w.numel()
+
+    def _grown(self, old, count, like):
+        """Memory of `count` bytes at least, and twice the old one's: all that is kept is less than
+        twice the newest."""
+        if old is None:
+            return _fresh(count, like)
+        new = _fresh(max(count, 2 * old.numel()), like)
+        self._replaced.append(old)
+        return new
 
 
 class Rotary(_Handle):
@@ -418,9 +428,7 @@ class GatedNorm(_Handle):
         if not count:
             return None
         if self._kept is None or self._kept.numel() < count:
-            if self._kept is not None:
-                torch.cuda.synchronize(like.device)
-            self._kept = _fresh(count, like)
+            self._kept = self._grown(self._kept, count, like)
         self._kept_for = (rstd, s)
         return self._kept.data_ptr()
 
