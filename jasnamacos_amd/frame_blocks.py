@@ -92,7 +92,11 @@ class _Norm(torch.autograd.Function):
 
 class FrameBlocks:
     """`layers` blocks of `channels` channels over frames of rows x columns tokens; a token sees
-    its own frame, the `back` frames before it and the first `sinks` ones."""
+    its own frame, the `back` frames before it and the first `sinks` ones.
+
+    Handles keep workspaces, so what may run at the same time has handles of its own: clip() and
+    its backward on each CUDA stream, and each FrameStream. A stream's graphs of clip() share its
+    handles, and are not replayed at the same time."""
 
     def __init__(self, ctx: HipDeformConv, channels: int, q_heads: int, kv_heads: int, head_dim: int, layers: int,
                  rows: int, columns: int, back: int, sinks: int = 1, dtype=torch.bfloat16, seed: int = 0, device="cuda"):
@@ -102,9 +106,11 @@ class FrameBlocks:
         pairs = head_dim // 2
         self.rotary = Rotary(ctx, head_dim, (pairs - 2 * (pairs // 3), pairs // 3, pairs // 3))
         self.freq = self.rotary.frequencies(device=device)
-        self.attention = FrameAttention(ctx, q_heads, kv_heads, head_dim, self.frame_tokens, back, 0, sinks)
         self.append = CacheAppend(ctx)
-        self.norm = GatedNorm(ctx, channels, self.frame_tokens, residual_scale=1.0 / math.sqrt(layers))
+        self.new_handles = lambda: (
+            FrameAttention(ctx, q_heads, kv_heads, head_dim, self.frame_tokens, back, 0, sinks),
+            GatedNorm(ctx, channels, self.frame_tokens, residual_scale=1.0 / math.sqrt(layers)))
+        self._handles = {}  # by CUDA stream
         self.channels, self.head_dim = channels, head_dim
         g = torch.Generator().manual_seed(seed)
 
@@ -117,6 +123,20 @@ class FrameBlocks:
         self.layers = [{"qkv": weight(channels, sum(self.split) * head_dim), "back": weight(q_heads * head_dim, channels),
                         "gate": weight(channels, channels), "w_post": ones(), "w_pre": ones()} for _ in range(layers)]
 
+    def _of_this_stream(self):
+        key = torch.cuda.current_stream().cuda_stream
+        if key not in self._handles:
+            self._handles[key] = self.new_handles()
+        return self._handles[key]
+
+    @property
+    def attention(self) -> FrameAttention:
+        return self._of_this_stream()[0]
+
+    @property
+    def norm(self) -> GatedNorm:
+        return self._of_this_stream()[1]
+
     def parameters(self):
         return [self.first] + [w for layer in self.layers for w in layer.values()]
 
@@ -124,20 +144,21 @@ class FrameBlocks:
         """The queries, keys and values of a packed projection, as they lie."""
         return qkv.view(len(qkv), sum(self.split), self.head_dim).split(self.split, 1)
 
-    def _start(self, x):
+    def _start(self, x, norm):
         """The first block's input: the norm of x, a closed gate before it."""
         closed = torch.zeros(len(x) // self.frame_tokens, self.channels, dtype=x.dtype, device=x.device)
-        return _Norm.apply(x, x, closed, self.first, self.first, self.norm)
+        return _Norm.apply(x, x, closed, self.first, self.first, norm)
 
     def clip(self, x, style, clips: int = 1):
         """x: [clips * frames * rows * columns][channels]; style: [clips * frames][channels], which
         the gates come from. The output of the last block's norm, differentiable."""
         longest = len(x) // clips
         positions = frame_positions(0, longest // self.frame_tokens, self.rows, self.columns, x.device).repeat(clips, 1)
-        x, y = self._start(x)
+        norm = self.norm
+        x, y = self._start(x, norm)
         for w in self.layers:
             h = _Attend.apply(y @ w["qkv"], self, positions, longest) @ w["back"]
-            x, y = _Norm.apply(h, x, style @ w["gate"], w["w_post"], w["w_pre"], self.norm)
+            x, y = _Norm.apply(h, x, style @ w["gate"], w["w_post"], w["w_pre"], norm)
         return y
 
     def stream(self, streams: int, frames: int, page_tokens: int = 16) -> "FrameStream":
@@ -154,6 +175,7 @@ class FrameStream:
         if blocks.frame_tokens % page_tokens:
             raise ValueError(f"{page_tokens} tokens a page do not divide a frame of {blocks.frame_tokens}")
         self.blocks, self.streams, self.time, self.frames = blocks, streams, 0, frames
+        self.attention, self.norm = blocks.new_handles()
         per_frame = blocks.frame_tokens // page_tokens
         kept = min(frames, blocks.sinks + blocks.back + 1)
         # A frame past the sinks lies where the one that has just left its window was.
@@ -178,16 +200,16 @@ class FrameStream:
         self.time += 1
         self.lens += n
         stream = torch.cuda.current_stream()
-        x, y = b._start(x)
+        x, y = b._start(x, self.norm)
         for w, (k_pages, v_pages) in zip(b.layers, self.pages):
             q, k, v = b.heads(y @ w["qkv"])
             turned = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             out = torch.empty_like(turned)
             b.append.run_dev(k, v, k_pages, v_pages, self.table, self.cu_q, self.lens, b.rotary, self.positions, b.freq,
                              q, turned, stream=stream)
-            b.attention.paged_dev(turned, k_pages, v_pages, self.table, self.cu_q, self.lens, out, max_q=n,
-                                  max_kv=self.time * n, stream=stream)
-            x, y = _Norm.apply(out.flatten(1) @ w["back"], x, style @ w["gate"], w["w_post"], w["w_pre"], b.norm)
+            self.attention.paged_dev(turned, k_pages, v_pages, self.table, self.cu_q, self.lens, out, max_q=n,
+                                     max_kv=self.time * n, stream=stream)
+            x, y = _Norm.apply(out.flatten(1) @ w["back"], x, style @ w["gate"], w["w_post"], w["w_pre"], self.norm)
         self.positions[:, 0] += 1
         return y
 
