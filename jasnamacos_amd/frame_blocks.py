@@ -20,6 +20,7 @@ import sys
 import time
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .deform_conv import HipDeformConv
 from .frame_attention import CacheAppend, FrameAttention, GatedNorm, Rotary
@@ -51,6 +52,7 @@ class _Attend(torch.autograd.Function):
         return out.flatten(1)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         qkv, turned, out, lse, positions = ctx.saved_tensors
         blocks, stream = ctx.blocks, torch.cuda.current_stream()
@@ -80,6 +82,7 @@ class _Norm(torch.autograd.Function):
         return x_out, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx_out, dy):
         h, x_out, gate, w_post, w_pre, rstd, low = ctx.saved_tensors
         dh, dx, dgate = torch.empty_like(h), torch.empty_like(h), torch.empty_like(gate)

@@ -1,5 +1,5 @@
-"""The example's blocks without a device: which handles they use. The operators' calls are
-recorded, not run."""
+"""The example's blocks without a device: which handles they use, and that they refuse second
+derivatives. The operators' calls are recorded, not run."""
 from __future__ import annotations
 
 import types
@@ -51,3 +51,14 @@ def test_handles(blocks):
         sets.append(one)
         kept.append(serving)  # alive: no other handle has its handles' ids
     assert len(set().union(*sets)) == sum(map(len, sets))
+
+
+def test_second_derivatives_are_refused(blocks):
+    """The operators have no gradient of their gradients: not a sum that leaves them out."""
+    net, _, _ = blocks
+    for w in net.parameters():
+        w.requires_grad_()
+    y = net.clip(torch.randn(18, 48), torch.randn(3, 48))
+    grads = torch.autograd.grad(y.sum(), net.parameters(), create_graph=True, allow_unused=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        sum(g.square().sum() for g in grads if g is not None).backward()
