@@ -769,7 +769,8 @@ dcn_status dcn_cache_append_dev(dcn_context* ctx, const dcn_cache* cache, const 
  * infinities included. Query head h reads key head h / (q_heads / kv_heads).
  * Softmax statistics and sums are FP32. Sequence s holds rows cu_q[s] .. cu_q[s + 1] of the
  * queries and cu_kv[s] .. cu_kv[s + 1] of the keys; null: rows s * max_q .. of max_q each
- * (keys: max_kv). max_q and max_kv are at least the longest sequence's lengths: they size
+ * (keys: max_kv). max_q and max_kv are at least the longest sequence's lengths (more than
+ * the rows that there are counts as those): they size
  * the launch (max_q times the heads that share a key head is below 2^31 - 256). Rows of no sequence are not written. */
 typedef struct dcn_attention_shape {
     int32_t dtype; /* dcn_dtype */

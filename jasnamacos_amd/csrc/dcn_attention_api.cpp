@@ -99,6 +99,15 @@ dcn_status check_cache(dcn_context* ctx, const dcn_cache* c, dcn::PagesArgs* out
     return DCN_OK;
 }
 
+// The bounds of the sequences' lengths are not above the rows that there are: plans and launches are
+// made for lengths that occur. (The paged call's keys are bounded by its table, in the kernels.)
+dcn_attention_shape fitted(const dcn_attention_shape& shape, bool paged) {
+    dcn_attention_shape s = shape;
+    if (s.q_tokens >= 0 && s.max_q > s.q_tokens) s.max_q = (int32_t)s.q_tokens;
+    if (!paged && s.kv_tokens >= 0 && s.max_kv > s.kv_tokens) s.max_kv = (int32_t)s.kv_tokens;
+    return s;
+}
+
 // The sizes, spans and strides of one attention call; pointers come later.
 dcn_status check_attention(dcn_context* ctx, const dcn_attention_shape* s, bool paged, dcn::AttentionArgs* a) {
     REQUIRE_SHAPE(known_dtype(s->dtype), "attention dtype " + std::to_string(s->dtype) + " is unknown");
@@ -306,23 +315,26 @@ dcn_status dcn_cache_append_dev(dcn_context* ctx, const dcn_cache* cache, const 
 size_t dcn_attention_workspace_bytes(const dcn_attention_shape* shape, dcn_attention_pass pass) {
     dcn::AttentionArgs a{};
     try {
-        if (!shape || check_attention(nullptr, shape, pass == DCN_ATTENTION_PAGED, &a) != DCN_OK) return 0;
-        return attention_workspace(shape, pass);
+        if (!shape) return 0;
+        const dcn_attention_shape s = fitted(*shape, pass == DCN_ATTENTION_PAGED);
+        if (check_attention(nullptr, &s, pass == DCN_ATTENTION_PAGED, &a) != DCN_OK) return 0;
+        return attention_workspace(&s, pass);
     } catch (const std::exception&) {
         return 0;
     }
 }
 
-dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape* shape, const void* d_q,
+dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape* given, const void* d_q,
                                      const void* d_k, const void* d_v, const int32_t* d_cu_q,
                                      const int32_t* d_cu_kv, void* d_out, float* d_lse, void* d_workspace,
                                      size_t workspace_bytes, void* stream) {
     return entry(ctx, [&]() -> dcn_status {
-        REQUIRE_POINTER(shape);
+        if (!given) return null_fail(ctx, "shape");
+        DCN_TRY(check_even(ctx, given, d_cu_q, d_cu_kv));
+        const dcn_attention_shape own = fitted(*given, false), *shape = &own;
         dcn::AttentionArgs a{};
         DCN_TRY(check_attention(ctx, shape, false, &a));
         DCN_TRY(check_out_strides(ctx, "out", shape->out_stride, shape->q_tokens, shape->q_heads, shape->head_dim));
-        DCN_TRY(check_even(ctx, shape, d_cu_q, d_cu_kv));
         if (!shape->sequences || !shape->max_q || !shape->q_tokens) return DCN_OK;
         DCN_TRY(check_pointer(ctx, "q", d_q, shape->dtype));
         DCN_TRY(check_pointer(ctx, "out", d_out, shape->dtype));
@@ -346,14 +358,17 @@ dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape
     });
 }
 
-dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_cache* cache,
+dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* given, const dcn_cache* cache,
                                    const void* d_q, const void* d_k_pages, const void* d_v_pages,
                                    const int32_t* d_cu_q, const int32_t* d_kv_lens, const int32_t* d_table,
                                    void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes,
                                    void* stream) {
     return entry(ctx, [&]() -> dcn_status {
-        REQUIRE_POINTER(shape);
+        if (!given) return null_fail(ctx, "shape");
         REQUIRE_POINTER(cache);
+        REQUIRE_SHAPE(d_cu_q || (int64_t)given->sequences * given->max_q <= given->q_tokens,
+                      "sequences * max_q exceeds q_tokens");
+        const dcn_attention_shape own = fitted(*given, true), *shape = &own;
         dcn::AttentionArgs a{};
         DCN_TRY(check_cache(ctx, cache, &a.pages));
         DCN_TRY(check_attention(ctx, shape, true, &a));
@@ -361,8 +376,6 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
                           cache->head_dim == shape->head_dim,
                       "attention and cache have different types, key heads or head sizes");
         DCN_TRY(check_out_strides(ctx, "out", shape->out_stride, shape->q_tokens, shape->q_heads, shape->head_dim));
-        REQUIRE_SHAPE(d_cu_q || (int64_t)shape->sequences * shape->max_q <= shape->q_tokens,
-                      "sequences * max_q exceeds q_tokens");
         if (!shape->sequences || !shape->max_q || !shape->q_tokens) return DCN_OK;
         DCN_TRY(check_pointer(ctx, "q", d_q, shape->dtype));
         DCN_TRY(check_pointer(ctx, "out", d_out, shape->dtype));
@@ -389,13 +402,15 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
     });
 }
 
-dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shape* shape, const void* d_q,
+dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shape* given, const void* d_q,
                                       const void* d_k, const void* d_v, const void* d_out, const float* d_lse,
                                       const void* d_dout, const int32_t* d_cu_q, const int32_t* d_cu_kv, void* d_dq,
                                       void* d_dk, void* d_dv, void* d_workspace, size_t workspace_bytes,
                                       void* stream) {
     return entry(ctx, [&]() -> dcn_status {
-        REQUIRE_POINTER(shape);
+        if (!given) return null_fail(ctx, "shape");
+        DCN_TRY(check_even(ctx, given, d_cu_q, d_cu_kv));
+        const dcn_attention_shape own = fitted(*given, false), *shape = &own;
         dcn::AttentionArgs a{};
         DCN_TRY(check_attention(ctx, shape, false, &a));
         const int dim = shape->head_dim;
@@ -404,7 +419,6 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
         DCN_TRY(check_out_strides(ctx, "dq", shape->dq_stride, shape->q_tokens, shape->q_heads, dim));
         DCN_TRY(check_out_strides(ctx, "dk", shape->dk_stride, shape->kv_tokens, shape->kv_heads, dim));
         DCN_TRY(check_out_strides(ctx, "dv", shape->dv_stride, shape->kv_tokens, shape->kv_heads, dim));
-        DCN_TRY(check_even(ctx, shape, d_cu_q, d_cu_kv));
         if (!shape->sequences) return DCN_OK;
         if (shape->q_tokens && shape->max_q) {
             DCN_TRY(check_pointer(ctx, "q", d_q, shape->dtype));

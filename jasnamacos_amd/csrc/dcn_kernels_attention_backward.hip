@@ -563,14 +563,14 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join_kernel(AttentionA
 
 KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, int frame, int back, int ahead, int sinks) {
     KeyPlan p;
-    p.blocks = (max_kv + kKeys - 1) / kKeys;
+    p.blocks = (int)(((int64_t)max_kv + kKeys - 1) / kKeys);
     const int64_t all = ((int64_t)max_q * group + 63) / 64;
     // Query tiles of a block: those of its window, or all.
     int64_t tiles = all;
     p.sink_blocks = 0;
     if (back >= 0) {
         const int64_t frames = (int64_t)back + 1 + (ahead < 0 ? 0 : ahead) + (kKeys + frame - 1) / frame;
-        const int64_t window = ahead < 0 ? all : (frames * frame * group + 63) / 64 + 1;
+        const int64_t window = ahead < 0 || frames > max_q / frame ? all : (frames * frame * group + 63) / 64 + 1;
         tiles = window < all ? window : all;
         const int64_t keys = (int64_t)sinks * frame < max_kv ? (int64_t)sinks * frame : max_kv;
         if (tiles < all) p.sink_blocks = (int)((keys + kKeys - 1) / kKeys);
