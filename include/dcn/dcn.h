@@ -770,8 +770,11 @@ dcn_status dcn_cache_append_dev(dcn_context* ctx, const dcn_cache* cache, const 
  * Softmax statistics and sums are FP32. Sequence s holds rows cu_q[s] .. cu_q[s + 1] of the
  * queries and cu_kv[s] .. cu_kv[s + 1] of the keys; null: rows s * max_q .. of max_q each
  * (keys: max_kv). max_q and max_kv are at least the longest sequence's lengths (more than
- * the rows that there are counts as those): they size
- * the launch (max_q times the heads that share a key head is below 2^31 - 256). Rows of no sequence are not written. */
+ * the rows that there are counts as those): they size the launch, which has a workgroup for
+ * each 32 to 128 rows (keys) of max_q times the heads that share a key head (of max_kv), key
+ * head and sequence, below 2^24 in all (heads of more than 128 channels: max_q and max_kv
+ * below 2^26 in the backward); a call that is larger fails before anything is launched. Rows
+ * of no sequence are not written. */
 typedef struct dcn_attention_shape {
     int32_t dtype; /* dcn_dtype */
     int32_t sequences;

@@ -53,6 +53,10 @@ struct AttentionArgs {
     int any_splits;  // launch_attention_any: workgroups that share a row block's keys
 };
 
+// A launch has fewer than 2^32 threads along x: rows or items past that go into launches of their own,
+// of this many threads each.
+constexpr int64_t kMostThreads = INT64_C(1) << 31;
+
 // Keys that `tokens` adjacent queries see at most, in tiles of `tile`.
 inline int64_t attention_keys(int max_kv, int frame, int back, int sinks, int64_t tokens, int tile) {
     const int64_t frames = (int64_t)back + 1 + sinks;

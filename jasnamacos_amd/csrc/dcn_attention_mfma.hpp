@@ -156,7 +156,7 @@ inline bool block_map(int64_t x, int64_t heads, int64_t sequences, BlockMap* m) 
     const int64_t pairs = heads * sequences, classes = pairs % 8 == 0 ? 8 : (pairs % 4 == 0 ? 4 : (pairs % 2 == 0 ? 2 : 1));
     const int64_t share = 8 / classes, each = (pairs / classes * x + share - 1) / share;
     *m = BlockMap{(int)x, (int)heads, (int)pairs, (int)classes, (unsigned)(8 * each)};
-    return 8 * each < INT32_MAX && x < INT32_MAX;
+    return x < INT32_MAX && each < (INT64_C(1) << 32) / kThreads / 8;  // fewer than 2^32 threads
 }
 // Block, key head and sequence of this workgroup; false for the padding.
 __device__ __forceinline__ bool block_of(const BlockMap& m, int* block, int* head, int* sequence) {

@@ -500,15 +500,16 @@ hipError_t by_keys(const AttentionArgs& a, hipStream_t stream) {
 
 template <typename T, int NB, bool VEC>
 hipError_t run_grad(const AttentionArgs& a, hipStream_t stream) {
-    BlockMap map;
+    BlockMap rows, keys;
+    if (!block_map(((int64_t)a.max_q * a.group + kRowsWg - 1) / kRowsWg, a.kv_heads, a.sequences, &rows) ||
+        !block_map(((int64_t)a.max_kv + kRowsWg - 1) / kRowsWg, a.kv_heads, a.sequences, &keys))
+        return hipErrorInvalidConfiguration;
     if (a.max_q > 0) {
-        if (!block_map(((int64_t)a.max_q * a.group + kRowsWg - 1) / kRowsWg, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
-        attention_any_grad_kernel<T, NB, false, VEC><<<map.grid, kThreads, 0, stream>>>(a, map);
+        attention_any_grad_kernel<T, NB, false, VEC><<<rows.grid, kThreads, 0, stream>>>(a, rows);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (a.max_kv <= 0) return hipSuccess;
-    if (!block_map(((int64_t)a.max_kv + kRowsWg - 1) / kRowsWg, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
-    attention_any_grad_kernel<T, NB, true, VEC><<<map.grid, kThreads, 0, stream>>>(a, map);
+    attention_any_grad_kernel<T, NB, true, VEC><<<keys.grid, kThreads, 0, stream>>>(a, keys);
     return hipGetLastError();
 }
 template <typename T>

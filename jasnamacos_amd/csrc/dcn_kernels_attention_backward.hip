@@ -589,17 +589,17 @@ KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, 
 
 template <typename T, int D>
 hipError_t run(const AttentionArgs& a, const KeyPlan& p, hipStream_t stream) {
-    BlockMap map;
+    BlockMap rows, keys;  // both before a launch: a call that is too large leaves everything as it was
+    if (!block_map(((int64_t)a.max_q * a.group + 127) / 128, a.kv_heads, a.sequences, &rows) ||
+        !block_map(p.items(), a.kv_heads, a.sequences, &keys))
+        return hipErrorInvalidConfiguration;
     if (a.max_q > 0) {
-        const int64_t rows = (int64_t)a.max_q * a.group;
-        if (!block_map((rows + 127) / 128, a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
-        attention_dq_kernel<T, D><<<map.grid, kThreads, 0, stream>>>(a, map);
+        attention_dq_kernel<T, D><<<rows.grid, kThreads, 0, stream>>>(a, rows);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (a.max_kv <= 0) return hipSuccess;
     float* parts = (float*)a.workspace + ((a.q_tokens * a.q_heads + 3) & ~INT64_C(3));
-    if (!block_map(p.items(), a.kv_heads, a.sequences, &map)) return hipErrorInvalidConfiguration;
-    attention_dkv_kernel<T, D><<<map.grid, kThreads, 0, stream>>>(a, map, p, parts);
+    attention_dkv_kernel<T, D><<<keys.grid, kThreads, 0, stream>>>(a, keys, p, parts);
     if (hipError_t e = hipGetLastError()) return e;
     const int joined = p.parts > 1 ? p.blocks : (p.sink_parts > 1 ? p.sink_blocks : 0);
     if (!joined) return hipSuccess;

@@ -155,6 +155,8 @@ __global__ __launch_bounds__(kWave) void attention_row_dkv_kernel(AttentionArgs 
 
 template <typename T>
 hipError_t rows_backward(const AttentionArgs& a, hipStream_t stream) {
+    constexpr int most = (int)((INT64_C(1) << 32) / kWave) - 1;  // fewer than 2^32 threads
+    if (a.max_q > most || a.max_kv > most) return hipErrorInvalidConfiguration;
     if (a.max_q > 0) {
         attention_row_dq_kernel<T><<<dim3(a.max_q, a.q_heads, a.sequences), kWave, 0, stream>>>(a);
         if (hipError_t e = hipGetLastError()) return e;

@@ -155,11 +155,11 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
 }
 
 template <typename T, int LANES, int NV, bool WIDE>
-__global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
+__global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a, int64_t first) {
     __shared__ float scratch[kThreads / 64];
     constexpr int slots = kThreads / LANES;
     const int lane = threadIdx.x % LANES, c = a.channels;
-    const int64_t row = (int64_t)blockIdx.x * slots + threadIdx.x / LANES;
+    const int64_t row = first + (int64_t)blockIdx.x * slots + threadIdx.x / LANES;
     if (row >= a.tokens) return;  // whole slots; a row of 256 lanes is the whole workgroup
     const int64_t base = row * c;
     float h[NV][kVec], sum = 0.f;
@@ -438,10 +438,13 @@ __global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormArgs a, Cut
 template <typename T, int LANES, int NV, bool WIDE>
 hipError_t run(const NormArgs& a, bool backward, hipStream_t stream) {
     if (!backward) {
-        constexpr int slots = kThreads / LANES;
-        norm_forward_kernel<T, LANES, NV, WIDE>
-            <<<(unsigned)((a.tokens + slots - 1) / slots), kThreads, 0, stream>>>(a);
-        return hipGetLastError();
+        constexpr int64_t slots = kThreads / LANES, most = kMostThreads / LANES;  // rows of a workgroup, a launch
+        for (int64_t first = 0; first < a.tokens; first += most) {
+            const int64_t rows = a.tokens - first < most ? a.tokens - first : most;
+            norm_forward_kernel<T, LANES, NV, WIDE><<<(unsigned)((rows + slots - 1) / slots), kThreads, 0, stream>>>(a, first);
+            if (hipError_t e = hipGetLastError()) return e;
+        }
+        return hipSuccess;
     }
     const Cut cut = cut_of(a.channels, a.tokens, a.gate_tokens);
     float* w_parts = a.workspace;

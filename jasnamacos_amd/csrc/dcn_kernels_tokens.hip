@@ -120,10 +120,10 @@ struct Chunk {
 
 // One thread: one chunk of one token, over the heads blockIdx.y, blockIdx.y + gridDim.y, ...
 template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs r, int64_t tokens, int heads, HeadsIn x,
-                                                          HeadsOut out) {
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs r, int64_t first, int64_t tokens, int heads,
+                                                          HeadsIn x, HeadsOut out) {
     const int chunks = Chunk<T, N>::count(r);
-    const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t item = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int64_t token = item / chunks;
     if (token >= tokens) return;
     Chunk<T, N> c;
@@ -138,9 +138,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs r, int64_t 
 
 // One thread: one chunk of one new token; heads as above, q's, then k's, then v's.
 template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void append_kernel(RotaryArgs r, AppendArgs a) {
+__global__ __launch_bounds__(kThreads) void append_kernel(RotaryArgs r, AppendArgs a, int64_t first) {
     const int chunks = Chunk<T, N>::count(r);
-    const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t item = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int64_t token = item / chunks;
     if (token >= a.tokens) return;
     // The sequence: the last one that starts at or before the token.
@@ -192,19 +192,30 @@ bool divides(const RotaryArgs& r, int n) {
     return r.dim % n == 0 && (r.interleaved ? 2 * r.pairs : r.pairs) % n == 0;
 }
 
-// Heads a launch spreads over grid.y: as many as give the card about 2,048 waves a slice.
+// Heads a launch spreads over grid.y (65,535 at most): as many as give the card about 2,048 waves a slice.
 unsigned head_slices(int64_t items, int heads) {
-    const int64_t want = (131072 + items - 1) / items;
-    return (unsigned)(want < 1 ? 1 : (want > heads ? heads : want));
+    const int64_t want = (131072 + items - 1) / items, most = heads < 65535 ? heads : 65535;
+    return (unsigned)(want < 1 ? 1 : (want > most ? most : want));
+}
+
+// launch(first, grid) over all items.
+template <typename F>
+hipError_t in_launches(int64_t items, int heads, F launch) {
+    for (int64_t first = 0; first < items; first += kMostThreads) {
+        const int64_t n = items - first < kMostThreads ? items - first : kMostThreads;
+        launch(first, dim3((unsigned)((n + kThreads - 1) / kThreads), head_slices(items, heads)));
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
 }
 
 template <typename T, int N>
 hipError_t rotary(int64_t tokens, int heads, const HeadsIn& x, const HeadsOut& out, const RotaryArgs& r,
                   hipStream_t stream) {
     const int64_t items = tokens * Chunk<T, N>::count(r);
-    const dim3 grid((unsigned)((items + kThreads - 1) / kThreads), head_slices(items, heads));
-    rotary_kernel<T, N><<<grid, kThreads, 0, stream>>>(r, tokens, heads, x, out);
-    return hipGetLastError();
+    return in_launches(items, heads, [&](int64_t first, dim3 grid) {
+        rotary_kernel<T, N><<<grid, kThreads, 0, stream>>>(r, first, tokens, heads, x, out);
+    });
 }
 
 template <typename T>
@@ -220,9 +231,9 @@ template <typename T, int N>
 hipError_t append(const AppendArgs& a, const RotaryArgs& r, hipStream_t stream) {
     const int64_t items = a.tokens * Chunk<T, N>::count(r);
     const int heads = (a.q.p ? a.q_heads : 0) + 2 * a.kv_heads;
-    const dim3 grid((unsigned)((items + kThreads - 1) / kThreads), head_slices(items, heads));
-    append_kernel<T, N><<<grid, kThreads, 0, stream>>>(r, a);
-    return hipGetLastError();
+    return in_launches(items, heads, [&](int64_t first, dim3 grid) {
+        append_kernel<T, N><<<grid, kThreads, 0, stream>>>(r, a, first);
+    });
 }
 
 template <typename T>
