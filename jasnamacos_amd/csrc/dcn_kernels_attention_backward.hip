@@ -228,6 +228,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionArgs
 struct KeyPlan {
     int blocks, sink_blocks, parts, sink_parts;
     __host__ __device__ int items() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * parts; }
+    // Items whose sums the workspace holds, the first ones: those of blocks that are cut.
+    __host__ __device__ int kept() const { return parts > 1 ? items() : (sink_parts > 1 ? sink_blocks * sink_parts : 0); }
     __host__ __device__ void item(int i, int* block, int* part, int* of) const {
         if (i < sink_blocks * sink_parts) {
             *block = i / sink_parts;
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attention_dkv_kerne
     const float fk = up == 0.f ? 0.f : a.scale / up, fv = kScaled<T> ? 1.f / kWeightLift : 1.f;
     if (of > 1) {
         // [item][dk, dv][key][D] FP32, in order of the parts
-        const int64_t item = ((int64_t)pl.seq * a.kv_heads + pl.kh) * plan.items() + at;
+        const int64_t item = ((int64_t)pl.seq * a.kv_heads + pl.kh) * plan.kept() + at;
         float* to = parts + ((item * 2) * kKeys + 32 * wave + (lane & 31)) * D + 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join_kernel(AttentionA
     const int of = block < plan.sink_blocks ? plan.sink_parts : plan.parts;
     const int first = block < plan.sink_blocks ? block * plan.sink_parts
                                                : plan.sink_blocks * plan.sink_parts + (block - plan.sink_blocks) * plan.parts;
-    const int64_t item = ((int64_t)blockIdx.z * a.kv_heads + blockIdx.y) * plan.items() + first;
+    const int64_t item = ((int64_t)blockIdx.z * a.kv_heads + blockIdx.y) * plan.kept() + first;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -569,7 +571,7 @@ KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, 
     int64_t tiles = all;
     p.sink_blocks = 0;
     if (back >= 0) {
-        const int64_t frames = (int64_t)back + 1 + (ahead < 0 ? 0 : ahead) + (kKeys + frame - 1) / frame;
+        const int64_t frames = (int64_t)back + 1 + (ahead < 0 ? 0 : ahead) + ((int64_t)kKeys + frame - 1) / frame;
         const int64_t window = ahead < 0 || frames > max_q / frame ? all : (frames * frame * group + 63) / 64 + 1;
         tiles = window < all ? window : all;
         const int64_t keys = (int64_t)sinks * frame < max_kv ? (int64_t)sinks * frame : max_kv;
@@ -580,10 +582,17 @@ KeyPlan key_plan(int sequences, int kv_heads, int group, int max_q, int max_kv, 
     int64_t parts = groups > 0 ? 256 / groups : 1;
     if (parts > tiles / 8) parts = tiles / 8;
     p.parts = (int)(parts < 1 ? 1 : parts);
-    // A sink block's parts are about as long as another block's.
-    const int64_t each = (tiles + p.parts - 1) / p.parts;
-    const int64_t sink_parts = each > 0 ? (all + each - 1) / each : 1;
-    p.sink_parts = p.sink_blocks ? (int)(sink_parts < p.parts ? p.parts : (sink_parts > 256 ? 256 : sink_parts)) : p.parts;
+    // A sink block's parts are about as long as another block's, where four workgroups a CU do not share
+    // its work anyhow: each part is 2 x 128 rows of the workspace, written and read again (BF16, a window of
+    // 16 tokens, 4,096 sinks: 4 x 8,192 tokens, 8 heads of 64, 1,762 us and 2.2 GB without that limit, 983 us and
+    // 1 MB with it; 1 x 65,536: 4,159 and 2,163 us).
+    p.sink_parts = p.parts;
+    if (p.sink_blocks) {
+        const int64_t each = (tiles + p.parts - 1) / p.parts, most = 1024 / ((int64_t)p.sink_blocks * kv_heads * sequences);
+        const int64_t wanted = each > 0 ? (all + each - 1) / each : 1;
+        const int64_t sink_parts = wanted < most ? wanted : most;
+        p.sink_parts = (int)(sink_parts < p.parts ? p.parts : (sink_parts > 256 ? 256 : sink_parts));
+    }
     return p;
 }
 
@@ -619,8 +628,7 @@ size_t attention_backward_workspace(const dcn_attention_shape& s) {
     const fa::KeyPlan p = fa::key_plan(s.sequences, s.kv_heads, s.q_heads / s.kv_heads, s.max_q, s.max_kv, s.frame_tokens, s.back,
                                        s.ahead, s.sinks);
     size_t n = ((size_t)s.q_tokens * s.q_heads + 3) & ~(size_t)3;
-    if (p.parts > 1 || p.sink_parts > 1)
-        n += (size_t)s.sequences * s.kv_heads * p.items() * 2 * fa::kKeys * s.head_dim;
+    n += (size_t)s.sequences * s.kv_heads * p.kept() * 2 * fa::kKeys * s.head_dim;
     return n * sizeof(float);
 }
 

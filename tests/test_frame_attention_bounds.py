@@ -36,3 +36,15 @@ def test_forward(dtype):
 def test_windows_past_the_rows():
     """A window longer than the queries is no window."""
     assert workspace(fa.PASS_BACKWARD, back=MOST, ahead=MOST, frame=65536) == workspace(fa.PASS_BACKWARD, ahead=-1)
+
+
+@pytest.mark.parametrize("shape", [
+    dict(sequences=64, q_heads=32, kv_heads=8, dim=128, back=100, sinks=2000, max_q=2000, max_kv=2000),
+    dict(sequences=4, q_heads=8, kv_heads=8, back=16, sinks=4096, max_q=8192, max_kv=8192),
+    dict(q_heads=8, kv_heads=8, back=16, sinks=4096, max_q=65536, max_kv=65536),
+    dict(q_heads=2, kv_heads=1, frame=2**31 - 1, back=0, sinks=1, max_q=300, max_kv=300)])
+def test_many_sinks(shape):
+    """The parts of the sinks' gradients: four workgroups a CU of 2 x 128 FP32 rows at most."""
+    tokens = shape.get("sequences", 1) * shape["max_q"]
+    rows = (tokens * shape["q_heads"] + 3) // 4 * 4
+    assert workspace(fa.PASS_BACKWARD, **shape, q_tokens=tokens, kv_tokens=tokens) <= 4 * (rows + 1024 * 2 * 128 * shape.get("dim", 64))
