@@ -44,21 +44,23 @@ def _need(condition, message: str) -> None:
         raise DeformConvError(INVALID_SHAPE, message)
 
 
-def _on_device(name: str, t) -> None:
+def _on_device(name: str, t, device: int) -> None:
     if t is None:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
     if not t.is_cuda:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is not on a device")
+    if t.get_device() != device:
+        raise DeformConvError(INVALID_ARGUMENT, f"{name} is on device {t.get_device()}; the context is on {device}")
 
 
-def _heads(name: str, t, dtype, shape) -> tuple:
+def _heads(name: str, t, dtype, shape, device: int) -> tuple:
     """The strides of a tensor of heads of this shape."""
-    if t is not None and t.shape == shape and t.dtype is dtype and t.is_cuda:
+    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device:
         strides = t.stride()
         if strides[2] == 1 or shape[2] == 1:
             return strides
         raise DeformConvError(INVALID_SHAPE, f"{name} channels are not adjacent")
-    _on_device(name, t)
+    _on_device(name, t, device)
     if t.dtype is not dtype:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
     raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}")
@@ -73,21 +75,21 @@ def _rows(name: str, t) -> int:
     return t.shape[0]
 
 
-def _whole(name: str, t, dtype, shape) -> None:
+def _whole(name: str, t, dtype, shape, device: int) -> None:
     """An adjacent tensor of this type and shape."""
-    if t is not None and t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.is_cuda:
+    if t is not None and t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.get_device() == device:
         return
-    _on_device(name, t)
+    _on_device(name, t, device)
     if t.dtype is not dtype:
         raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected {dtype}")
     raise DeformConvError(INVALID_SHAPE, f"{name} is {tuple(t.shape)}; expected {shape}, adjacent")
 
 
-def _index(name: str, t, count) -> None:
+def _index(name: str, t, count, device: int) -> None:
     """An adjacent int32 array of this length."""
-    if t is not None and t.dtype is torch.int32 and t.shape == (count,) and t.is_contiguous() and t.is_cuda:
+    if t is not None and t.dtype is torch.int32 and t.shape == (count,) and t.is_contiguous() and t.get_device() == device:
         return
-    _on_device(name, t)
+    _on_device(name, t, device)
     raise DeformConvError(INVALID_SHAPE, f"{name} is not {count} adjacent int32 values")
 
 
@@ -174,18 +176,19 @@ class Rotary(_Handle):
         parts = [base ** (-torch.arange(n, dtype=torch.float64) / max(1, n)) for n in self.pairs]
         return torch.cat(parts).float().to(device)
 
-    def _check(self, positions, freq, tokens) -> None:
-        _whole("positions", positions, torch.int32, (tokens, 3))
-        _whole("freq", freq, torch.float32, self._freq_shape)
+    def _check(self, positions, freq, tokens, device) -> None:
+        _whole("positions", positions, torch.int32, (tokens, 3), device)
+        _whole("freq", freq, torch.float32, self._freq_shape, device)
 
     def run_dev(self, x, positions, freq, out, inverse: bool = False, stream=None) -> None:
         """out = x turned by positions ([tokens][3] int32) times freq; inverse: the gradient."""
         tokens, dtype = _rows("x", x), x.dtype
         heads = x.shape[1]
         shape = (tokens, heads, self.head_dim)
-        xt, xh, _ = _heads("x", x, dtype, shape)
-        ot, oh, _ = _heads("out", out, dtype, shape)
-        self._check(positions, freq, tokens)
+        device = self.ctx.device
+        xt, xh, _ = _heads("x", x, dtype, shape, device)
+        ot, oh, _ = _heads("out", out, dtype, shape, device)
+        self._check(positions, freq, tokens, device)
         _dtype(x)
         status = self._lib.dcn_rotary_dev(
             self._ctx, self._c[dtype], tokens, heads, x.data_ptr(), xt, xh, positions.data_ptr(), freq.data_ptr(),
@@ -194,7 +197,7 @@ class Rotary(_Handle):
             self.ctx._check(status)
 
 
-def _cache(k_pages, v_pages, table) -> bytes:
+def _cache(k_pages, v_pages, table, device: int) -> bytes:
     """The packed dcn_cache."""
     if k_pages is None or table is None:
         raise DeformConvError(INVALID_ARGUMENT, "k_pages or table is missing")
@@ -202,9 +205,9 @@ def _cache(k_pages, v_pages, table) -> bytes:
         raise DeformConvError(INVALID_SHAPE, "pages are [pages][page_tokens][heads][channels], the table "
                                              "[sequences][width]")
     shape, dtype = k_pages.shape, k_pages.dtype
-    _whole("k_pages", k_pages, dtype, shape)
-    _whole("v_pages", v_pages, dtype, shape)
-    _whole("table", table, torch.int32, table.shape)
+    _whole("k_pages", k_pages, dtype, shape, device)
+    _whole("v_pages", v_pages, dtype, shape, device)
+    _whole("table", table, torch.int32, table.shape, device)
     pages, page_tokens, heads, dim = shape
     try:
         return _CACHE.pack(pages, page_tokens, table.shape[1], heads, dim, _dtype(k_pages))
@@ -220,23 +223,24 @@ class CacheAppend(_Handle):
         """k, v: the new tokens of all sequences, sequence s in rows cu_q[s] .. cu_q[s + 1], the
         last of its kv_lens[s] tokens. Keys are turned by `rotary` on the way, and so is q into
         q_out where it is given."""
-        cache = _cache(k_pages, v_pages, table)
+        device = self.ctx.device
+        cache = _cache(k_pages, v_pages, table, device)
         tokens, sequences, dtype = _rows("k", k), table.shape[0], k_pages.dtype
         _, _, kv_heads, dim = k_pages.shape
         shape = (tokens, kv_heads, dim)
-        ks, vs = _heads("k", k, dtype, shape), _heads("v", v, dtype, shape)
-        _index("cu_q", cu_q, sequences + 1)
-        _index("kv_lens", kv_lens, sequences)
+        ks, vs = _heads("k", k, dtype, shape, device), _heads("v", v, dtype, shape, device)
+        _index("cu_q", cu_q, sequences + 1, device)
+        _index("kv_lens", kv_lens, sequences, device)
         q_heads, qs, os = 0, _NO_STRIDES, _NO_STRIDES
         if q is not None:
             _rows("q", q)
             q_heads = q.shape[1]
             shape = (tokens, q_heads, dim)
             _rows("q_out", q_out)
-            qs, os = _heads("q", q, dtype, shape), _heads("q_out", q_out, dtype, shape)
+            qs, os = _heads("q", q, dtype, shape, device), _heads("q_out", q_out, dtype, shape, device)
         r = None
         if rotary is not None:
-            rotary._check(positions, freq, tokens)
+            rotary._check(positions, freq, tokens, device)
             r = rotary._c[dtype]
         try:
             s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
@@ -287,9 +291,9 @@ class FrameAttention(_Handle):
         else:
             sequences = q_tokens // max_q if max_q else (kv_tokens // max_kv if max_kv else 0)
         if cu_q is not None:
-            _index("cu_q", cu_q, sequences + 1)
+            _index("cu_q", cu_q, sequences + 1, self.ctx.device)
         if cu_kv is not None:
-            _index("cu_kv", cu_kv, sequences + 1)
+            _index("cu_kv", cu_kv, sequences + 1, self.ctx.device)
         return sequences, max_q, max_kv
 
     def _forward_parts(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv):
@@ -297,10 +301,11 @@ class FrameAttention(_Handle):
         q_tokens, kv_tokens, dtype = _rows("q", q), _rows("k", k), q.dtype
         runs = self._runs(q_tokens, kv_tokens, cu_q, cu_kv, max_q, max_kv)
         q_shape, k_shape = (q_tokens, self.q_heads, self.head_dim), (kv_tokens, self.kv_heads, self.head_dim)
-        strides = (_heads("q", q, dtype, q_shape), _heads("k", k, dtype, k_shape), _heads("v", v, dtype, k_shape),
-                   _heads("out", out, dtype, q_shape))
+        device = self.ctx.device
+        strides = (_heads("q", q, dtype, q_shape, device), _heads("k", k, dtype, k_shape, device),
+                   _heads("v", v, dtype, k_shape, device), _heads("out", out, dtype, q_shape, device))
         if lse is not None:
-            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads))
+            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads), device)
         return (q, *runs, q_tokens, kv_tokens, *strides)
 
     def _forward_shape(self, q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv) -> _lib.DcnAttentionShape:
@@ -329,9 +334,9 @@ class FrameAttention(_Handle):
         parts = self._forward_parts(q, k, v, out, lse, cu_q, cu_kv, max_q, max_kv)
         if lse is None:
             raise DeformConvError(INVALID_ARGUMENT, "lse is missing")
-        dtype, q_shape, k_shape = q.dtype, q.shape, k.shape
-        s = self._pack(*parts, _heads("dout", dout, dtype, q_shape), _heads("dq", dq, dtype, q_shape),
-                       _heads("dk", dk, dtype, k_shape), _heads("dv", dv, dtype, k_shape))
+        dtype, q_shape, k_shape, device = q.dtype, q.shape, k.shape, self.ctx.device
+        s = self._pack(*parts, _heads("dout", dout, dtype, q_shape, device), _heads("dq", dq, dtype, q_shape, device),
+                       _heads("dk", dk, dtype, k_shape, device), _heads("dv", dv, dtype, k_shape, device))
         w, size = self._workspace_of(s, PASS_BACKWARD, q)
         self.ctx._check(self._lib.dcn_attention_backward_dev(
             self.ctx.ctx, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
@@ -343,20 +348,21 @@ class FrameAttention(_Handle):
         """forward_dev over a paged cache: sequence s has kv_lens[s] keys, its queries being the
         last tokens (one, or a frame's). cu_q None: max_q queries each. max_kv bounds kv_lens
         (default: the table's width)."""
-        cache = _cache(k_pages, v_pages, table)
+        device = self.ctx.device
+        cache = _cache(k_pages, v_pages, table, device)
         sequences, q_tokens, dtype = table.shape[0], _rows("q", q), k_pages.dtype
         if cu_q is not None:
-            _index("cu_q", cu_q, sequences + 1)
-        _index("kv_lens", kv_lens, sequences)
+            _index("cu_q", cu_q, sequences + 1, device)
+        _index("kv_lens", kv_lens, sequences, device)
         if max_q is None:
             max_q = q_tokens if cu_q is not None else (q_tokens // sequences if sequences else 0)
         if max_kv is None:
             max_kv = table.shape[1] * k_pages.shape[1]
         shape = (q_tokens, self.q_heads, self.head_dim)
         if lse is not None:
-            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads))
-        s = self._pack(q, sequences, int(max_q), int(max_kv), q_tokens, 0, _heads("q", q, dtype, shape), _NO_STRIDES,
-                       _NO_STRIDES, _heads("out", out, dtype, shape))
+            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads), device)
+        s = self._pack(q, sequences, int(max_q), int(max_kv), q_tokens, 0, _heads("q", q, dtype, shape, device), _NO_STRIDES,
+                       _NO_STRIDES, _heads("out", out, dtype, shape, device))
         w, size = self._workspace_of(s, PASS_PAGED, q)
         status = self._lib.dcn_attention_paged_dev(
             self._ctx, s, cache, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q), kv_lens.data_ptr(),
@@ -392,13 +398,13 @@ class GatedNorm(_Handle):
         for name, t in needed:
             if t is None:
                 raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
-        tokens, dtype, channels = x.shape[0], x.dtype, self.channels
+        tokens, dtype, channels, device = x.shape[0], x.dtype, self.channels, self.ctx.device
         for shape, kind, group in (((tokens, channels), dtype, needed), ((tokens, channels), dtype, tensors),
                                    ((-(-tokens // self.gate_tokens), channels), dtype, gates),
                                    ((channels,), dtype, vectors), ((channels,), torch.float32, sums)):
             for name, t in group:
-                if t is not None and not (t.shape == shape and t.dtype is kind and t.is_contiguous() and t.is_cuda):
-                    _whole(name, t, kind, shape)
+                if t is not None and not (t.shape == shape and t.dtype is kind and t.is_contiguous() and t.get_device() == device):
+                    _whole(name, t, kind, shape, device)
 
     def low_bytes(self, x) -> int:
         """Bytes of forward_dev's `low` for a residual stream like x."""
@@ -411,7 +417,7 @@ class GatedNorm(_Handle):
         count = self._lib.dcn_gated_norm_low_bytes(s)
         if not count:
             return None
-        _on_device("low", low)
+        _on_device("low", low, self.ctx.device)
         if low.dtype != torch.uint8 or low.numel() < count or not low.is_contiguous():
             raise DeformConvError(INVALID_SHAPE, f"low is not {count} adjacent uint8 values")
         return low.data_ptr()
@@ -450,7 +456,7 @@ class GatedNorm(_Handle):
         self._check_all(x, (("h", h), ("x", x), ("x_out", x_out)), (("y", y),), (("gate", gate),),
                         (("w_post", w_post), ("w_pre", w_pre)))
         if rstd is not None:
-            _whole("rstd", rstd, torch.float32, (x.shape[0], 2))
+            _whole("rstd", rstd, torch.float32, (x.shape[0], 2), self.ctx.device)
         status = self._lib.dcn_gated_norm_forward_dev(
             self._ctx, s, h.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre), x_out.data_ptr(), _ptr(y),
             _ptr(rstd), None if rstd is None else self._low_to_write(s, low, x, rstd), stream and _stream(stream))
@@ -467,7 +473,7 @@ class GatedNorm(_Handle):
         self._check_all(x_out, (("h", h), ("x_out", x_out), ("dx_out", dx_out), ("dh", dh), ("dx", dx)),
                         (("dy", dy),), (("gate", gate), ("dgate", dgate)), (("w_post", w_post), ("w_pre", w_pre)),
                         (("dw_post", dw_post), ("dw_pre", dw_pre)))
-        _whole("rstd", rstd, torch.float32, (x_out.shape[0], 2))
+        _whole("rstd", rstd, torch.float32, (x_out.shape[0], 2), self.ctx.device)
         w, size = self._room(s, lambda: self._lib.dcn_gated_norm_workspace_bytes(s), x_out)
         self.ctx._check(self._lib.dcn_gated_norm_backward_dev(
             self.ctx.ctx, s, h.data_ptr(), x_out.data_ptr(), _ptr(gate), _ptr(w_post), _ptr(w_pre),
