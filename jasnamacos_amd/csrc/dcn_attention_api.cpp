@@ -46,6 +46,11 @@ dcn_status check_pointer(dcn_context* ctx, const char* name, const void* p, int 
     return DCN_OK;
 }
 
+// One that may be null.
+dcn_status check_optional(dcn_context* ctx, const char* name, const void* p, int dtype) {
+    return p ? check_pointer(ctx, name, p, dtype) : DCN_OK;
+}
+
 constexpr int kMaxHeads = 65535;        // grid.y
 constexpr int kMaxSequences = 65535;    // grid.z
 constexpr int64_t kMaxStride = INT64_C(1) << 40;
@@ -342,6 +347,9 @@ dcn_status dcn_attention_forward_dev(dcn_context* ctx, const dcn_attention_shape
             DCN_TRY(check_pointer(ctx, "k", d_k, shape->dtype));
             DCN_TRY(check_pointer(ctx, "v", d_v, shape->dtype));
         }
+        DCN_TRY(check_optional(ctx, "lse", d_lse, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "cu_q", d_cu_q, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "cu_kv", d_cu_kv, DCN_DTYPE_F32));
         DCN_TRY(check_workspace(ctx, d_workspace, workspace_bytes, attention_workspace(shape, DCN_ATTENTION_FORWARD)));
         a.q.p = d_q;
         a.k.p = d_k;
@@ -383,6 +391,8 @@ dcn_status dcn_attention_paged_dev(dcn_context* ctx, const dcn_attention_shape* 
         DCN_TRY(check_pointer(ctx, "v_pages", d_v_pages, shape->dtype));
         DCN_TRY(check_pointer(ctx, "kv_lens", d_kv_lens, DCN_DTYPE_F32));
         DCN_TRY(check_pointer(ctx, "table", d_table, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "lse", d_lse, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "cu_q", d_cu_q, DCN_DTYPE_F32));
         DCN_TRY(check_workspace(ctx, d_workspace, workspace_bytes, attention_workspace(shape, DCN_ATTENTION_PAGED)));
         const int64_t ts = (int64_t)cache->kv_heads * cache->head_dim;
         a.q.p = d_q;
@@ -433,6 +443,8 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
             DCN_TRY(check_pointer(ctx, "dk", d_dk, shape->dtype));
             DCN_TRY(check_pointer(ctx, "dv", d_dv, shape->dtype));
         }
+        DCN_TRY(check_optional(ctx, "cu_q", d_cu_q, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "cu_kv", d_cu_kv, DCN_DTYPE_F32));
         DCN_TRY(check_workspace(ctx, d_workspace, workspace_bytes, attention_workspace(shape, DCN_ATTENTION_BACKWARD)));
         a.q.p = d_q;
         a.k.p = d_k;
@@ -468,6 +480,11 @@ dcn_status dcn_gated_norm_forward_dev(dcn_context* ctx, const dcn_norm_shape* sh
         DCN_TRY(check_pointer(ctx, "h", d_h, shape->dtype));
         DCN_TRY(check_pointer(ctx, "x", d_x, shape->dtype));
         DCN_TRY(check_pointer(ctx, "x_out", d_x_out, shape->dtype));
+        DCN_TRY(check_optional(ctx, "gate", d_gate, shape->dtype));
+        DCN_TRY(check_optional(ctx, "w_post", d_w_post, shape->dtype));
+        DCN_TRY(check_optional(ctx, "w_pre", d_w_pre, shape->dtype));
+        DCN_TRY(check_optional(ctx, "y", d_y, shape->dtype));
+        DCN_TRY(check_optional(ctx, "rstd", d_rstd, DCN_DTYPE_F32));
         a.h = d_h;
         a.x = d_x;
         a.gate = d_gate;
@@ -523,6 +540,13 @@ dcn_status dcn_gated_norm_backward_dev(dcn_context* ctx, const dcn_norm_shape* s
             DCN_TRY(check_pointer(ctx, "dh", d_dh, shape->dtype));
             DCN_TRY(check_pointer(ctx, "dx", d_dx, shape->dtype));
         }
+        DCN_TRY(check_optional(ctx, "gate", d_gate, shape->dtype));
+        DCN_TRY(check_optional(ctx, "w_post", d_w_post, shape->dtype));
+        DCN_TRY(check_optional(ctx, "w_pre", d_w_pre, shape->dtype));
+        DCN_TRY(check_optional(ctx, "dy", d_dy, shape->dtype));
+        DCN_TRY(check_optional(ctx, "dgate", d_dgate, shape->dtype));
+        DCN_TRY(check_optional(ctx, "dw_post", d_dw_post, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "dw_pre", d_dw_pre, DCN_DTYPE_F32));
         a.h = d_h;
         a.x_out = const_cast<void*>(d_x_out);
         a.gate = d_gate;
