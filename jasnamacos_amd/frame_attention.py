@@ -284,10 +284,10 @@ class FrameAttention(_Handle):
         rows in equal runs of max_q and max_kv."""
         max_q = q_tokens if max_q is None else int(max_q)
         max_kv = kv_tokens if max_kv is None else int(max_kv)
-        if cu_q is not None:
-            sequences = cu_q.shape[0] - 1
-        elif cu_kv is not None:
-            sequences = cu_kv.shape[0] - 1
+        starts = cu_kv if cu_q is None else cu_q
+        if starts is not None:
+            _need(starts.dim() == 1, f"an index array has {starts.dim()} dimensions; expected one")
+            sequences = starts.shape[0] - 1
         else:
             sequences = q_tokens // max_q if max_q else (kv_tokens // max_kv if max_kv else 0)
         if cu_q is not None:
