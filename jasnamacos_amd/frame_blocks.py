@@ -93,6 +93,15 @@ class _Norm(torch.autograd.Function):
         return dh, dx, dgate, dw_post.to(w_post.dtype), dw_pre.to(w_pre.dtype), None
 
 
+def _normed(norm, h, x, gate, w_post, w_pre):
+    """(x_out, y); what a backward reads is made only where gradients are on."""
+    if torch.is_grad_enabled():
+        return _Norm.apply(h, x, gate, w_post, w_pre, norm)
+    x_out, y = torch.empty_like(x), torch.empty_like(x)
+    norm.forward_dev(h, x, gate, w_post, w_pre, x_out, y, stream=torch.cuda.current_stream())
+    return x_out, y
+
+
 class FrameBlocks:
     """`layers` blocks of `channels` channels over frames of rows x columns tokens; a token sees
     its own frame, the `back` frames before it and the first `sinks` ones.
@@ -150,7 +159,7 @@ class FrameBlocks:
     def _start(self, x, norm):
         """The first block's input: the norm of x, a closed gate before it."""
         closed = torch.zeros(len(x) // self.frame_tokens, self.channels, dtype=x.dtype, device=x.device)
-        return _Norm.apply(x, x, closed, self.first, self.first, norm)
+        return _normed(norm, x, x, closed, self.first, self.first)
 
     def clip(self, x, style, clips: int = 1):
         """x: [clips * frames * rows * columns][channels]; style: [clips * frames][channels], which
@@ -161,7 +170,7 @@ class FrameBlocks:
         x, y = self._start(x, norm)
         for w in self.layers:
             h = _Attend.apply(y @ w["qkv"], self, positions, longest) @ w["back"]
-            x, y = _Norm.apply(h, x, style @ w["gate"], w["w_post"], w["w_pre"], norm)
+            x, y = _normed(norm, h, x, style @ w["gate"], w["w_post"], w["w_pre"])
         return y
 
     def stream(self, streams: int, frames: int, page_tokens: int = 16) -> "FrameStream":
@@ -212,7 +221,7 @@ class FrameStream:
                              q, turned, stream=stream)
             self.attention.paged_dev(turned, k_pages, v_pages, self.table, self.cu_q, self.lens, out, max_q=n,
                                      max_kv=self.time * n, stream=stream)
-            x, y = _Norm.apply(out.flatten(1) @ w["back"], x, style @ w["gate"], w["w_post"], w["w_pre"], self.norm)
+            x, y = _normed(self.norm, out.flatten(1) @ w["back"], x, style @ w["gate"], w["w_post"], w["w_pre"])
         self.positions[:, 0] += 1
         return y
 

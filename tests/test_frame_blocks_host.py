@@ -1,5 +1,5 @@
-"""The example's blocks without a device: which handles they use, and that they refuse second
-derivatives. The operators' calls are recorded, not run."""
+"""The example's blocks without a device: which handles they use, what serving leaves out, and that
+second derivatives are refused. The operators' calls are recorded, not run."""
 from __future__ import annotations
 
 import types
@@ -62,3 +62,20 @@ def test_second_derivatives_are_refused(blocks):
     grads = torch.autograd.grad(y.sum(), net.parameters(), create_graph=True, allow_unused=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         sum(g.square().sum() for g in grads if g is not None).backward()
+
+
+def test_serving_keeps_nothing_for_a_backward(blocks, monkeypatch):
+    """Norms write their statistics and rounded-off halves where gradients are on."""
+    net, _, _ = blocks
+    kept = []
+
+    def forward_dev(self, h, x, gate, w_post, w_pre, x_out, y=None, rstd=None, low=None, stream=None):
+        kept.append(rstd is not None)
+    monkeypatch.setattr(fa.GatedNorm, "forward_dev", forward_dev)
+    x, style = torch.randn(18, 48), torch.randn(3, 48)
+    net.stream(1, 4, 2).step(x[:6], style[:1])
+    with torch.no_grad():
+        net.clip(x, style)
+    assert kept == [False] * 6
+    net.clip(x, style)
+    assert kept[6:] == [True] * 3
