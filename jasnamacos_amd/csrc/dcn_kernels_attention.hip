@@ -96,8 +96,9 @@ struct RowState {
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[mb][r]);
         top = both_max(top) * c;
-        if (__builtin_expect(__any(top > m + kSlack), 0)) {
-            const float next = fmaxf(m, top);
+        const bool raise = top > m + kSlack;
+        if (__builtin_expect(__any(raise), 0)) {
+            const float next = raise ? top : m;  // the other rows stay: no row's bits go by its neighbours'
             const float old = exp2f(m - (next == -INFINITY ? 0.f : next));
             m = next;
             l *= old;

@@ -131,8 +131,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NB <= 4 ? 2 : 1) void att
 #pragma unroll
         for (int x = 1; x < 16; ++x) top = fmaxf(top, s[x]);
         top = both_max(top);
-        if (__any(top > m + kSlack)) {
-            const float next = fmaxf(m, top), old = exp2f(m - (next == -INFINITY ? 0.f : next));
+        const bool raise = top > m + kSlack;
+        if (__any(raise)) {
+            const float next = raise ? top : m, old = exp2f(m - (next == -INFINITY ? 0.f : next));
             m = next;
             l *= old;
 #pragma unroll
