@@ -286,7 +286,8 @@ class FrameAttention(_Handle):
         max_kv = kv_tokens if max_kv is None else int(max_kv)
         starts = cu_kv if cu_q is None else cu_q
         if starts is not None:
-            _need(starts.dim() == 1, f"an index array has {starts.dim()} dimensions; expected one")
+            if starts.dim() != 1:
+                raise DeformConvError(INVALID_SHAPE, f"an index array has {starts.dim()} dimensions; expected one")
             sequences = starts.shape[0] - 1
         else:
             sequences = q_tokens // max_q if max_q else (kv_tokens // max_kv if max_kv else 0)
