@@ -43,7 +43,7 @@ class _Attend(torch.autograd.Function):
         tq, tk = turned.split((q.shape[1], k.shape[1]), 1)
         out = torch.empty_like(tq, memory_format=torch.contiguous_format)
         lse = torch.empty(len(qkv), q.shape[1], dtype=torch.float32, device=qkv.device)
-        stream = torch.cuda.current_stream()
+        stream = torch.cuda.current_stream(qkv.device)
         blocks.rotary.run_dev(q, positions, blocks.freq, tq, stream=stream)
         blocks.rotary.run_dev(k, positions, blocks.freq, tk, stream=stream)
         blocks.attention.forward_dev(tq, tk, v, out, lse, max_q=longest, max_kv=longest, stream=stream)
@@ -55,7 +55,7 @@ class _Attend(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         qkv, turned, out, lse, positions = ctx.saved_tensors
-        blocks, stream = ctx.blocks, torch.cuda.current_stream()
+        blocks, stream = ctx.blocks, torch.cuda.current_stream(qkv.device)
         _, _, v = blocks.heads(qkv)
         dqkv, dturned = torch.empty_like(qkv), torch.empty_like(turned)
         dq, dk, dv = blocks.heads(dqkv)
@@ -76,7 +76,7 @@ class _Norm(torch.autograd.Function):
         x_out, y = torch.empty_like(x), torch.empty_like(x)
         rstd = torch.empty(len(x), 2, dtype=torch.float32, device=x.device)
         low = torch.empty(norm.low_bytes(x), dtype=torch.uint8, device=x.device)
-        norm.forward_dev(h, x, gate, w_post, w_pre, x_out, y, rstd, low, stream=torch.cuda.current_stream())
+        norm.forward_dev(h, x, gate, w_post, w_pre, x_out, y, rstd, low, stream=torch.cuda.current_stream(x.device))
         ctx.save_for_backward(h, x_out, gate, w_post, w_pre, rstd, low)
         ctx.norm = norm
         return x_out, y
@@ -89,7 +89,7 @@ class _Norm(torch.autograd.Function):
         dw_post = torch.empty(len(w_post), dtype=torch.float32, device=h.device)
         dw_pre = torch.empty_like(dw_post)
         ctx.norm.backward_dev(h, x_out, gate, w_post, w_pre, rstd, dx_out.contiguous(), dy.contiguous(), dh, dx, dgate,
-                              dw_post, dw_pre, low, stream=torch.cuda.current_stream())
+                              dw_post, dw_pre, low, stream=torch.cuda.current_stream(h.device))
         return dh, dx, dgate, dw_post.to(w_post.dtype), dw_pre.to(w_pre.dtype), None
 
 
@@ -98,7 +98,7 @@ def _normed(norm, h, x, gate, w_post, w_pre):
     if torch.is_grad_enabled():
         return _Norm.apply(h, x, gate, w_post, w_pre, norm)
     x_out, y = torch.empty_like(x), torch.empty_like(x)
-    norm.forward_dev(h, x, gate, w_post, w_pre, x_out, y, stream=torch.cuda.current_stream())
+    norm.forward_dev(h, x, gate, w_post, w_pre, x_out, y, stream=torch.cuda.current_stream(x.device))
     return x_out, y
 
 
@@ -136,7 +136,7 @@ class FrameBlocks:
                         "gate": weight(channels, channels), "w_post": ones(), "w_pre": ones()} for _ in range(layers)]
 
     def _of_this_stream(self):
-        key = torch.cuda.current_stream().cuda_stream
+        key = torch.cuda.current_stream(self.first.device).cuda_stream
         if key not in self._handles:
             self._handles[key] = self.new_handles()
         return self._handles[key]
@@ -211,7 +211,7 @@ class FrameStream:
             raise ValueError(f"the streams have had their {self.frames} frames")
         self.time += 1
         self.lens += n
-        stream = torch.cuda.current_stream()
+        stream = torch.cuda.current_stream(x.device)
         x, y = b._start(x, self.norm)
         for w, (k_pages, v_pages) in zip(b.layers, self.pages):
             q, k, v = b.heads(y @ w["qkv"])

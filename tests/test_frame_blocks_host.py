@@ -16,7 +16,11 @@ from jasnamacos_amd import frame_blocks as fb
 def blocks(monkeypatch):
     """(FrameBlocks, used handles, the current stream)."""
     used, stream = [], types.SimpleNamespace(cuda_stream=0)
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: stream)
+
+    def current_stream(device=None):
+        assert device == torch.device("cpu")  # the blocks' own, not the current device's
+        return stream
+    monkeypatch.setattr(torch.cuda, "current_stream", current_stream)
     for kind, calls in ((fa.FrameAttention, ("forward_dev", "backward_dev", "paged_dev")), (fa.GatedNorm, ("forward_dev", "backward_dev"))):
         for call in calls:
             monkeypatch.setattr(kind, call, lambda self, *a, **kw: used.append(self))
