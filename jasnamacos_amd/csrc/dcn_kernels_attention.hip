@@ -7,7 +7,8 @@
 // softmax; the maximum is raised (and the sums rescaled) only when a score passes it by more
 // than 2^8, which FP32 sums do not notice. Two shapes:
 //   tile kernel  four waves of 32 rows each share tiles of 64 keys;
-//   few kernel   up to 32 rows: four waves take tiles of 32 keys in turn, each with its own
+//   few kernel   32 rows a workgroup, where there are no more or where 128-row workgroups would leave
+//                CUs idle: four or eight waves take tiles of 32 keys in turn, each with its own
 //                buffers and no barrier, and are joined at the end.
 // Both may split the key tiles over workgroups; a second kernel then joins the parts.
 //
@@ -17,7 +18,7 @@
 // 890 TFLOP/s of the 1,220 that a large product reaches; 2 x 4,096 causal tokens, 16 heads of 64: 116 us,
 // of 128: 184 us. Few kernel: HBM where histories are long (32 tokens on 16,384 of 20,011 keys, 32 heads of 128
 // on 8: 314 us, 5.5 TB/s), else the chain of launch, first tile and join (one token on 777 keys, 8 heads of 64:
-// 8.7 us).
+// 9.1 us).
 #include "dcn_attention_mfma.hpp"
 
 namespace dcn {

@@ -11,10 +11,13 @@
 //
 // A workgroup has 32 rows; its four (or eight) waves take the key tiles in turn, without a barrier
 // until their sums are joined through LDS. Where rows are few, workgroups share the key tiles of a
-// block of rows, and a second kernel joins their parts. Bound: the FP32 products, a sixteenth of the 16-bit rate, and
-// for few rows the loads' latency. 2,048 causal tokens, 8 FP32 heads of 64: 110 us (39 of the
-// 157 TFLOP/s), of 128: 172 us; FP16 heads of 96: 165 us. One FP32 token on 8,000 paged keys, 8
-// sequences of 32 heads of 128 on 8: 170 us (3.1 TB/s).
+// block of rows, and a second kernel joins their parts. Bound: the FP32 products, a sixteenth of the
+// 16-bit rate, of which it reaches under a third: every wave loads its keys and values from memory
+// itself; for few rows the loads' latency. More than 64 channels do not fit 256 registers at two
+// waves a SIMD: 67 to 78 of them are spilled up to 128 channels, 168 to 174 where rows are off four
+// elements, 185 and 377 above 128 (one wave a SIMD, 512 registers). 2,048 causal tokens, 8 FP32 heads
+// of 64: 95 us (45 of the 157 TFLOP/s), of 128: 162 us, of 256: 772 us; FP16 heads of 96: 163 us. One
+// FP32 token on 8,000 paged keys, 8 sequences of 32 heads of 128 on 8: 170 us (3.1 TB/s).
 #include "dcn_attention_mfma.hpp"
 
 namespace dcn {
@@ -273,8 +276,11 @@ __global__ __launch_bounds__(kThreads) void attention_any_join_kernel(AttentionA
 // keys (dK, dV), both as above. A lane owns a row (KEYS: a key) x1 = q, x2 = dO (k, v) as B operands
 // and the workgroup's waves take tiles of 32 of the other side, y1 = k, y2 = v (q, dO):
 //   S = y1 x1, dP = y2 x2, dS = P (dP - delta), sum1 = sum dS y1 (dQ, dK), sum2 = sum P y2 (dV).
-// Bound as above. A step of 1,024 causal tokens, forward included: 8 FP32 heads of 64: 281 us, BF16 heads
-// of 96: 434 us (a row at a time 2.7 and 4.0 ms). 128 channels leave one wave a SIMD.
+// delta is the sum of dO and out as it was rounded: in 16 bits that is off by a rounding's share of
+// |dO| |out|, which rows of few keys show most (the 16-bit kernels take theirs from P and dP).
+// Bound as above; 2 to 113 registers are spilled, but for query gradients of 65 to 128 aligned channels. A
+// step of 1,024 causal tokens, forward included: 8 FP32 heads of 64: 272 us, BF16 heads of 96: 430 us (a row
+// at a time 2.7 and 4.0 ms). 128 channels leave one wave a SIMD.
 template <typename T, int NB, bool KEYS, bool VEC>
 __global__ __launch_bounds__(kThreads, NB == 2 ? 2 : 1) void attention_any_grad_kernel(AttentionArgs a, BlockMap map) {
     constexpr int LINE = NB * 32 + 4;

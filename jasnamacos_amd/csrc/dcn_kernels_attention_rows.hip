@@ -6,7 +6,7 @@
 // 64 rows of the other side: lane = row for the dot products (the wave's own vector is in LDS as
 // FP32), then lane = channel for the weighted sum, the 64 weights in LDS. Rows that do not see each
 // other are never read, so nothing in them can reach the result. Bound: the dot products' strided
-// loads (1,024 causal tokens, 8 FP32 heads of 64: 2.6 ms).
+// loads (1,024 causal tokens, 8 heads of 256: FP32 11.4 ms, BF16 10.9).
 #include "dcn_attention_device.hpp"
 
 namespace dcn {

@@ -6,8 +6,8 @@ by their place in time, height and width (Rotary), lets every token see the fram
 (FrameAttention), projects back, and adds the result to the residual stream under a gate for
 each frame (GatedNorm, which also makes the next block's input). Serving appends each new
 frame's keys and values to the pages (CacheAppend) and reads them there; the pages of frames
-that have left the window take the newer ones, so a stream of any length has a cache of
-sinks + back + 1 frames. No counterpart in the reference.
+that have left the window take the newer ones, so a stream has a cache of sinks + back + 1
+frames however many it is made for. No counterpart in the reference.
 
     python -m jasnamacos_amd.frame_blocks [--dtype bf16] [--frames 12] [--rows 16 --columns 16]
 

@@ -48,3 +48,10 @@ def test_many_sinks(shape):
     tokens = shape.get("sequences", 1) * shape["max_q"]
     rows = (tokens * shape["q_heads"] + 3) // 4 * 4
     assert workspace(fa.PASS_BACKWARD, **shape, q_tokens=tokens, kv_tokens=tokens) <= 4 * (rows + 1024 * 2 * 128 * shape.get("dim", 64))
+
+
+@pytest.mark.parametrize("keys,parts", [(8000, 31), (540, 2), (300, 1)])
+def test_fp32_heads_in_parts(keys, parts):
+    """One token, 8 heads of 64: a workgroup a CU, of eight waves with a tile of 32 keys each at least."""
+    size = workspace(fa.PASS_FORWARD, dtype=2, q_heads=8, kv_heads=8, max_q=1, q_tokens=1, max_kv=keys, kv_tokens=keys)
+    assert size == (8 * parts * (64 + 4) * 4 if parts > 1 else 0)
