@@ -822,6 +822,75 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
                                       void* d_dk, void* d_dv, void* d_workspace, size_t workspace_bytes,
                                       void* stream);
 
+/* A microscaled cache: the keys and values of 32 adjacent channels (a block) are codes of
+ * 8 bits (e4m3: sign, 4 exponent bits of bias 7, 3 fraction bits; largest magnitude 448) or of
+ * 4 (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times one power of two, 2^(scale byte - 127).
+ * A head's tokens of a page lie together:
+ *   k, v                [pages][kv_heads][page_tokens][head_dim] bytes, or with 4 bits
+ *                       [...][head_dim / 2], the channel of the lower index in the low half
+ *   k_scales, v_scales  [pages][kv_heads][page_tokens][head_dim / 32] bytes
+ * head_dim is a multiple of 32. What is written of a block: the smallest power of two (2^-127
+ * at least) at which its largest magnitude is 448 (6) at most, codes to the nearest, ties to even.
+ * Magnitudes whose code would read back as an infinity of the dtype count as the largest that does not
+ * (FP16: 61440, with 4 bits 49152; BF16 and FP32: 1.875 * 2^127, with 4 bits 1.5 * 2^127).
+ * A block with an infinity or a NaN is written as zeros with the scale byte 255, which
+ * reads as NaN; so does the e4m3 code of seven ones.
+ *
+ * dcn_pages: a cache with the buffers it lies in. cache.dtype is that of the tensors
+ * outside; bits 8 or 4: microscaled; 0: pages of that dtype as dcn_cache has them (the scales are
+ * then ignored), which only dcn_attention_pages_dev takes, with a prefix. */
+typedef struct dcn_pages {
+    dcn_cache cache;
+    int32_t bits;
+    int32_t reserved; /* 0 */
+    void* k;
+    void* v;
+    void* k_scales;
+    void* v_scales;
+} dcn_pages;
+/* dcn_cache_append_dev into a microscaled cache. Keys are quantised from their rotation in
+ * FP32, without a rounding to the dtype in between. */
+dcn_status dcn_cache_append_mx_dev(dcn_context* ctx, const dcn_pages* pages, const dcn_append_shape* shape,
+                                   const dcn_rotary* rotary, const void* d_q, const void* d_k, const void* d_v,
+                                   const int32_t* d_positions, const float* d_freq, const int32_t* d_cu_q,
+                                   const int32_t* d_kv_lens, const int32_t* d_table, void* d_q_out, void* stream);
+/* Reads a microscaled cache back: rows cu[s] .. cu[s + 1] of k_out and v_out ([tokens][kv_heads]
+ * [head_dim], rounded to the dtype) get the last of sequence s's kv_lens[s] tokens, as an append wrote
+ * them. Rows of no sequence, of tokens past the table's width and of tokens whose page is
+ * not in the pool are not written. */
+typedef struct dcn_read_shape {
+    int32_t sequences;
+    int32_t reserved; /* 0 */
+    int64_t tokens;   /* rows of k_out and v_out */
+    int64_t k_stride[2], v_stride[2]; /* token, head */
+} dcn_read_shape;
+dcn_status dcn_cache_read_dev(dcn_context* ctx, const dcn_pages* pages, const dcn_read_shape* shape,
+                              const int32_t* d_cu, const int32_t* d_kv_lens, const int32_t* d_table, void* d_k_out,
+                              void* d_v_out, void* stream);
+
+/* A run of tokens that stands before those of every sequence: tokens[0] of them (a device
+ * value; 0 .. max_tokens, more count as max_tokens), token p in row p % page_tokens of page
+ * table[p / page_tokens]. max_tokens is at most width * page_tokens. */
+typedef struct dcn_prefix {
+    int32_t width; /* entries of the table */
+    int32_t max_tokens;
+    const int32_t* table;
+    const int32_t* tokens;
+} dcn_prefix;
+/* dcn_attention_paged_dev over a microscaled cache, or over one of either kind in which
+ * the sequences share a prefix (null: none). With a prefix of P tokens, sequence s's keys are the
+ * prefix's and then its own kv_lens[s], of which its table speaks: query i of nq is token
+ * P + kv_lens[s] - nq + i, and frames, the window and sinks count from the prefix's first token.
+ * shape.max_kv bounds kv_lens. The prefix's keys are read once for the queries of all
+ * sequences (heads of 64 and 128 channels in 16 bits; others are read for each query), whose
+ * results are then joined in FP32. (width + table_width) * page_tokens must be below 2^31. */
+size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages,
+                                           const dcn_prefix* prefix);
+dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_pages* pages,
+                                   const dcn_prefix* prefix, const void* d_q, const int32_t* d_cu_q,
+                                   const int32_t* d_kv_lens, const int32_t* d_table, void* d_out, float* d_lse,
+                                   void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* The norms around a block's residual addition, over adjacent [tokens][channels] tensors:
  *   n = h * r1, r1 = 1 / sqrt(mean(h^2) + eps);  x_out = x + residual_scale * gate * n * w_post
  *   y = x_out * r2 * w_pre, r2 = 1 / sqrt(mean(x_out^2) + eps)

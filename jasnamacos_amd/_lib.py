@@ -116,6 +116,25 @@ class DcnAttentionShape(C.Structure):
                        + [(n + "_stride", C.c_int64 * 2) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")])
 
 
+class DcnPages(C.Structure):
+    """dcn_pages."""
+
+    _fields_ = ([("cache", DcnCache)] + _fields(("bits", "reserved"))
+                + [(n, C.c_void_p) for n in ("k", "v", "k_scales", "v_scales")])
+
+
+class DcnReadShape(C.Structure):
+    """dcn_read_shape."""
+
+    _fields_ = _fields(("sequences", "reserved"), [("tokens", C.c_int64)] + [(n + "_stride", C.c_int64 * 2) for n in ("k", "v")])
+
+
+class DcnPrefix(C.Structure):
+    """dcn_prefix."""
+
+    _fields_ = _fields(("width", "max_tokens"), [("table", C.c_void_p), ("tokens", C.c_void_p)])
+
+
 class DcnNormShape(C.Structure):
     """dcn_norm_shape."""
 
@@ -265,6 +284,10 @@ SIGNATURES: dict[str, tuple] = {
     "dcn_attention_paged_dev": (C.c_int, [CtxP, c_void, c_void] + [c_void] * 9
                                 + [c_size, c_void]),
     "dcn_attention_backward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 12 + [c_size, c_void]),
+    "dcn_cache_append_mx_dev": (C.c_int, [CtxP, c_void, c_void, c_void] + [c_void] * 10),
+    "dcn_cache_read_dev": (C.c_int, [CtxP, c_void, c_void] + [c_void] * 6),
+    "dcn_attention_pages_workspace_bytes": (c_size, [c_void, c_void, c_void]),
+    "dcn_attention_pages_dev": (C.c_int, [CtxP, c_void, c_void, c_void] + [c_void] * 7 + [c_size, c_void]),
     "dcn_gated_norm_forward_dev": (C.c_int, [CtxP, c_void] + [c_void] * 10),
     "dcn_gated_norm_low_bytes": (c_size, [c_void]),
     "dcn_gated_norm_workspace_bytes": (c_size, [c_void]),

@@ -79,6 +79,22 @@ struct AppendArgs {
 };
 hipError_t launch_append(int dtype, const AppendArgs& a, const RotaryArgs& r, hipStream_t stream);
 
+// The buffers of a microscaled cache: a head's tokens of a page lie together.
+struct MxArgs {
+    int bits, heads, dim;
+    uint8_t *k, *v, *ks, *vs;
+};
+hipError_t launch_append_mx(int dtype, const AppendArgs& a, const MxArgs& mx, const RotaryArgs& r, hipStream_t stream);
+struct ReadArgs {
+    int sequences;
+    int64_t tokens;
+    const int32_t* cu;
+    const int32_t* kv_lens;
+    PagesArgs pages;
+    HeadsOut k, v;
+};
+hipError_t launch_cache_read(int dtype, const ReadArgs& a, const MxArgs& mx, hipStream_t stream);
+
 struct NormArgs {
     int channels;
     int64_t tokens, gate_tokens;
@@ -110,6 +126,16 @@ int attention_any_splits(const dcn_attention_shape& s);
 size_t attention_any_workspace(const dcn_attention_shape& s);
 hipError_t launch_attention_any_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
+
+// Attention over microscaled pages, or with a prefix that the sequences share.
+struct PagesAttention {
+    AttentionArgs a;          // the sequences' own keys; as-is pages are a.k and a.v
+    MxArgs mx;                // mx.bits 0: as-is pages
+    PagesArgs prefix;         // table null: none
+    const int32_t* prefix_len;
+    int max_prefix;
+};
+hipError_t launch_attention_pages_any(int dtype, const PagesAttention& p, hipStream_t stream);
 
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).
 hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream);

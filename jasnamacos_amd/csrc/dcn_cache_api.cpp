@@ -1,0 +1,168 @@
+// C-ABI host layer of the microscaled cache (append, read back) and of the attention over it
+// and over prefixes that sequences share. Checks every size, stride and pointer that a kernel relies on,
+// then launches; nothing here allocates or synchronises.
+#include "dcn_attention_host.hpp"
+
+using namespace dcn::host;
+
+namespace {
+
+// The sizes of a cache and how it holds them; as_is: pages of the dtype are taken too.
+dcn_status check_pages(dcn_context* ctx, const dcn_pages* p, bool as_is, dcn::PagesArgs* pages, dcn::MxArgs* mx) {
+    DCN_TRY(check_cache(ctx, &p->cache, pages));
+    REQUIRE_SHAPE(p->bits == 8 || p->bits == 4 || (as_is && p->bits == 0),
+                  "pages of " + std::to_string(p->bits) + " bits: microscaled ones have 8 or 4");
+    REQUIRE_SHAPE(p->reserved == 0, "pages reserved must be 0");
+    REQUIRE_SHAPE(!p->bits || p->cache.head_dim % 32 == 0, "a microscaled cache needs a head_dim of whole blocks of 32");
+    *mx = dcn::MxArgs{p->bits, p->cache.kv_heads, p->cache.head_dim, (uint8_t*)p->k, (uint8_t*)p->v, (uint8_t*)p->k_scales, (uint8_t*)p->v_scales};
+    return DCN_OK;
+}
+
+dcn_status check_aligned(dcn_context* ctx, const char* name, const void* p, size_t to) {
+    if (!p) return null_fail(ctx, name);
+    if ((uintptr_t)p % to)
+        return fail(ctx, DCN_INVALID_ARGUMENT, std::string(name) + " is not aligned to " + std::to_string(to) + " bytes");
+    return DCN_OK;
+}
+
+// The buffers of a cache.
+dcn_status check_buffers(dcn_context* ctx, const dcn_pages* p) {
+    if (!p->bits) {
+        DCN_TRY(check_pointer(ctx, "k_pages", p->k, p->cache.dtype));
+        return check_pointer(ctx, "v_pages", p->v, p->cache.dtype);
+    }
+    DCN_TRY(check_aligned(ctx, "k codes", p->k, 16));
+    DCN_TRY(check_aligned(ctx, "v codes", p->v, 16));
+    DCN_TRY(check_aligned(ctx, "k_scales", p->k_scales, 4));
+    return check_aligned(ctx, "v_scales", p->v_scales, 4);
+}
+
+// The sizes of an attention call, after which p has everything but the pointers.
+dcn_status check_call(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_pages* pages, const dcn_prefix* prefix,
+                      dcn::PagesAttention* p) {
+    DCN_TRY(check_pages(ctx, pages, prefix != nullptr, &p->a.pages, &p->mx));
+    DCN_TRY(check_attention(ctx, shape, true, &p->a));
+    const dcn_cache& c = pages->cache;
+    REQUIRE_SHAPE(c.dtype == shape->dtype && c.kv_heads == shape->kv_heads && c.head_dim == shape->head_dim,
+                  "attention and cache have different types, key heads or head sizes");
+    p->prefix = p->a.pages;
+    p->prefix.table = nullptr;
+    p->prefix.width = 0;
+    if (prefix) {
+        REQUIRE_SHAPE(prefix->width >= 0 && ((int64_t)prefix->width + c.table_width) * c.page_tokens <= INT32_MAX,
+                      "(prefix width + table_width) * page_tokens must be below 2^31");
+        REQUIRE_SHAPE(prefix->max_tokens >= 0 && prefix->max_tokens <= (int64_t)prefix->width * c.page_tokens,
+                      "prefix max_tokens must be 0..width * page_tokens");
+        p->prefix.width = prefix->width;
+        p->max_prefix = prefix->max_tokens;
+    }
+    return DCN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+dcn_status dcn_cache_append_mx_dev(dcn_context* ctx, const dcn_pages* pages, const dcn_append_shape* shape,
+                                   const dcn_rotary* rotary, const void* d_q, const void* d_k, const void* d_v,
+                                   const int32_t* d_positions, const float* d_freq, const int32_t* d_cu_q,
+                                   const int32_t* d_kv_lens, const int32_t* d_table, void* d_q_out, void* stream) {
+    return entry(ctx, [&]() -> dcn_status {
+        REQUIRE_POINTER(pages);
+        REQUIRE_POINTER(shape);
+        const dcn_cache* cache = &pages->cache;
+        dcn::AppendArgs a{};
+        dcn::MxArgs mx;
+        DCN_TRY(check_pages(ctx, pages, false, &a.pages, &mx));
+        dcn::RotaryArgs r{};
+        r.dim = cache->head_dim;
+        DCN_TRY(check_append(ctx, cache, shape, rotary, d_q != nullptr, &r));
+        if (!shape->tokens || !shape->sequences) return DCN_OK;
+        DCN_TRY(check_append_pointers(ctx, cache, shape, r, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out));
+        DCN_TRY(check_buffers(ctx, pages));
+        fill_append(&a, &r, cache, shape, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out);
+        DCN_HIP(ctx, dcn::launch_append_mx(cache->dtype, a, mx, r, (hipStream_t)stream));
+        return DCN_OK;
+    });
+}
+
+dcn_status dcn_cache_read_dev(dcn_context* ctx, const dcn_pages* pages, const dcn_read_shape* shape, const int32_t* d_cu,
+                              const int32_t* d_kv_lens, const int32_t* d_table, void* d_k_out, void* d_v_out, void* stream) {
+    return entry(ctx, [&]() -> dcn_status {
+        REQUIRE_POINTER(pages);
+        REQUIRE_POINTER(shape);
+        const dcn_cache* cache = &pages->cache;
+        dcn::ReadArgs a{};
+        dcn::MxArgs mx;
+        DCN_TRY(check_pages(ctx, pages, false, &a.pages, &mx));
+        REQUIRE_SHAPE(shape->reserved == 0, "read reserved must be 0");
+        REQUIRE_SHAPE(shape->sequences >= 0 && shape->tokens >= 0 && shape->tokens <= INT32_MAX,
+                      "read sequences and tokens must be 0..2^31-1");
+        DCN_TRY(check_out_strides(ctx, "k_out", shape->k_stride, shape->tokens, cache->kv_heads, cache->head_dim));
+        DCN_TRY(check_out_strides(ctx, "v_out", shape->v_stride, shape->tokens, cache->kv_heads, cache->head_dim));
+        if (!shape->tokens || !shape->sequences) return DCN_OK;
+        DCN_TRY(check_buffers(ctx, pages));
+        DCN_TRY(check_pointer(ctx, "cu", d_cu, DCN_DTYPE_F32));
+        DCN_TRY(check_pointer(ctx, "kv_lens", d_kv_lens, DCN_DTYPE_F32));
+        DCN_TRY(check_pointer(ctx, "table", d_table, DCN_DTYPE_F32));
+        DCN_TRY(check_pointer(ctx, "k_out", d_k_out, cache->dtype));
+        DCN_TRY(check_pointer(ctx, "v_out", d_v_out, cache->dtype));
+        a.sequences = shape->sequences;
+        a.tokens = shape->tokens;
+        a.cu = d_cu;
+        a.kv_lens = d_kv_lens;
+        a.pages.table = d_table;
+        a.k = {d_k_out, shape->k_stride[0], shape->k_stride[1]};
+        a.v = {d_v_out, shape->v_stride[0], shape->v_stride[1]};
+        DCN_HIP(ctx, dcn::launch_cache_read(cache->dtype, a, mx, (hipStream_t)stream));
+        return DCN_OK;
+    });
+}
+
+size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages, const dcn_prefix* prefix) {
+    return 0;
+}
+
+dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* given, const dcn_pages* pages,
+                                   const dcn_prefix* prefix, const void* d_q, const int32_t* d_cu_q,
+                                   const int32_t* d_kv_lens, const int32_t* d_table, void* d_out, float* d_lse,
+                                   void* d_workspace, size_t workspace_bytes, void* stream) {
+    return entry(ctx, [&]() -> dcn_status {
+        if (!given) return null_fail(ctx, "shape");
+        REQUIRE_POINTER(pages);
+        REQUIRE_SHAPE(d_cu_q || (int64_t)given->sequences * given->max_q <= given->q_tokens,
+                      "sequences * max_q exceeds q_tokens");
+        const dcn_attention_shape own = fitted(*given, true), *shape = &own;
+        dcn::PagesAttention p{};
+        DCN_TRY(check_call(ctx, shape, pages, prefix, &p));
+        DCN_TRY(check_out_strides(ctx, "out", shape->out_stride, shape->q_tokens, shape->q_heads, shape->head_dim));
+        if (!shape->sequences || !shape->max_q || !shape->q_tokens) return DCN_OK;
+        DCN_TRY(check_buffers(ctx, pages));
+        DCN_TRY(check_pointer(ctx, "q", d_q, shape->dtype));
+        DCN_TRY(check_pointer(ctx, "out", d_out, shape->dtype));
+        DCN_TRY(check_pointer(ctx, "kv_lens", d_kv_lens, DCN_DTYPE_F32));
+        DCN_TRY(check_pointer(ctx, "table", d_table, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "lse", d_lse, DCN_DTYPE_F32));
+        DCN_TRY(check_optional(ctx, "cu_q", d_cu_q, DCN_DTYPE_F32));
+        const bool shared = prefix && prefix->max_tokens;
+        if (shared) {
+            DCN_TRY(check_pointer(ctx, "prefix table", prefix->table, DCN_DTYPE_F32));
+            DCN_TRY(check_pointer(ctx, "prefix tokens", prefix->tokens, DCN_DTYPE_F32));
+        }
+        const int64_t ts = (int64_t)pages->cache.kv_heads * pages->cache.head_dim;
+        p.a.q.p = d_q;
+        p.a.k = {pages->k, ts, pages->cache.head_dim};
+        p.a.v = {pages->v, ts, pages->cache.head_dim};
+        p.a.out.p = d_out;
+        p.a.lse = d_lse;
+        p.a.cu_q = d_cu_q;
+        p.a.cu_kv = d_kv_lens;
+        p.a.pages.table = d_table;
+        p.prefix.table = shared ? prefix->table : nullptr;
+        p.prefix_len = shared ? prefix->tokens : nullptr;
+        DCN_HIP(ctx, dcn::launch_attention_pages_any(shape->dtype, p, (hipStream_t)stream));
+        return DCN_OK;
+    });
+}
+
+}  // extern "C"

@@ -3,8 +3,10 @@ frames attend to the frames before them.
 
   Rotary          rotary positions with three axes (time, height, width), and their gradient
   CacheAppend     new keys and values into a paged cache, rotated on the way
+  MxPages         the buffers of a microscaled cache: codes of 8 or 4 bits, a power of two for 32
+  CacheRead       a microscaled cache read back
   FrameAttention  attention over a window of frames with the first ones kept visible:
-                  forward, backward, and over the paged cache
+                  forward, backward, over the paged cache, and for streams that share a prefix
   GatedNorm       the norms after and before a block, its gate and its residual scale
 
 No counterpart in the reference. Tensors are torch tensors on the context's device;
@@ -98,6 +100,10 @@ _ROTARY = struct.Struct("6i")
 _CACHE = struct.Struct("6i")
 _APPEND = struct.Struct("iiq8q")
 _ATTENTION = struct.Struct("11ifqq16q")
+_PAGES = struct.Struct("8i4Q")
+_AS_IS = struct.Struct("2i4Q")  # of a dcn_pages, what follows its dcn_cache
+_READ = struct.Struct("iiq4q")
+_PREFIX = struct.Struct("2i2Q")
 _NORM = struct.Struct("iiqqff")
 _NO_STRIDES = (0, 0)
 
@@ -225,8 +231,31 @@ class CacheAppend(_Handle):
         q_out where it is given."""
         device = self.ctx.device
         cache = _cache(k_pages, v_pages, table, device)
-        tokens, sequences, dtype = _rows("k", k), table.shape[0], k_pages.dtype
-        _, _, kv_heads, dim = k_pages.shape
+        s, r = self._shape(k, v, table, cu_q, kv_lens, rotary, positions, freq, q, q_out, k_pages.dtype, *k_pages.shape[2:])
+        status = self._lib.dcn_cache_append_dev(
+            self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
+            kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
+            stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
+
+    def run_mx_dev(self, k, v, pages: "MxPages", table, cu_q, kv_lens, rotary: Rotary | None = None, positions=None, freq=None,
+                   q=None, q_out=None, stream=None) -> None:
+        """run_dev into a microscaled cache (dcn_cache_append_mx_dev)."""
+        if k is None:
+            raise DeformConvError(INVALID_ARGUMENT, "k is missing")
+        cache = pages._pack(table, k.dtype, self.ctx.device)
+        s, r = self._shape(k, v, table, cu_q, kv_lens, rotary, positions, freq, q, q_out, k.dtype, pages.kv_heads, pages.head_dim)
+        status = self._lib.dcn_cache_append_mx_dev(
+            self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
+            kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
+
+    def _shape(self, k, v, table, cu_q, kv_lens, rotary, positions, freq, q, q_out, dtype, kv_heads, dim):
+        """The packed dcn_append_shape and dcn_rotary (or None), after the checks."""
+        device = self.ctx.device
+        tokens, sequences = _rows("k", k), table.shape[0]
         shape = (tokens, kv_heads, dim)
         ks, vs = _heads("k", k, dtype, shape, device), _heads("v", v, dtype, shape, device)
         _index("cu_q", cu_q, sequences + 1, device)
@@ -246,10 +275,86 @@ class CacheAppend(_Handle):
             s = _APPEND.pack(sequences, q_heads, tokens, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1])
         except struct.error:
             raise _outside() from None
-        status = self._lib.dcn_cache_append_dev(
-            self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
-            kv_lens.data_ptr(), table.data_ptr(), _ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
-            stream and _stream(stream))
+        return s, r
+
+
+class MxPages:
+    """The buffers of a microscaled cache (dcn_pages): blocks of 32 channels are codes of 8 bits (e4m3)
+    or 4 (e2m1) and one power of two. k and v are uint8 [pages][kv_heads][page_tokens][head_dim, or
+    half of it with 4 bits], k_scales and v_scales uint8 [pages][kv_heads][page_tokens][head_dim / 32]."""
+
+    def __init__(self, k, v, k_scales, v_scales):
+        for name, t in (("k", k), ("v", v), ("k_scales", k_scales), ("v_scales", v_scales)):
+            if t is None:
+                raise DeformConvError(INVALID_ARGUMENT, f"{name} is missing")
+            if t.dtype is not torch.uint8:
+                raise DeformConvError(INVALID_ARGUMENT, f"{name} is {t.dtype}; expected torch.uint8")
+            _need(t.dim() == 4, f"{name} has {t.dim()} dimensions; expected [pages][kv_heads][page_tokens][...]")
+        self.head_dim = 32 * k_scales.shape[3]
+        _need(self.head_dim > 0 and k.shape[3] in (self.head_dim, self.head_dim // 2),
+              f"{k.shape[3]} bytes of codes do not belong to {k_scales.shape[3]} scales")
+        self.bits = 8 if k.shape[3] == self.head_dim else 4
+        device = k.get_device()
+        _whole("v", v, torch.uint8, k.shape, device)
+        _whole("k", k, torch.uint8, k.shape, device)
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            _whole(name, t, torch.uint8, k.shape[:3] + (k_scales.shape[3],), device)
+        self._buffers, self._device = (k, v, k_scales, v_scales), device
+        self.kv_heads, self.page_tokens = k.shape[1], k.shape[2]
+
+    k = property(lambda self: self._buffers[0])
+    v = property(lambda self: self._buffers[1])
+    k_scales = property(lambda self: self._buffers[2])
+    v_scales = property(lambda self: self._buffers[3])
+
+    @classmethod
+    def zeros(cls, pages: int, page_tokens: int, kv_heads: int, head_dim: int, bits: int = 8, device="cuda") -> "MxPages":
+        _need(bits in (4, 8), f"{bits} bits: a microscaled cache has 8 or 4")
+        _need(head_dim > 0 and head_dim % 32 == 0, "a microscaled cache needs a head_dim of whole blocks of 32")
+        shape = (pages, kv_heads, page_tokens)
+        return cls(*(torch.zeros(*shape, n, dtype=torch.uint8, device=device)
+                     for n in (head_dim * bits // 8,) * 2 + (head_dim // 32,) * 2))
+
+    def _pack(self, table, dtype, device: int) -> bytes:
+        """The packed dcn_pages of a call with this table."""
+        if table is None:
+            raise DeformConvError(INVALID_ARGUMENT, "table is missing")
+        if table.dim() != 2:
+            raise DeformConvError(INVALID_SHAPE, "the table is [sequences][width]")
+        _whole("table", table, torch.int32, table.shape, device)
+        if self._device != device:
+            _on_device("k", self.k, device)
+        code = DTYPES.get(dtype)
+        if code is None:
+            raise DeformConvError(INVALID_ARGUMENT, f"dtype {dtype} is not float16, bfloat16 or float32")
+        k, v, k_scales, v_scales = self._buffers
+        try:
+            return _PAGES.pack(k.shape[0], self.page_tokens, table.shape[1], self.kv_heads, self.head_dim, code, self.bits, 0,
+                               k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
+        except struct.error:
+            raise _outside() from None
+
+
+class CacheRead(_Handle):
+    """Reads a microscaled cache back (dcn_cache_read_dev)."""
+
+    def run_dev(self, pages: MxPages, table, cu, kv_lens, k_out, v_out, stream=None) -> None:
+        """Rows cu[s] .. cu[s + 1] of k_out and v_out ([tokens][kv_heads][head_dim]) get the last of
+        sequence s's kv_lens[s] tokens, rounded to their type."""
+        device = self.ctx.device
+        tokens, dtype = _rows("k_out", k_out), k_out.dtype
+        packed = pages._pack(table, dtype, device)
+        shape = (tokens, pages.kv_heads, pages.head_dim)
+        ks, vs = _heads("k_out", k_out, dtype, shape, device), _heads("v_out", v_out, dtype, shape, device)
+        sequences = table.shape[0]
+        _index("cu", cu, sequences + 1, device)
+        _index("kv_lens", kv_lens, sequences, device)
+        try:
+            s = _READ.pack(sequences, 0, tokens, ks[0], ks[1], vs[0], vs[1])
+        except struct.error:
+            raise _outside() from None
+        status = self._lib.dcn_cache_read_dev(self._ctx, packed, s, cu.data_ptr(), kv_lens.data_ptr(), table.data_ptr(),
+                                              k_out.data_ptr(), v_out.data_ptr(), stream and _stream(stream))
         if status:
             self.ctx._check(status)
 
@@ -368,6 +473,70 @@ class FrameAttention(_Handle):
         status = self._lib.dcn_attention_paged_dev(
             self._ctx, s, cache, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(cu_q), kv_lens.data_ptr(),
             table.data_ptr(), out.data_ptr(), _ptr(lse), w, size, stream and _stream(stream))
+        if status:
+            self.ctx._check(status)
+
+    def paged_mx_dev(self, q, pages: MxPages, table, cu_q, kv_lens, out, lse=None, max_q=None, max_kv=None, stream=None) -> None:
+        """paged_dev over a microscaled cache."""
+        if q is None:
+            raise DeformConvError(INVALID_ARGUMENT, "q is missing")
+        cache = pages._pack(table, q.dtype, self.ctx.device)
+        self._pages(q, cache, pages.page_tokens, None, table, cu_q, kv_lens, out, lse, max_q, max_kv, stream)
+
+    def shared_dev(self, q, pages, prefix_table, prefix_len, table, cu_q, kv_lens, out, lse=None, max_q=None, max_kv=None,
+                   max_prefix=None, stream=None) -> None:
+        """paged_dev, or paged_mx_dev, for sequences that share a prefix: prefix_len[0] tokens on the
+        pages of prefix_table ([width]) stand before every sequence's own kv_lens[s], of which `table`
+        and max_kv speak. pages: an MxPages, or (k_pages, v_pages). Positions, the window and the sinks
+        count from the prefix's first token. max_prefix bounds prefix_len (default: the table's width)."""
+        device = self.ctx.device
+        if q is None:
+            raise DeformConvError(INVALID_ARGUMENT, "q is missing")
+        if isinstance(pages, MxPages):
+            cache, page_tokens = pages._pack(table, q.dtype, device), pages.page_tokens
+        else:
+            k_pages, v_pages = pages
+            sizes = _cache(k_pages, v_pages, table, device)
+            if k_pages.dtype is not q.dtype:
+                raise DeformConvError(INVALID_ARGUMENT, f"k_pages is {k_pages.dtype}; expected {q.dtype}")
+            cache, page_tokens = sizes + _AS_IS.pack(0, 0, k_pages.data_ptr(), v_pages.data_ptr(), 0, 0), k_pages.shape[1]
+        if prefix_table is None:
+            raise DeformConvError(INVALID_ARGUMENT, "prefix_table is missing")
+        if prefix_table.dim() != 1:
+            raise DeformConvError(INVALID_SHAPE, f"prefix_table has {prefix_table.dim()} dimensions; expected one")
+        width = prefix_table.shape[0]
+        _index("prefix_table", prefix_table, width, device)
+        _index("prefix_len", prefix_len, 1, device)
+        if max_prefix is None:
+            max_prefix = width * page_tokens
+        try:
+            prefix = _PREFIX.pack(width, int(max_prefix), prefix_table.data_ptr(), prefix_len.data_ptr())
+        except struct.error:
+            raise _outside() from None
+        self._pages(q, cache, page_tokens, prefix, table, cu_q, kv_lens, out, lse, max_q, max_kv, stream)
+
+    def _pages(self, q, cache, page_tokens, prefix, table, cu_q, kv_lens, out, lse, max_q, max_kv, stream) -> None:
+        """dcn_attention_pages_dev."""
+        device = self.ctx.device
+        sequences, q_tokens, dtype = table.shape[0], _rows("q", q), q.dtype
+        if cu_q is not None:
+            _index("cu_q", cu_q, sequences + 1, device)
+        _index("kv_lens", kv_lens, sequences, device)
+        if max_q is None:
+            max_q = q_tokens if cu_q is not None else (q_tokens // sequences if sequences else 0)
+        if max_kv is None:
+            max_kv = table.shape[1] * page_tokens
+        shape = (q_tokens, self.q_heads, self.head_dim)
+        if lse is not None:
+            _whole("lse", lse, torch.float32, (q_tokens, self.q_heads), device)
+        s = self._pack(q, sequences, int(max_q), int(max_kv), q_tokens, 0, _heads("q", q, dtype, shape, device), _NO_STRIDES,
+                       _NO_STRIDES, _heads("out", out, dtype, shape, device))
+        # Sizes without pointers and strides: those have no part in the workspace's.
+        w, size = self._room((s[:64], cache[:32], prefix and prefix[:8]),
+                             lambda: self._lib.dcn_attention_pages_workspace_bytes(s, cache, prefix), q)
+        status = self._lib.dcn_attention_pages_dev(
+            self._ctx, s, cache, prefix, q.data_ptr(), _ptr(cu_q), kv_lens.data_ptr(), table.data_ptr(), out.data_ptr(),
+            _ptr(lse), w, size, stream and _stream(stream))
         if status:
             self.ctx._check(status)
 
