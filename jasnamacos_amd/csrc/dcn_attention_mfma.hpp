@@ -158,16 +158,20 @@ inline bool block_map(int64_t x, int64_t heads, int64_t sequences, BlockMap* m) 
     *m = BlockMap{(int)x, (int)heads, (int)pairs, (int)classes, (unsigned)(8 * each)};
     return x < INT32_MAX && each < (INT64_C(1) << 32) / kThreads / 8;  // fewer than 2^32 threads
 }
-// Block, key head and sequence of this workgroup; false for the padding.
-__device__ __forceinline__ bool block_of(const BlockMap& m, int* block, int* head, int* sequence) {
-    const int xcd = blockIdx.x & 7, share = 8 / m.classes;
-    const int item = (int)(blockIdx.x >> 3) * share + xcd / m.classes;
+// Block, key head and sequence of workgroup `index`; false for the padding.
+__device__ __forceinline__ bool block_of(const BlockMap& m, unsigned index, int* block, int* head, int* sequence) {
+    const int xcd = index & 7, share = 8 / m.classes;
+    const int item = (int)(index >> 3) * share + xcd / m.classes;
     const int nth = item / m.x, pair = xcd % m.classes + m.classes * nth;
     if (pair >= m.pairs) return false;
     *block = item - nth * m.x;
     *head = pair % m.heads;
     *sequence = pair / m.heads;
     return true;
+}
+
+__device__ __forceinline__ bool block_of(const BlockMap& m, int* block, int* head, int* sequence) {
+    return block_of(m, blockIdx.x, block, head, sequence);
 }
 
 // Where one workgroup works.

@@ -59,6 +59,16 @@ dcn_status check_call(dcn_context* ctx, const dcn_attention_shape* shape, const 
     return DCN_OK;
 }
 
+// Whether the matrix kernels take a call of these sizes: as in the paged call, and rows of all sequences
+// and of the pool that an int counts.
+bool matrix_call(const dcn_attention_shape* s, const dcn_pages* p) {
+    const int64_t rows = (int64_t)p->cache.pages * p->cache.page_tokens * (p->bits ? p->cache.kv_heads : 1);
+    return matrix_heads(s) && p->cache.page_tokens >= 8 && rows <= INT32_MAX && s->q_tokens * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
+}
+size_t workspace_of(const dcn_attention_shape* s, const dcn_pages* pages, const dcn::PagesAttention& p) {
+    return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, p.max_prefix) : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -120,7 +130,15 @@ dcn_status dcn_cache_read_dev(dcn_context* ctx, const dcn_pages* pages, const dc
 }
 
 size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages, const dcn_prefix* prefix) {
-    return 0;
+    dcn::PagesAttention p{};
+    try {
+        if (!shape || !pages) return 0;
+        const dcn_attention_shape s = fitted(*shape, true);
+        if (check_call(nullptr, &s, pages, prefix, &p) != DCN_OK) return 0;
+        return workspace_of(&s, pages, p);
+    } catch (const std::exception&) {
+        return 0;
+    }
 }
 
 dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* given, const dcn_pages* pages,
@@ -144,6 +162,7 @@ dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* 
         DCN_TRY(check_pointer(ctx, "table", d_table, DCN_DTYPE_F32));
         DCN_TRY(check_optional(ctx, "lse", d_lse, DCN_DTYPE_F32));
         DCN_TRY(check_optional(ctx, "cu_q", d_cu_q, DCN_DTYPE_F32));
+        DCN_TRY(check_workspace(ctx, d_workspace, workspace_bytes, workspace_of(shape, pages, p)));
         const bool shared = prefix && prefix->max_tokens;
         if (shared) {
             DCN_TRY(check_pointer(ctx, "prefix table", prefix->table, DCN_DTYPE_F32));
@@ -160,7 +179,10 @@ dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* 
         p.a.pages.table = d_table;
         p.prefix.table = shared ? prefix->table : nullptr;
         p.prefix_len = shared ? prefix->tokens : nullptr;
-        DCN_HIP(ctx, dcn::launch_attention_pages_any(shape->dtype, p, (hipStream_t)stream));
+        p.a.workspace = d_workspace;
+        const bool matrix = matrix_call(shape, pages) && matrix_tensor(p.a.q) && matrix_tensor(p.a.out) &&
+                            (pages->bits || (matrix_tensor(p.a.k) && matrix_tensor(p.a.v)));
+        DCN_HIP(ctx, (matrix ? dcn::launch_attention_pages : dcn::launch_attention_pages_any)(shape->dtype, p, (hipStream_t)stream));
         return DCN_OK;
     });
 }
