@@ -136,7 +136,7 @@ struct PagesAttention {
     int max_prefix;
 };
 hipError_t launch_attention_pages(int dtype, const PagesAttention& p, hipStream_t stream);
-size_t attention_pages_workspace(const dcn_attention_shape& s, int max_prefix);
+size_t attention_pages_workspace(const dcn_attention_shape& s, int bits, int max_prefix);
 hipError_t launch_attention_pages_any(int dtype, const PagesAttention& p, hipStream_t stream);
 
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).

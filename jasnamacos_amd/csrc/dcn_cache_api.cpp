@@ -66,7 +66,7 @@ bool matrix_call(const dcn_attention_shape* s, const dcn_pages* p) {
     return matrix_heads(s) && p->cache.page_tokens >= 8 && rows <= INT32_MAX && s->q_tokens * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
 }
 size_t workspace_of(const dcn_attention_shape* s, const dcn_pages* pages, const dcn::PagesAttention& p) {
-    return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, p.max_prefix) : 0;
+    return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, pages->bits, p.max_prefix) : 0;
 }
 
 }  // namespace
