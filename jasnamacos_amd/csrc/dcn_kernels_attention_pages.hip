@@ -51,17 +51,17 @@ __device__ __forceinline__ void tile_block(const PagesCall& c, unsigned number, 
     const bool idle = high1 == kNowhere;  // no rows: the wave copies only
     int count;
     Cursor<ROWS> now(c, b, low, high, &count);
-    Spread all = spread_in(c, b, low, high, now.second), mine = spread_in(c, b, low1, high1, now.second);
+    Spread all = spread_in(c, b, low, high, now.second), mine = spread_in(c, b, low1, high1, now.second);  // all: of the run ahead
     const int from = pl.split * b.per, to = last_tile(count, from, b);
     const float scale = p.a.scale * kLog2e;
     Stage<T, D, BITS, ROWS, kWaves> stage(p, pl.kh, wave, lane);
     Cursor<ROWS> ahead = now;
     bool next_part = false;  // whether some row does not see all of the tile that was found last
     auto find = [&](int i) {
-        ahead.go(c, b, low, high, i);
+        if (ahead.go(c, b, low, high, i)) all = spread_in(c, b, low, high, 1);
         const int t0 = ahead.tile(i);
         stage.find(p, ahead.run, pl.kh, t0, wave);
-        next_part = stage.holes || !all_see<ROWS>(spread_in(c, b, low, high, ahead.second), t0);
+        next_part = stage.holes || !all_see<ROWS>(all, t0);
     };
     // Of the present tile, the one behind it, and the one behind that: holes, and whether it is seen in part.
     unsigned long long holes = 0, holes1 = 0;
@@ -89,10 +89,7 @@ __device__ __forceinline__ void tile_block(const PagesCall& c, unsigned number, 
     st.settle();
     for (int i = from; i < to; ++i) {
         const int buf = (i - from) & 1;
-        if (now.go(c, b, low, high, i)) {
-            all = spread_in(c, b, low, high, 1);
-            mine = spread_in(c, b, low1, high1, 1);
-        }
+        if (now.go(c, b, low, high, i)) mine = spread_in(c, b, low1, high1, 1);
         const int t0 = now.tile(i);
         char(*here)[BYTES] = lds[buf], (*other)[BYTES] = lds[buf ^ 1];
         unsigned long long holes2 = 0;
