@@ -89,6 +89,7 @@ dcn_status dcn_cache_append_mx_dev(dcn_context* ctx, const dcn_pages* pages, con
         DCN_TRY(check_append(ctx, cache, shape, rotary, d_q != nullptr, &r));
         if (!shape->tokens || !shape->sequences) return DCN_OK;
         DCN_TRY(check_append_pointers(ctx, cache, shape, r, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out));
+        if (d_q && d_q == d_q_out) return fail(ctx, DCN_INVALID_ARGUMENT, "q_out is q: an append of this kind does not turn in place");
         DCN_TRY(check_buffers(ctx, pages));
         fill_append(&a, &r, cache, shape, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out);
         DCN_HIP(ctx, dcn::launch_append_mx(cache->dtype, a, mx, r, (hipStream_t)stream));

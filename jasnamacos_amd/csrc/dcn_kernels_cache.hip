@@ -36,145 +36,160 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     return v > b ? v : b;
 }
 
-// The rotation of channels at .. at + 7: channel c turns into x[c] cos + x[partner] sin (with the
-// sine's sign), where it turns at all.
+// The rotation of channels at .. at + 7. A channel is fma(a, u, b v) of its pair's two, a first: u, v are
+// cosine and minus sine for the first of a pair, sine and cosine for the second.
 template <bool WIDE>
 struct Turn8 {
-    float c[8], s[8];
-    int partner[WIDE ? 1 : 8];  // WIDE: of the first channel; -1: passes
-    bool inside;                // WIDE: pairs inside the eight channels
+    float u[8], v[8];
+    int a[WIDE ? 1 : 8], b[WIDE ? 1 : 8];  // where the two are (WIDE: those of the first channel); b < 0: the channel passes
+    bool inside;                           // WIDE: pairs inside the eight channels: u cosines, v sines
 
+    __device__ __forceinline__ void pass(int at) {
+        inside = false;
+#pragma unroll
+        for (int i = 0; i < (WIDE ? 1 : 8); ++i) {
+            a[i] = at + i;
+            b[i] = -1;
+        }
+    }
     __device__ __forceinline__ void set(const RotaryArgs& r, int at, const int32_t* pos) {
-        inside = WIDE && r.interleaved;
+        pass(at);
         if constexpr (WIDE) {
-            partner[0] = at >= 2 * r.pairs ? -1 : (r.interleaved ? at : (at < r.pairs ? at + r.pairs : at - r.pairs));
-            if (partner[0] < 0) return;
-            const int first = r.interleaved ? at >> 1 : (at < r.pairs ? at : at - r.pairs), n = r.interleaved ? 4 : 8;
-            const float sign = at < r.pairs ? -1.f : 1.f;
+            if (at >= 2 * r.pairs) return;
+            inside = r.interleaved;
+            const bool second = !inside && at >= r.pairs;
+            const int first = inside ? at >> 1 : (second ? at - r.pairs : at);
+            if (!inside) {
+                a[0] = first;
+                b[0] = first + r.pairs;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i < n) {
-                    turn(r, pos, first + i, &c[i], &s[i]);
-                    if (!r.interleaved) s[i] *= sign;
-                }
+                if (i < (inside ? 4 : 8)) take(r, pos, first + i, second, inside, i);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int ch = at + i;
-                partner[i] = -1;
                 if (ch >= 2 * r.pairs) continue;
                 const bool second = r.interleaved ? ch & 1 : ch >= r.pairs;
-                turn(r, pos, r.interleaved ? ch >> 1 : (second ? ch - r.pairs : ch), &c[i], &s[i]);
-                if (!second) s[i] = -s[i];
-                partner[i] = r.interleaved ? ch ^ 1 : (second ? ch - r.pairs : ch + r.pairs);
+                const int pair = r.interleaved ? ch >> 1 : (second ? ch - r.pairs : ch);
+                a[i] = r.interleaved ? ch & ~1 : pair;
+                b[i] = r.interleaved ? ch | 1 : pair + r.pairs;
+                take(r, pos, pair, second, false, i);
             }
         }
     }
+    __device__ __forceinline__ void take(const RotaryArgs& r, const int32_t* pos, int pair, bool second, bool plain, int i) {
+        float c, s;
+        turn(r, pos, pair, &c, &s);
+        u[i] = second ? s : c;
+        v[i] = plain ? s : (second ? c : -s);
+    }
 };
 
-// One thread: eight channels of one new token, over the heads of its slice. Slices below q_slices
-// turn queries (a pair of channels by one thread: q_out may be q), the others take keys, then values.
+// Eight values as codes, and their block's scale where the lane is the first of its four.
+template <typename T, int BITS>
+__device__ __forceinline__ void store_codes(const MxArgs& mx, bool value, int64_t row, int dim, int at, float* z) {
+    constexpr uint32_t infinity = 0x7f800000u;
+    const float most = mx_most<T, BITS>();
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = __builtin_bit_cast(uint32_t, z[i]) & 0x7fffffffu;
+        top = bits > top ? bits : top;
+    }
+    top = quad_max(top);
+    // Rare: a block that reads as NaN, or magnitudes past the largest (whose clamped bits are its own then).
+    const bool bad = top >= infinity;
+    const uint32_t limit = __builtin_bit_cast(uint32_t, most);
+    if (__builtin_expect(__any(top > limit), 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = bad ? 0.f : fminf(fmaxf(z[i], -most), most);
+        top = top > limit ? limit : top;
+    }
+    const uint32_t scale = bad ? kMxNan : mx_scale<BITS>(top);
+    const mx_u32x2 codes = mx_encode<BITS>(z, mx_factor(bad ? 127 : scale));
+    uint8_t* to = (value ? mx.v : mx.k) + (row * dim + at) * BITS / 8;
+    if constexpr (BITS == 8)
+        *(mx_u32x2*)to = codes;
+    else
+        *(uint32_t*)to = codes[0];
+    if ((at & 31) == 0) (value ? mx.vs : mx.ks)[row * (dim / 32) + at / 32] = (uint8_t)scale;
+}
+
+// One thread: eight channels of one new token, over the heads blockIdx.y, blockIdx.y + gridDim.y, ...: q's, then
+// k's, then v's. Sines and cosines cost more than a head's copy, so they are taken once for all heads.
 template <typename T, int BITS, bool WIDE>
-__global__ __launch_bounds__(kThreads) void append_mx_kernel(RotaryArgs r, AppendArgs a, MxArgs mx, int64_t first, int q_slices) {
+__global__ __launch_bounds__(kThreads) void append_mx_kernel(RotaryArgs r, AppendArgs a, MxArgs mx, int64_t first) {
     const int chunks = r.dim / 8;
     const int64_t item = first + (int64_t)blockIdx.x * kThreads + threadIdx.x, given = item / chunks;
     const int64_t token = given < a.tokens ? given : a.tokens - 1;
     Target t;
     if (!target_of(a, a.cu_q, token, &t) || given >= a.tokens) return;
-    const int index = (int)(item - given * chunks);
-    const int32_t* pos = r.positions + token * 3;
-    if ((int)blockIdx.y < q_slices) {
-        constexpr int N = WIDE ? 16 / sizeof(T) : 1;
-        const T* from = (const T*)a.q.p + token * a.q.ts;
-        T* to = (T*)a.q_out.p + token * a.q_out.ts;
-        for (int i = index; i < Chunk<T, N>::count(r); i += chunks) {
-            Chunk<T, N> c;
-            c.set(r, i, pos);
-            for (int h = blockIdx.y; h < a.q_heads; h += kBatch * q_slices)
-                c.template apply_all<kBatch>(
-                    [&](int u) { return h + u * q_slices < a.q_heads ? from + (h + u * q_slices) * a.q.hs : nullptr; },
-                    [&](int u) { return h + u * q_slices < a.q_heads ? to + (h + u * q_slices) * a.q_out.hs : nullptr; }, true);
-        }
-        return;
-    }
     const int64_t row0 = t.place < 0 ? -1 : mx_row(a.pages, mx.heads, t.sequence, 0, t.place);
-    if (row0 < 0) return;
-    const int at = index * 8, slice = blockIdx.y - q_slices, step = gridDim.y - q_slices, nk = a.kv_heads;
-    Turn8<WIDE> turn8;
-    if (slice < nk) turn8.set(r, at, pos);
-    for (int h0 = slice; h0 < 2 * nk; h0 += kBatch * step) {
+    const int at = (int)(item - given * chunks) * 8, nq = a.q.p ? a.q_heads : 0, nk = a.kv_heads, step = gridDim.y;
+    const int heads = row0 < 0 ? nq : nq + 2 * nk, turned = row0 < 0 ? nq : nq + nk;
+    if ((int)blockIdx.y >= heads) return;
+    Turn8<WIDE> turns;
+    turns.pass(at);
+    if ((int)blockIdx.y < turned) turns.set(r, at, r.positions + token * 3);
+    for (int h0 = blockIdx.y; h0 < heads; h0 += kBatch * step) {
         T x[kBatch][8], y[kBatch][8];
-        bool turns[kBatch];
+        // The loads of all heads before the first is used.
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const int h = h0 + u * step;
-            turns[u] = h < nk;
-            if (h >= 2 * nk) continue;
-            const T* p = h < nk ? (const T*)a.k.p + token * a.k.ts + h * a.k.hs : (const T*)a.v.p + token * a.v.ts + (h - nk) * a.v.hs;
+            if (h >= heads) continue;
+            const HeadsIn& in = h < nq ? a.q : (h < nq + nk ? a.k : a.v);
+            const T* p = (const T*)in.p + token * in.ts + (h < nq ? h : (h < nq + nk ? h - nq : h - nq - nk)) * in.hs;
+            const bool turn = h < turned;
             if constexpr (WIDE) {
-                Vec<T, 8>::load(p + at, x[u]);
-                turns[u] = turns[u] && turn8.partner[0] >= 0;
-                if (turns[u] && !turn8.inside) Vec<T, 8>::load(p + turn8.partner[0], y[u]);
+                Vec<T, 8>::load(p + (turn ? turns.a[0] : at), x[u]);
+                if (turn && turns.b[0] >= 0) Vec<T, 8>::load(p + turns.b[0], y[u]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x[u][i] = p[at + i];
-                    if (turns[u] && turn8.partner[i] >= 0) y[u][i] = p[turn8.partner[i]];
+                    x[u][i] = p[turn ? turns.a[i] : at + i];
+                    if (turn && turns.b[i] >= 0) y[u][i] = p[turns.b[i]];
                 }
             }
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const int h = h0 + u * step;
-            if (h >= 2 * nk) break;
+            if (h >= heads) break;
             float z[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[i] = widen(x[u][i]);
-            if (turns[u]) {
-                if constexpr (WIDE) {
-                    if (turn8.inside) {
+            if (h < turned) {
+                if (turns.inside) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = z[2 * i], q = z[2 * i + 1];
-                            z[2 * i] = fmaf(p, turn8.c[i], -(q * turn8.s[i]));
-                            z[2 * i + 1] = fmaf(p, turn8.s[i], q * turn8.c[i]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], turn8.c[i], widen(y[u][i]) * turn8.s[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = z[2 * i], q = z[2 * i + 1];
+                        z[2 * i] = fmaf(p, turns.u[i], -(q * turns.v[i]));
+                        z[2 * i + 1] = fmaf(p, turns.v[i], q * turns.u[i]);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (turn8.partner[i] >= 0) z[i] = fmaf(z[i], turn8.c[i], widen(y[u][i]) * turn8.s[i]);
+                        if (turns.b[WIDE ? 0 : i] >= 0) z[i] = fmaf(z[i], turns.u[i], widen(y[u][i]) * turns.v[i]);
                 }
             }
-            constexpr uint32_t infinity = 0x7f800000u;
-            uint32_t top = 0;
-            const float most = mx_most<T, BITS>();
+            if (h < nq) {
+                T out[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                uint32_t bits = __builtin_bit_cast(uint32_t, z[i]) & 0x7fffffffu;
-                if (bits < infinity) {
-                    z[i] = fminf(fmaxf(z[i], -most), most);
-                    bits = __builtin_bit_cast(uint32_t, z[i]) & 0x7fffffffu;
+                for (int i = 0; i < 8; ++i) out[i] = narrow<T>(z[i]);
+                T* to = (T*)a.q_out.p + token * a.q_out.ts + h * a.q_out.hs + at;
+                if constexpr (WIDE) {
+                    Vec<T, 8>::store(to, out);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) to[i] = out[i];
                 }
-                top = bits > top ? bits : top;
+            } else {
+                const bool value = h >= nq + nk;
+                store_codes<T, BITS>(mx, value, row0 + ((int64_t)(value ? h - nq - nk : h - nq) << a.pages.shift), r.dim, at, z);
             }
-            top = quad_max(top);
-            const bool bad = top >= infinity;
-            const uint32_t scale = bad ? kMxNan : mx_scale<BITS>(top);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = bad ? 0.f : z[i];
-            const mx_u32x2 codes = mx_encode<BITS>(z, mx_factor(bad ? 127 : scale));
-            const int64_t row = row0 + ((int64_t)(h < nk ? h : h - nk) << a.pages.shift);
-            uint8_t *to = h < nk ? mx.k : mx.v, *scales = h < nk ? mx.ks : mx.vs;
-            uint8_t* place = to + (row * r.dim + at) * BITS / 8;
-            if constexpr (BITS == 8)
-                *(mx_u32x2*)place = codes;
-            else
-                *(uint32_t*)place = codes[0];
-            if ((index & 3) == 0) scales[row * (r.dim / 32) + (index >> 2)] = (uint8_t)scale;
         }
     }
 }
@@ -226,19 +241,9 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a, MxArgs
 
 template <typename T, int BITS, bool WIDE>
 hipError_t append_mx(const AppendArgs& a, const MxArgs& mx, const RotaryArgs& r, hipStream_t stream) {
-    const int64_t items = a.tokens * (r.dim / 8);
-    const int nq = a.q.p ? a.q_heads : 0, heads = nq + 2 * a.kv_heads;
-    for (int64_t first = 0; first < items; first += kMostThreads) {
-        const int64_t n = items - first < kMostThreads ? items - first : kMostThreads;
-        // Slices for queries and for keys and values by their heads, one each at least.
-        const int slices = (int)head_slices(items, heads);
-        int q = nq ? (int)((int64_t)slices * nq / heads) : 0;
-        if (nq && q < 1) q = 1;
-        const int kv = slices - q < 1 ? 1 : slices - q;
-        append_mx_kernel<T, BITS, WIDE><<<dim3((unsigned)((n + kThreads - 1) / kThreads), q + kv), kThreads, 0, stream>>>(r, a, mx, first, q);
-        if (hipError_t e = hipGetLastError()) return e;
-    }
-    return hipSuccess;
+    return in_launches(a.tokens * (r.dim / 8), (a.q.p ? a.q_heads : 0) + 2 * a.kv_heads, [&](int64_t first, dim3 grid) {
+        append_mx_kernel<T, BITS, WIDE><<<grid, kThreads, 0, stream>>>(r, a, mx, first);
+    });
 }
 
 template <typename T, int BITS>
