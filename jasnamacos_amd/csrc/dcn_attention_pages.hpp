@@ -208,7 +208,7 @@ __device__ __forceinline__ void positions_of(const PagesCall& c, const Block& b,
             return;
         }
     }
-    int first = a.sequences > 64 ? find_sequence(a.cu_q, a.sequences, tok[0]) : 0;
+    int first = a.sequences > 64 ? uniform(find_sequence(a.cu_q, a.sequences, tok[0])) : 0;  // lane 0's, the lowest
     bool found[N] = {}, all;
     do {
         // Lane i has the end of sequence first + i, and its keys.

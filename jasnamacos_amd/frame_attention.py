@@ -244,7 +244,7 @@ class CacheAppend(_Handle):
         """run_dev into a microscaled cache (dcn_cache_append_mx_dev)."""
         if k is None:
             raise DeformConvError(INVALID_ARGUMENT, "k is missing")
-        cache = pages._pack(table, k.dtype, self.ctx.device)
+        cache = _mx(pages)._pack(table, k.dtype, self.ctx.device)
         s, r = self._shape(k, v, table, cu_q, kv_lens, rotary, positions, freq, q, q_out, k.dtype, pages.kv_heads, pages.head_dim)
         status = self._lib.dcn_cache_append_mx_dev(
             self._ctx, cache, s, r, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(positions), _ptr(freq), cu_q.data_ptr(),
@@ -276,6 +276,12 @@ class CacheAppend(_Handle):
         except struct.error:
             raise _outside() from None
         return s, r
+
+
+def _mx(pages) -> "MxPages":
+    if not isinstance(pages, MxPages):
+        raise DeformConvError(INVALID_ARGUMENT, f"pages is {type(pages).__name__}; expected MxPages")
+    return pages
 
 
 class MxPages:
@@ -343,7 +349,7 @@ class CacheRead(_Handle):
         sequence s's kv_lens[s] tokens, rounded to their type."""
         device = self.ctx.device
         tokens, dtype = _rows("k_out", k_out), k_out.dtype
-        packed = pages._pack(table, dtype, device)
+        packed = _mx(pages)._pack(table, dtype, device)
         shape = (tokens, pages.kv_heads, pages.head_dim)
         ks, vs = _heads("k_out", k_out, dtype, shape, device), _heads("v_out", v_out, dtype, shape, device)
         sequences = table.shape[0]
@@ -480,7 +486,7 @@ class FrameAttention(_Handle):
         """paged_dev over a microscaled cache."""
         if q is None:
             raise DeformConvError(INVALID_ARGUMENT, "q is missing")
-        cache = pages._pack(table, q.dtype, self.ctx.device)
+        cache = _mx(pages)._pack(table, q.dtype, self.ctx.device)
         self._pages(q, cache, pages.page_tokens, None, table, cu_q, kv_lens, out, lse, max_q, max_kv, stream)
 
     def shared_dev(self, q, pages, prefix_table, prefix_len, table, cu_q, kv_lens, out, lse=None, max_q=None, max_kv=None,
@@ -495,6 +501,8 @@ class FrameAttention(_Handle):
         if isinstance(pages, MxPages):
             cache, page_tokens = pages._pack(table, q.dtype, device), pages.page_tokens
         else:
+            if not isinstance(pages, (tuple, list)) or len(pages) != 2:
+                raise DeformConvError(INVALID_ARGUMENT, "pages is neither an MxPages nor (k_pages, v_pages)")
             k_pages, v_pages = pages
             sizes = _cache(k_pages, v_pages, table, device)
             if k_pages.dtype is not q.dtype:

@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .deform_conv import HipDeformConv
-from .frame_attention import CacheAppend, FrameAttention, GatedNorm, Rotary
+from .frame_attention import CacheAppend, FrameAttention, GatedNorm, MxPages, Rotary
 
 
 def frame_positions(first: int, frames: int, rows: int, columns: int, device="cuda"):
@@ -173,34 +173,66 @@ class FrameBlocks:
             x, y = _normed(norm, h, x, style @ w["gate"], w["w_post"], w["w_pre"])
         return y
 
-    def stream(self, streams: int, frames: int, page_tokens: int = 16) -> "FrameStream":
-        """Serving state of this many streams of at most `frames` frames."""
-        return FrameStream(self, streams, frames, page_tokens)
+    def stream(self, streams: int, frames: int, page_tokens: int = 16, bits: int = 0) -> "FrameStream":
+        """Serving state of this many streams of at most `frames` frames; bits 8 or 4: their cache is a
+        microscaled one, else one of the blocks' type."""
+        return FrameStream(self, streams, frames, page_tokens, bits)
 
 
 class FrameStream:
     """The paged caches of a set of streams that take one frame each at a time."""
 
-    def __init__(self, blocks: FrameBlocks, streams: int, frames: int, page_tokens: int):
+    def __init__(self, blocks: FrameBlocks, streams: int, frames: int, page_tokens: int, bits: int = 0, begun=None, of: int = 0):
+        """begun, of: stream `of` of another FrameStream, which these continue."""
         if blocks.back < 0:
             raise ValueError("streams need a window with an end: back of zero or more")
         if blocks.frame_tokens % page_tokens:
             raise ValueError(f"{page_tokens} tokens a page do not divide a frame of {blocks.frame_tokens}")
-        self.blocks, self.streams, self.time, self.frames = blocks, streams, 0, frames
+        first = begun.time if begun else 0
+        self.blocks, self.streams, self.time, self.frames = blocks, streams, first, frames
+        self.page_tokens, self.bits = page_tokens, bits
         self.attention, self.norm = blocks.new_handles()
-        per_frame = blocks.frame_tokens // page_tokens
-        kept = min(frames, blocks.sinks + blocks.back + 1)
+        n, per_frame = blocks.frame_tokens, blocks.frame_tokens // page_tokens
         # A frame past the sinks lies where the one that has just left its window was.
-        slot = [f if f < blocks.sinks else blocks.sinks + (f - blocks.sinks) % (blocks.back + 1) for f in range(frames)]
-        pages = (torch.tensor(slot)[:, None] * per_frame + torch.arange(per_frame)).reshape(1, -1)
-        self.table = (pages + kept * per_frame * torch.arange(streams)[:, None]).to(torch.int32).to(blocks.device)
-        shape = (streams * kept * per_frame, page_tokens, blocks.split[1], blocks.head_dim)
-        self.pages = [tuple(torch.empty(shape, dtype=blocks.dtype, device=blocks.device) for _ in range(2))
-                      for _ in blocks.layers]
-        n = blocks.frame_tokens
+        sinks = max(0, min(blocks.sinks, frames) - first)
+        slot = [f if f < sinks else sinks + (f - sinks) % (blocks.back + 1) for f in range(frames - first)]
+        self.kept = min(frames - first, sinks + blocks.back + 1) * per_frame  # pages of a stream
+        shared = begun.kept if begun else 0
+        pages = (torch.tensor(slot, dtype=torch.int64)[:, None] * per_frame + torch.arange(per_frame)).reshape(1, -1)
+        self.table = (shared + pages + self.kept * torch.arange(streams)[:, None]).to(torch.int32).to(blocks.device)
+        self.pages = [self._new_pages(shared + streams * self.kept) for _ in blocks.layers]
+        self.prefix = None  # (table, length) of the frames before these streams' own
+        if begun:
+            for new, old in zip(self.pages, begun.pages):
+                for to, x in zip(self._buffers(new), self._buffers(old)):
+                    to[:shared] = x[of * shared:(of + 1) * shared]
+            table = begun.table[of, :first * per_frame] - of * shared
+            self.prefix = table.contiguous(), torch.tensor([first * n], dtype=torch.int32).to(blocks.device)
         self.cu_q = (torch.arange(streams + 1) * n).to(torch.int32).to(blocks.device)
         self.lens = torch.zeros(streams, dtype=torch.int32, device=blocks.device)
-        self.positions = frame_positions(0, 1, blocks.rows, blocks.columns, blocks.device).repeat(streams, 1)
+        self.positions = frame_positions(first, 1, blocks.rows, blocks.columns, blocks.device).repeat(streams, 1)
+
+    def _new_pages(self, count: int):
+        b = self.blocks
+        if self.bits:
+            return MxPages.zeros(count, self.page_tokens, b.split[1], b.head_dim, self.bits, b.device)
+        shape = (count, self.page_tokens, b.split[1], b.head_dim)
+        return tuple(torch.empty(shape, dtype=b.dtype, device=b.device) for _ in range(2))
+
+    @staticmethod
+    def _buffers(pages):
+        return (pages.k, pages.v, pages.k_scales, pages.v_scales) if isinstance(pages, MxPages) else pages
+
+    def fork(self, copies: int, of: int = 0) -> "FrameStream":
+        """Streams that each continue stream `of` of these in their own way, from its next frame on. Its
+        frames are read once for all of them. Of a stream that was not forked itself."""
+        if self.prefix is not None:
+            raise ValueError("these streams continue another one: fork that one instead")
+        if not self.time:
+            raise ValueError("the streams have had no frame yet")
+        if not 0 <= of < self.streams:
+            raise ValueError(f"there is no stream {of} of {self.streams}")
+        return FrameStream(self.blocks, copies, self.frames, self.page_tokens, self.bits, self, of)
 
     @torch.no_grad()
     def step(self, x, style):
@@ -213,14 +245,25 @@ class FrameStream:
         self.lens += n
         stream = torch.cuda.current_stream(x.device)
         x, y = b._start(x, self.norm)
-        for w, (k_pages, v_pages) in zip(b.layers, self.pages):
+        for w, pages in zip(b.layers, self.pages):
             q, k, v = b.heads(y @ w["qkv"])
             turned = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             out = torch.empty_like(turned)
-            b.append.run_dev(k, v, k_pages, v_pages, self.table, self.cu_q, self.lens, b.rotary, self.positions, b.freq,
-                             q, turned, stream=stream)
-            self.attention.paged_dev(turned, k_pages, v_pages, self.table, self.cu_q, self.lens, out, max_q=n,
-                                     max_kv=self.time * n, stream=stream)
+            turn = (b.rotary, self.positions, b.freq, q, turned)
+            if self.bits:
+                b.append.run_mx_dev(k, v, pages, self.table, self.cu_q, self.lens, *turn, stream=stream)
+            else:
+                b.append.run_dev(k, v, *pages, self.table, self.cu_q, self.lens, *turn, stream=stream)
+            if self.prefix:
+                first = self.prefix[0].shape[0] * self.page_tokens
+                self.attention.shared_dev(turned, pages, *self.prefix, self.table, self.cu_q, self.lens, out, max_q=n,
+                                          max_kv=self.time * n - first, max_prefix=first, stream=stream)
+            elif self.bits:
+                self.attention.paged_mx_dev(turned, pages, self.table, self.cu_q, self.lens, out, max_q=n,
+                                            max_kv=self.time * n, stream=stream)
+            else:
+                self.attention.paged_dev(turned, *pages, self.table, self.cu_q, self.lens, out, max_q=n,
+                                         max_kv=self.time * n, stream=stream)
             x, y = _normed(self.norm, out.flatten(1) @ w["back"], x, style @ w["gate"], w["w_post"], w["w_pre"])
         self.positions[:, 0] += 1
         return y
@@ -235,6 +278,8 @@ def main(argv=None) -> int:
     ap.add_argument("--layers", type=int, default=2)
     ap.add_argument("--back", type=int, default=3)
     ap.add_argument("--steps", type=int, default=5)
+    ap.add_argument("--bits", type=int, choices=(0, 8, 4), default=0, help="of the streamed cache's values (0: the type's own)")
+    ap.add_argument("--forks", type=int, default=0, help="continue the stream in so many ways from its middle on")
     args = ap.parse_args(argv)
     dtype = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[args.dtype]
     blocks = FrameBlocks(HipDeformConv(0), 512, 8, 4, 64, args.layers, args.rows, args.columns, args.back, dtype=dtype)
@@ -256,7 +301,8 @@ def main(argv=None) -> int:
         print(f"step {step}: loss {loss.item():.5f}", flush=True)
     with torch.no_grad():
         whole = blocks.clip(x, style).view(args.frames, blocks.frame_tokens, 512)
-    serving = blocks.stream(1, args.frames, next(p for p in (64, 16, 4, 1) if blocks.frame_tokens % p == 0))
+    page = next(p for p in (64, 16, 4, 1) if blocks.frame_tokens % p == 0)
+    serving = blocks.stream(1, args.frames, page, args.bits)
     frames = x.view(args.frames, blocks.frame_tokens, 512)
     got, times = [], []
     for f, s in zip(frames, style):
@@ -268,8 +314,21 @@ def main(argv=None) -> int:
     got, each = torch.stack(got), sorted(times)[len(times) // 2]
     off = ((got - whole).double().norm() / whole.double().norm()).item()
     print(f"{args.frames} frames streamed, {each * 1e6:.0f} us a frame (median); against the whole clip: relative difference {off:.1e}")
-    # Two orders of the same sums: a few roundings of each block apart.
-    return 0 if off < args.layers * {"f16": 2.0**-8, "bf16": 2.0**-5, "f32": 2.0**-18}[args.dtype] else 1
+    # Two orders of the same sums: a few roundings of each block apart. A code is half a step off at most, 2^-4 of
+    # itself in 8 bits and 2^-2 in 4, of keys and of values.
+    limit = args.layers * ({"f16": 2.0**-8, "bf16": 2.0**-5, "f32": 2.0**-18}[args.dtype] + {0: 0.0, 8: 2.0**-3, 4: 2.0**-1}[args.bits])
+    if args.forks:
+        half = max(1, args.frames // 2)
+        begun = blocks.stream(1, args.frames, page, args.bits)
+        for f, s in zip(frames[:half], style[:half]):
+            begun.step(f.contiguous(), s[None])
+        forks = begun.fork(args.forks)
+        for f, s in zip(frames[half:], style[half:]):  # the first goes on as the stream did, the others with another style
+            last = forks.step(f.repeat(args.forks, 1), torch.cat([s[None], data(args.forks - 1)]))
+        off_fork = ((last[:blocks.frame_tokens] - got[-1]).double().norm() / got[-1].double().norm()).item() if half < args.frames else 0.0
+        print(f"{args.forks} continuations from frame {half}: the first differs from the stream by {off_fork:.1e}")
+        off = max(off, off_fork)
+    return 0 if off < limit else 1
 
 
 if __name__ == "__main__":

@@ -42,6 +42,7 @@ APPEND = [
     ("bf16", 5, 3, 160, 1, [7], [9], (1, 2, 2), True),
     ("f32", 2, 2, 256, 32, [130], [200], (64, 32, 32), False),
     ("bf16", 8, 8, 64, 64, [300, 1], [777, 1], (32, 0, 0), False),
+    ("f16", 1, 1, 32, 8, [0, 1, 3] * 45, [0, 9, 3] * 45, (8, 4, 4), False),  # more sequences than a wave has lanes
 ]
 
 
@@ -64,7 +65,7 @@ def _append_inputs(torch, case, fa, ctx, odd):
     return dtype, q if hq else None, k, v, cu, pos, table, pages, rotary
 
 
-@pytest.mark.parametrize("case", APPEND, ids=lambda c: f"{c[0]}-{c[1]}.{c[2]}x{c[3]}-p{c[4]}-{c[5]}")
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: f"{c[0]}-{c[1]}.{c[2]}x{c[3]}-p{c[4]}-{c[5][:4]}")
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("odd", [0, 1])
 def test_append(fa, gpu_ctx, case, bits, odd):
@@ -250,8 +251,10 @@ ATTEND = [
     ("bf16", 96, 2, 2, 1, [20], [70], 1, 20, 0, 1),
     ("f16", 256, 2, 1, 2, [20], [50], 1, -1, 0, 0),
     ("bf16", 64, 2, 1, 4, [9], [77], 1, -1, 0, 0),  # pages of fewer than eight
+    ("f32", 64, 1, 1, 8, [0, 2, 1] * 50, [3, 2, 20] * 50, 1, -1, 0, 0),  # more sequences than a wave has lanes
+    ("bf16", 128, 8, 2, 16, [0, 2, 1] * 50, [3, 2, 20] * 50, 1, -1, 0, 0),
 ]
-IDS = [f"{c[0]}-d{c[1]}-h{c[2]}.{c[3]}-p{c[4]}-q{'.'.join(map(str, c[5]))}-k{'.'.join(map(str, c[6]))}-f{c[7]}w{c[8]}a{c[9]}s{c[10]}"
+IDS = [f"{c[0]}-d{c[1]}-h{c[2]}.{c[3]}-p{c[4]}-q{'.'.join(map(str, c[5][:5]))}-k{'.'.join(map(str, c[6][:5]))}-f{c[7]}w{c[8]}a{c[9]}s{c[10]}"
        for c in ATTEND]
 
 

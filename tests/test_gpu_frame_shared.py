@@ -219,3 +219,89 @@ def test_runs_without_starts(fa, gpu_ctx, bits):
     whole = torch.cat([pad, out.cpu(), pad[:1]])
     lses = torch.cat([torch.full((2, 4), float("nan")), lse.cpu(), torch.full((1, 4), float("nan"))])
     compare(torch, case, data, whole, lses)
+
+
+# Prefixes long enough, for sequences enough, that they are read once for all of them: the kernels of many rows
+# and of single tokens together, those of 32 rows, one after the other, windows that end inside the prefix.
+LARGE = [
+    ("bf16", 64, 8, 2, 64, 5003, [1] * 64, [1 + 7 * s % 90 for s in range(64)], 1, -1, 0, 0),
+    ("f16", 128, 4, 1, 16, 4100, [1] * 70, [1 + 5 * s % 40 for s in range(70)], 1, -1, 0, 0),
+    ("bf16", 64, 8, 2, 32, 4000, [1] * 66, [1 + 3 * s % 50 for s in range(66)], 1, 3500, 0, 2),
+    ("f16", 128, 8, 8, 8, 2200, [1] * 16, [2 + s for s in range(16)], 1, -1, 0, 0),
+    ("bf16", 128, 6, 2, 16, 3000, [s % 12 for s in range(48)], [s % 12 + s for s in range(48)], 1, -1, -1, 0),
+    ("f16", 64, 4, 4, 64, 6000, [0 if s % 5 == 3 else 1 for s in range(150)], [s % 3 for s in range(150)], 7, 600, 0, 3),
+    ("bf16", 64, 2, 2, 16, 9000, [3] * 40, [s % 7 for s in range(40)], 1, 8000, 0, 0),  # more queries than own keys
+]
+LARGE_IDS = [f"{c[0]}-d{c[1]}-h{c[2]}.{c[3]}-p{c[4]}-P{c[5]}-n{len(c[6])}-w{c[9]}" for c in LARGE]
+
+
+def visible_fast(torch, prefix, nq, nk, frame, back, ahead, sinks):
+    """As visible, in one go."""
+    p = (prefix + nk - nq + torch.arange(nq))[:, None]
+    f, fj = torch.div(p, frame, rounding_mode="floor"), (torch.arange(prefix + nk) // frame)[None]
+    return (p >= 0) & ((fj <= f + ahead) | (ahead < 0)) & ((fj >= f - back) | (back < 0) | (fj < sinks))
+
+
+def test_the_masks_agree():
+    import torch
+
+    for case in CASES:
+        for nq, nk in list(zip(case[6], case[7]))[:3]:
+            assert torch.equal(visible_fast(torch, case[5], nq, nk, *case[8:]), visible(torch, case[5], nq, nk, *case[8:]))
+
+
+@pytest.mark.parametrize("case", LARGE, ids=LARGE_IDS)
+@pytest.mark.parametrize("bits", [0, 8, 4])
+def test_read_once_for_all(fa, gpu_ctx, monkeypatch, case, bits):
+    import torch
+
+    print("case: read once", case, bits, flush=True)
+    monkeypatch.setattr("test_gpu_frame_shared.visible", visible_fast)
+    name, dim, hq, hk, page, prefix, nq, nk, frame, back, ahead, sinks = case
+    if bits == 4 or bits == 8:  # fewer bytes a key: a longer prefix is as many
+        case = case[:5] + (prefix * 16 // (4 * bits) + 1,) + case[6:]
+    data = make(torch, case, bits)
+    op = fa.FrameAttention(gpu_ctx, hq, hk, dim, frame, back, ahead, sinks)
+    compare(torch, case, data, *run(torch, fa, gpu_ctx, case, data, op))
+    got = [run(torch, fa, gpu_ctx, case, data, op) for _ in range(2)]
+    assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(*got)), "not the same bits again"
+
+
+@pytest.mark.parametrize("bits", [0, 8, 4])
+@pytest.mark.parametrize("case", [LARGE[0], LARGE[4], LARGE[5]], ids=lambda c: f"{c[0]}-d{c[1]}-P{c[5]}")
+def test_read_once_and_unseen(fa, gpu_ctx, monkeypatch, case, bits):
+    """NaN in the prefix where only some of the rows look, and in a page that is not there for the others."""
+    import torch
+
+    name, dim, hq, hk, page, prefix, nq, nk, frame, back, ahead, sinks = case
+    print("case: read once, unseen", case, bits, flush=True)
+    case = case[:4] + (page, prefix * 16 // (4 * bits) + 1 if bits else prefix) + case[6:]
+    prefix = case[5]
+    data = make(torch, case, bits)
+    q, cu, prefix_table, table, buffers, _ = data
+    holes = prefix_table.clone()
+    holes[3] = -1
+    gone = [torch.zeros(prefix + n, dtype=torch.bool) for n in nk]
+    for g in gone:
+        g[3 * page:4 * page] = True
+    monkeypatch.setattr("test_gpu_frame_shared.visible", visible_fast)
+    out, lse = run(torch, fa, gpu_ctx, case, data, prefix_table=holes)
+    compare(torch, case, data, out, lse, gone=gone)
+    see = [visible_fast(torch, prefix, nq[s], nk[s], frame, back, ahead, sinks) for s in range(len(nq))]
+    seen = torch.cat([v[:, :prefix] for v in see]).float().mean(0)
+    some = ((seen > 0) & (seen < 1)).nonzero().flatten().tolist()
+    for j in ([some[len(some) // 2]] if some else []) + [prefix - 1, 0]:
+        bad = [b.clone() for b in buffers]
+        at = int(prefix_table[j // page])
+        if bits:
+            bad[3][at, :, j % page, 0] = 255
+        else:
+            bad[1][at, j % page, :, 0] = float("nan")
+        got, got_lse = run(torch, fa, gpu_ctx, case, data, buffers=bad, prefix_table=holes)
+        sees, rows = torch.zeros(len(q), dtype=torch.bool), torch.zeros(len(q), dtype=torch.bool)
+        rows[cu[0]:cu[-1]] = True
+        for s in range(len(nq)):
+            sees[cu[s]:cu[s + 1]] = see[s][:, j]
+        assert torch.equal(got[rows & ~sees], out[rows & ~sees]) and torch.equal(got_lse[rows & ~sees], lse[rows & ~sees])
+        if sees.any():
+            assert torch.isnan(got[sees]).any(-1).all()
