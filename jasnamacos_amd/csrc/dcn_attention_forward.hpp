@@ -35,7 +35,8 @@ struct RowState {
         for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
     }
     // ROWS keys from t0. masked: some row may not see some key (holes: bit per key that is not there).
-    template <int ROWS>
+    // BY_HALF: 32 keys' reads at a time, for kernels whose registers the reads of 64 do not fit.
+    template <int ROWS, bool BY_HALF = false>
     __device__ __forceinline__ void add(const char* kt, const char* vt, int t0, float c, bool masked, unsigned long long holes,
                                         int lane) {
         constexpr int MB = ROWS / 32;
@@ -45,13 +46,19 @@ struct RowState {
         // the softmax: left to itself the compiler keeps two, and each step waits for LDS.
         {
             u32x4 kf[MB][D / 16];
+            if constexpr (!BY_HALF)
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
+                for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) kf[mb][i] = Ti::rows(kt, mb, i, lane);
+                    for (int i = 0; i < D / 16; ++i) kf[mb][i] = Ti::rows(kt, mb, i, lane);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) {
+                if constexpr (BY_HALF) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) kf[mb][i] = Ti::rows(kt, mb, i, lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
 #pragma unroll

@@ -119,7 +119,7 @@ __device__ __forceinline__ void tile_block(const PagesCall& c, unsigned number, 
         if (!idle && !none_sees<ROWS>(mine, t0)) {
             const bool masked = holes || !all_see<ROWS>(mine, t0);
             if (masked || bad) st.sp = b.span(c, at, now.second);
-            st.template add<ROWS>(here[0], here[1], t0, scale, masked, holes, lane);
+            st.template add<ROWS, D == 128 && BITS != 16>(here[0], here[1], t0, scale, masked, holes, lane);
             if (bad) add_bad<T, D, BITS>(p, now.run, pl.kh, st.o, st.sp, t0, ROWS, holes, lane);
         }
         holes = holes1;
@@ -518,18 +518,31 @@ struct PlanOf {
     int parts;
 };
 
-// Few rows, or so few workgroups of 128 rows that 32-row ones with several waves on the keys are done
-// sooner (measured for the 16-bit cache, whose kernels these are). Up to 16 rows take the token kernel.
-// Keys are taken in parts where workgroups would leave the card idle, until about 512 are there (two a
-// CU): one token of 32 streams on 18,001 keys of 8 bits, 32 heads of 128 on 8, in one part 217 us, in
-// two 156, in six 170. Tiles of 128 rows write long parts, so only whole shares are taken: a frame of
-// 3,600 tokens for two streams, 464 workgroups, 340 us in one part and 470 in two. Up to 64 tiles for
-// single tokens go to one workgroup of many waves: a join costs more (997 keys, 8 heads of 64: 10.6 us,
-// in parts 12.7).
-Blocks blocks_of(int dim, int64_t rows, int64_t pairs, int64_t keys, int64_t resident) {
+// Whether more than 32 rows take 32-row workgroups, whose waves share the keys out, and not 128-row ones.
+// The small ones fill the card where there are few (wide: 128-row workgroups) and read the keys four times
+// as often. Measured (us, 128 rows -> 32; 8 query heads on 4):
+//   64 channels, 8 bits: wide 32 at 3,000 keys 29 -> 24; 128 at 12,000 104 -> 94; 256 at 12,000 198 -> 159;
+//     456 at 4,000 100 -> 72 and at 12,000 310 -> 305; 464 at 14,400 344 -> 365; 928 at 4,000 154 -> 135;
+//     2,048 at 12,000 914 -> 924. 4 bits: 256 at 16,000 252 -> 199.
+//   64 channels, 16 bits: 128 at 4,000 47 -> 40 and at 8,000 73 -> 75; 192 at 4,000 74 -> 68; 456 at 4,000
+//     155 -> 187.
+//   128 channels, 8 bits: 128 at 3,000 55 -> 43; 256 at 12,000 274 -> 255; 928 at 4,000 221 -> 242.
+//     4 bits: 64 at 4,000 43 -> 52, 256 at 4,000 112 -> 125. 16 bits: 32 at 4,000 36 -> 37, 128 at 4,000
+//     61 -> 93.
+bool few_of(int dim, int bits, int64_t wide, int64_t keys) {
+    if (dim == 64 && bits) return wide <= 256 || (wide <= 1024 && keys <= 8192);
+    if (dim == 64) return wide <= 256 && keys <= 6144;
+    return bits == 8 && wide <= 256;
+}
+
+// Up to 16 rows take the token kernel. Keys are taken in parts where workgroups would leave the card idle,
+// until about 512 are there (two a CU): one token of 32 streams on 18,001 keys of 8 bits, 32 heads of 128
+// on 8, in one part 217 us, in two 156, in six 170. Tiles of 128 rows write long parts, so only whole
+// shares are taken: a frame of 3,600 tokens for two streams, 464 workgroups, 340 us in one part and 470 in
+// two. Up to 64 tiles for single tokens go to one workgroup of many waves: a join costs more (997 keys,
+// 8 heads of 64: 10.6 us, in parts 12.7).
+Blocks blocks_of(int dim, int64_t rows, int64_t pairs, int64_t keys, int64_t resident, bool few) {
     Blocks b;
-    const int64_t wide = (rows + 127) / 128 * pairs;
-    const bool few = rows <= 32 || (dim == 64 ? wide <= 256 && keys <= 4096 : wide <= 128 && keys <= 2048);
     b.rows = rows <= 16 ? 16 : (few ? 32 : 128);
     const int tile = few ? 32 : 64;
     b.blocks = (int)((rows + b.rows - 1) / b.rows);
@@ -565,8 +578,11 @@ PlanOf plan_of(int dim, int bits, int sequences, int kv_heads, int group, int64_
     const int64_t again = (sequences - 1) * first * kv_heads * dim * (bits ? bits : 16) / 4;
     p.shared = first > 0 && sequences > 1 && rows < 128 && again > kAgain;
     p.both = first > 0 && !p.shared;
-    p.own = blocks_of(dim, rows, pairs, own + (p.both ? first : 0), 512);
-    if (p.shared) p.prefix = blocks_of(dim, q_tokens * group, kv_heads, first, p.own.rows == 16 ? 256 : 512);
+    const int64_t keys = own + (p.both ? first : 0);
+    p.own = blocks_of(dim, rows, pairs, keys, 512, rows <= 32 || few_of(dim, bits, (rows + 127) / 128 * pairs, keys));
+    // The prefix's rows are many and its keys long: 128-row blocks, unless they are few rows.
+    if (p.shared)
+        p.prefix = blocks_of(dim, q_tokens * group, kv_heads, first, p.own.rows == 16 ? 256 : 512, q_tokens * group <= 32);
     p.parts = p.own.splits + (p.shared ? p.prefix.splits : 0);
     return p;
 }
