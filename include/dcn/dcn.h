@@ -881,9 +881,9 @@ typedef struct dcn_prefix {
  * the sequences share a prefix (null: none). With a prefix of P tokens, sequence s's keys are the
  * prefix's and then its own kv_lens[s], of which its table speaks: query i of nq is token
  * P + kv_lens[s] - nq + i, and frames, the window and sinks count from the prefix's first token.
- * shape.max_kv bounds kv_lens. The prefix's keys are read once for the queries of all
- * sequences (heads of 64 and 128 channels in 16 bits; others are read for each query), whose
- * results are then joined in FP32. (width + table_width) * page_tokens must be below 2^31. */
+ * shape.max_kv bounds kv_lens. Where sequences of few queries would read much of the prefix again, its keys
+ * are read once for all of them (heads of 64 and 128 channels in 16 bits) and the results
+ * joined in FP32. (width + table_width) * page_tokens must be below 2^31 - 63. */
 size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages,
                                            const dcn_prefix* prefix);
 dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_pages* pages,

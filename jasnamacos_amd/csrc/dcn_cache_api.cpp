@@ -48,9 +48,10 @@ dcn_status check_call(dcn_context* ctx, const dcn_attention_shape* shape, const 
     p->prefix = p->a.pages;
     p->prefix.table = nullptr;
     p->prefix.width = 0;
+    // The kernels' tiles end up to 64 keys past the last.
+    REQUIRE_SHAPE((!prefix || prefix->width >= 0) && ((int64_t)(prefix ? prefix->width : 0) + c.table_width) * c.page_tokens <= INT32_MAX - 63,
+                  "(prefix width + table_width) * page_tokens must be below 2^31 - 63");
     if (prefix) {
-        REQUIRE_SHAPE(prefix->width >= 0 && ((int64_t)prefix->width + c.table_width) * c.page_tokens <= INT32_MAX,
-                      "(prefix width + table_width) * page_tokens must be below 2^31");
         REQUIRE_SHAPE(prefix->max_tokens >= 0 && prefix->max_tokens <= (int64_t)prefix->width * c.page_tokens,
                       "prefix max_tokens must be 0..width * page_tokens");
         p->prefix.width = prefix->width;

@@ -566,7 +566,7 @@ Blocks blocks_of(int dim, int64_t rows, int64_t pairs, int64_t keys, int64_t res
 // pays for the join of its parts: about 12 us of reading, from the caches. 24 streams on 2,175 keys
 // (51 MB): shared 21 us, each on its own 12; 61 streams on 1,500 keys (180 MB): 21 and 31. Sequences whose
 // rows fill blocks of their own share nothing: a block reads the prefix once either way.
-constexpr int64_t kAgain = 120000000;
+constexpr double kAgain = 120e6;
 
 PlanOf plan_of(int dim, int bits, int sequences, int kv_heads, int group, int64_t q_tokens, int max_q, int max_kv, int max_prefix, int frame,
                int back, int sinks) {
@@ -575,7 +575,7 @@ PlanOf plan_of(int dim, int bits, int sequences, int kv_heads, int group, int64_
     // Keys that a block of rows sees at most.
     const auto keys_of = [&](int64_t tokens, int most) { return attention_keys(most, frame, back, sinks, tokens, 64); };
     const int64_t first = max_prefix ? keys_of(max_q, max_prefix) : 0, own = keys_of(128 / group, max_kv);
-    const int64_t again = (sequences - 1) * first * kv_heads * dim * (bits ? bits : 16) / 4;
+    const double again = (double)(sequences - 1) * first * kv_heads * dim * (bits ? bits : 16) / 4;
     p.shared = first > 0 && sequences > 1 && rows < 128 && again > kAgain;
     p.both = first > 0 && !p.shared;
     const int64_t keys = own + (p.both ? first : 0);

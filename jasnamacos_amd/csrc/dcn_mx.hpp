@@ -115,7 +115,7 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int sequences, i
                           (uint32_t)__builtin_amdgcn_readfirstlane((int)token);
     int low = 0, count = sequences;  // the sequence is in [low, low + count)
     while (count > 1) {
-        const int step = (count + 63) >> 6, at = lane * step;
+        const int step = (int)(((unsigned)count + 63) >> 6), at = lane * step;
         const unsigned long long votes = __ballot(at < count && cu[low + at] <= first);
         const int last = votes ? 63 - __builtin_clzll(votes) : 0;
         low += last * step;

@@ -224,8 +224,9 @@ class FrameStream:
         return (pages.k, pages.v, pages.k_scales, pages.v_scales) if isinstance(pages, MxPages) else pages
 
     def fork(self, copies: int, of: int = 0) -> "FrameStream":
-        """Streams that each continue stream `of` of these in their own way, from its next frame on. Its
-        frames are read once for all of them. Of a stream that was not forked itself."""
+        """Streams that each continue stream `of` of these in their own way, from its next frame on. What is
+        kept of its frames is copied once for all of them, on the current stream, as it is now. Of a stream
+        that was not forked itself."""
         if self.prefix is not None:
             raise ValueError("these streams continue another one: fork that one instead")
         if not self.time:

@@ -68,6 +68,12 @@ def test_calls_that_are_refused_need_no_workspace(bad):
     assert _bytes(**{"width": 4000, "max_kv": 60000, **bad}) == 0
 
 
+def test_keys_that_an_int_counts():
+    """Tiles end up to 63 keys past the last one."""
+    assert _bytes((2**27 - 4 - 4000, 16), width=4000, max_kv=60000) > 0  # 2^31 - 64 tokens
+    assert _bytes((2**27 - 3 - 4000, 16), width=4000, max_kv=60000) == 0
+
+
 def test_calls_without_a_context_are_refused():
     lib = _lib.load()
     p = fa._PAGES.pack(1, 16, 1, 1, 64, 1, 8, 0, 0, 0, 0, 0)
