@@ -305,3 +305,40 @@ def test_read_once_and_unseen(fa, gpu_ctx, monkeypatch, case, bits):
         assert torch.equal(got[rows & ~sees], out[rows & ~sees]) and torch.equal(got_lse[rows & ~sees], lse[rows & ~sees])
         if sees.any():
             assert torch.isnan(got[sees]).any(-1).all()
+
+
+def _lies(torch, how, shape, fill):
+    """A tensor of this shape [tokens][heads][dim] that lies in memory otherwise, and all of that memory."""
+    tokens, heads, dim = shape
+    if how == "heads first":
+        whole = torch.full((heads, tokens, dim), fill)
+        return (lambda w: w.transpose(0, 1)), whole
+    if how == "of a wider row":  # as the queries of a packed row of queries, keys and values
+        return (lambda w: w[:, :heads]), torch.full((tokens, heads + 5, dim), fill)
+    return (lambda w: w[:, :, 1:dim + 1]), torch.full((tokens, heads, dim + 3), fill)  # off 16 bytes: the kernels of any type
+
+
+@pytest.mark.parametrize("how", ["heads first", "of a wider row", "off 16 bytes"])
+@pytest.mark.parametrize("case", [CASES[2], CASES[3], CASES[9]], ids=[IDS[i] for i in (2, 3, 9)])
+@pytest.mark.parametrize("bits", [0, 8, 4])
+def test_strides(fa, gpu_ctx, case, bits, how):
+    import torch
+
+    name, dim, hq, hk, page, prefix, nq, nk, *rest = case
+    data = make(torch, case, bits)
+    q, cu, prefix_table, table, buffers, _ = data
+    view, q_whole = _lies(torch, how, q.shape, 7.0)
+    out_view, out_whole = _lies(torch, how, q.shape, 7.0)
+    q_whole, out_whole = q_whole.to(q.dtype).cuda(), out_whole.to(q.dtype).cuda()
+    view(q_whole).copy_(q)
+    out_view(out_whole).fill_(float("nan"))
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device="cuda")  # noqa: E731
+    on = [b.cuda() for b in buffers]
+    lse = torch.full(q.shape[:2], float("nan"), device="cuda")
+    fa.FrameAttention(gpu_ctx, hq, hk, dim, *rest).shared_dev(
+        view(q_whole), tuple(on) if len(on) == 2 else fa.MxPages(*on), prefix_table.cuda(), i32([prefix]), table.cuda(), i32(cu), i32(nk),
+        out_view(out_whole), lse, max_q=max(nq), max_kv=max(nk), max_prefix=prefix)
+    torch.cuda.synchronize()
+    compare(torch, case, data, out_view(out_whole).cpu(), lse.cpu())
+    out_view(out_whole).fill_(7.0)
+    assert (out_whole == 7.0).all(), "what lies between the rows was written"
