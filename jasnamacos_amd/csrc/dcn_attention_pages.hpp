@@ -393,6 +393,14 @@ struct Stage<T, D, 16, ROWS, WAVES> {
     }
 };
 
+// Of PER_LOAD keys that a wave's lanes take in groups, the key of group i: an order in which sixteen lanes'
+// stores to LDS meet different banks.
+template <int D, int PER_LOAD>
+__device__ __forceinline__ int shuffled(int i) {
+    if constexpr (D == 128) return PER_LOAD == 8 ? (i & 1) << 2 | i >> 1 : (PER_LOAD == 16 ? (i & 3) << 2 | i >> 2 : i);
+    return (i & ~6) | (i & 2) << 1 | (i & 4) >> 1;
+}
+
 // Microscaled pages: through registers. A wave has ROWS / WAVES adjacent keys of the tile; a lane's load
 // is a chunk of one key's codes, and its block's scale.
 template <typename T, int D, int BITS, int ROWS, int WAVES>
@@ -430,17 +438,17 @@ struct Stage {
             row[g] = r;
         }
     }
-    static __device__ __forceinline__ int key(int n, int lane) { return n * kPerLoad + lane / (kBytes / kChunk); }
+    static __device__ __forceinline__ int key(int lane) { return shuffled<D, kPerLoad>(lane / (kBytes / kChunk)); }  // of a load
     static __device__ __forceinline__ int channel(int lane) { return lane % (kBytes / kChunk) * kCodes; }
     __device__ __forceinline__ void load(int lane) {
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int in = key(n, lane);
+            const int in = key(lane);
             int r = row[n * kPerLoad / 8];
 #pragma unroll
             for (int g = 1; g < kPerLoad / 8; ++g) {
                 const int other = row[n * kPerLoad / 8 + g];  // read outside the choice: a choice of places would put them in memory
-                r = lane / (kBytes / kChunk) >> 3 == g ? other : r;
+                r = in >> 3 == g ? other : r;
             }
             const int64_t at = r + (in & 7);
             k[n] = *(const words*)(kp + at * kBytes + lane % (kBytes / kChunk) * kChunk);
@@ -456,7 +464,7 @@ struct Stage {
         unsigned long long rows = 0;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int in = wave * kKeys + key(n, lane), c0 = channel(lane) / 8;
+            const int in = wave * kKeys + n * kPerLoad + key(lane), c0 = channel(lane) / 8;
             const float fk = mx_factor(kf[n]), fv = mx_factor(vf[n]);
             u32x4 x[kGroups], y[kGroups];
             uint32_t two[kCodes];
@@ -643,12 +651,6 @@ struct FewStage {
         }
         return r + (in & 7);
     }
-    // Key of a load of values that lane group i takes: an order in which sixteen lanes' stores to LDS
-    // meet different banks.
-    static __device__ __forceinline__ int shuffled(int i) {
-        if constexpr (D == 128) return kPerLoad == 8 ? (i & 1) << 2 | i >> 1 : (kPerLoad == 16 ? (i & 3) << 2 | i >> 2 : i);
-        return (i & ~6) | (i & 2) << 1 | (i & 4) >> 1;
-    }
     __device__ __forceinline__ void load(const PagesAttention& p, int kh, int lane) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -665,7 +667,7 @@ struct FewStage {
         }
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int in = n * kPerLoad + shuffled(lane / kLanes), c = lane % kLanes;
+            const int in = n * kPerLoad + shuffled<D, kPerLoad>(lane / kLanes), c = lane % kLanes;
             const int64_t at = pool<kPerLoad / 8 ? kPerLoad / 8 : 1>(n * kPerLoad / 8, in);
             if constexpr (BITS == 16) {
                 v[n] = *(const u32x4*)((const char*)p.a.v.p + (at * p.a.v.ts + kh * p.a.v.hs) * 2 + c * 16);
@@ -680,7 +682,7 @@ struct FewStage {
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int in = n * kPerLoad + shuffled(lane / kLanes), c0 = lane % kLanes * kGroups;
+            const int in = n * kPerLoad + shuffled<D, kPerLoad>(lane / kLanes), c0 = lane % kLanes * kGroups;
             u32x4 x[kGroups];
             if constexpr (BITS == 16) {
                 x[0] = v[n];
