@@ -124,6 +124,8 @@ size_t norm_workspace_bytes(int channels, int64_t tokens, int64_t gate_tokens);
 hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream);
 int attention_any_splits(const dcn_attention_shape& s);
 size_t attention_any_workspace(const dcn_attention_shape& s);
+// The parts that workgroups which share a row block's keys leave (any_splits of a row), joined.
+hipError_t launch_attention_any_join(int dtype, const AttentionArgs& a, int splits, hipStream_t stream);
 hipError_t launch_attention_any_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_attention_rows_backward(int dtype, const AttentionArgs& a, hipStream_t stream);
 
@@ -138,6 +140,8 @@ struct PagesAttention {
 hipError_t launch_attention_pages(int dtype, const PagesAttention& p, hipStream_t stream);
 size_t attention_pages_workspace(const dcn_attention_shape& s, int bits, int max_prefix);
 hipError_t launch_attention_pages_any(int dtype, const PagesAttention& p, hipStream_t stream);
+int attention_pages_any_splits(const dcn_attention_shape& s, int max_prefix);
+size_t attention_pages_any_workspace(const dcn_attention_shape& s, int max_prefix);
 
 // Matrix-core kernels: 16-bit heads of 64 and 128 channels (dcn_kernels_attention.hip).
 hipError_t launch_attention_matrix(int dtype, const AttentionArgs& a, hipStream_t stream);

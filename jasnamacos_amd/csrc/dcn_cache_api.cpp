@@ -67,7 +67,8 @@ bool matrix_call(const dcn_attention_shape* s, const dcn_pages* p) {
     return matrix_heads(s) && p->cache.page_tokens >= 8 && rows <= INT32_MAX && s->q_tokens * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
 }
 size_t workspace_of(const dcn_attention_shape* s, const dcn_pages* pages, const dcn::PagesAttention& p) {
-    return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, pages->bits, p.max_prefix) : 0;
+    return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, pages->bits, p.max_prefix)
+                                 : dcn::attention_pages_any_workspace(*s, p.max_prefix);
 }
 
 }  // namespace
@@ -182,6 +183,8 @@ dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* 
         p.prefix.table = shared ? prefix->table : nullptr;
         p.prefix_len = shared ? prefix->tokens : nullptr;
         p.a.workspace = d_workspace;
+        // Tensors that keep a call of the matrix kernels' sizes from them have no room for the others' parts.
+        p.a.any_splits = matrix_call(shape, pages) ? 1 : dcn::attention_pages_any_splits(*shape, p.max_prefix);
         const bool matrix = matrix_call(shape, pages) && matrix_tensor(p.a.q) && matrix_tensor(p.a.out) &&
                             (pages->bits || (matrix_tensor(p.a.k) && matrix_tensor(p.a.v)));
         DCN_HIP(ctx, (matrix ? dcn::launch_attention_pages : dcn::launch_attention_pages_any)(shape->dtype, p, (hipStream_t)stream));

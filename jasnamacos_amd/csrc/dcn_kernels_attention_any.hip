@@ -18,39 +18,13 @@
 // elements, 185 and 377 above 128 (one wave a SIMD, 512 registers). 2,048 causal tokens, 8 FP32 heads
 // of 64: 95 us (45 of the 157 TFLOP/s), of 128: 162 us, of 256: 772 us; FP16 heads of 96: 163 us. One
 // FP32 token on 8,000 paged keys, 8 sequences of 32 heads of 128 on 8: 170 us (3.1 TB/s).
-#include "dcn_attention_mfma.hpp"
+#include "dcn_attention_any.hpp"
 
 namespace dcn {
 namespace fa {
 namespace {
 
-constexpr float kSlack = 8.f;
 constexpr int kRowsWg = 32, kTile = 32;
-
-// Channels at .. at + 3 of a row, as FP32; zeros past its end. Loads without a branch around
-// them, which would wait for each before the next.
-template <typename T, bool VEC>
-__device__ __forceinline__ f32x4 load4(const T* row, int at, int dim) {
-    f32x4 v;
-    if constexpr (VEC) {
-        typedef T four __attribute__((ext_vector_type(4)));
-        const four t = *(const four*)(row + (at < dim ? at : dim - 4));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = at < dim ? widen((T)t[i]) : 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float t = widen(row[at + i < dim ? at + i : dim - 1]);
-            v[i] = at + i < dim ? t : 0.f;
-        }
-    }
-    return v;
-}
-__device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ bool finite32(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) != 0x7f800000u; }
-
-// FP32 values of a part: the channels, then maximum and sum.
-__device__ __host__ inline int part_line(int dim) { return (dim + 3) / 4 * 4 + 4; }
 
 // VEC: rows of four-element alignment and heads of whole fours. NB: blocks of 32 channels.
 template <typename T, int NB, bool PAGED, bool VEC, int WAVES>
@@ -468,10 +442,11 @@ __global__ __launch_bounds__(kThreads, NB == 2 ? 2 : 1) void attention_any_grad_
     if constexpr (KEYS) join(sum2, a.dv, 1.f);
 }
 
-// Whether rows of a tensor lie on multiples of four elements.
 template <typename T>
-bool fours(const HeadsIn& h) {
-    return (uintptr_t)h.p % (4 * sizeof(T)) == 0 && h.ts % 4 == 0 && h.hs % 4 == 0;
+hipError_t join(const AttentionArgs& a, int splits, hipStream_t stream) {
+    const int64_t rows = (int64_t)a.max_q * a.q_heads;
+    attention_any_join_kernel<T><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, splits);
+    return hipGetLastError();
 }
 
 template <typename T, int NB, bool PAGED, bool VEC>
@@ -487,10 +462,7 @@ hipError_t run(const AttentionArgs& a, hipStream_t stream) {
     else
         attention_any_kernel<T, NB, PAGED, VEC, 4><<<map.grid, 256, 0, stream>>>(a, map, splits);
     if (hipError_t e = hipGetLastError()) return e;
-    if (splits == 1) return hipSuccess;
-    const int64_t rows = (int64_t)a.max_q * a.q_heads;
-    attention_any_join_kernel<T><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, splits);
-    return hipGetLastError();
+    return splits == 1 ? hipSuccess : join<T>(a, splits, stream);
 }
 template <typename T, int NB, bool PAGED>
 hipError_t by_rows(const AttentionArgs& a, hipStream_t stream) {
@@ -556,6 +528,12 @@ int attention_any_splits(const dcn_attention_shape& s) {
 size_t attention_any_workspace(const dcn_attention_shape& s) {
     const int splits = attention_any_splits(s);
     return splits == 1 ? 0 : (size_t)s.q_tokens * s.q_heads * splits * fa::part_line(s.head_dim) * sizeof(float);
+}
+
+hipError_t launch_attention_any_join(int dtype, const AttentionArgs& a, int splits, hipStream_t stream) {
+    if (dtype == DCN_DTYPE_F16) return fa::join<_Float16>(a, splits, stream);
+    if (dtype == DCN_DTYPE_BF16) return fa::join<fa::bf16>(a, splits, stream);
+    return fa::join<float>(a, splits, stream);
 }
 
 hipError_t launch_attention_any(int dtype, const AttentionArgs& a, hipStream_t stream) {

@@ -57,7 +57,10 @@ def test_workspace_bytes():
     assert shared > 0 and shared % (64 * 8 * (64 + 4) * 4) == 0
     assert _bytes((1000, 0), **many) == 0  # no prefix after all
     assert _bytes((1000, 16000), bits=0, **many) == shared or _bytes((1000, 16000), bits=0, **many) > 0
-    assert _bytes(head_dim=96, dim=96, width=4000, max_kv=60000) == 0  # a kernel without parts
+    other = _bytes(head_dim=96, dim=96, width=4000, max_kv=60000)  # the kernel of any type
+    assert other > 0 and other % (8 * (96 + 4) * 4) == 0
+    assert _bytes((1000, 16000), head_dim=96, dim=96, max_kv=16) > 0  # parts of the prefix
+    assert _bytes(head_dim=96, dim=96, sequences=64, q_tokens=64, width=4000, max_kv=60000) == 0  # workgroups for every CU
 
 
 @pytest.mark.parametrize("bad", [
