@@ -21,6 +21,12 @@ template <int D>
 constexpr int tile_bytes() {
     return 2 * 2 * 64 * D * 2;
 }
+// 128 rows, 32 a wave, over tiles of 64 keys in LDS that the four waves fill together: the 16-bit kernels'
+// loop, with codes loaded two tiles ahead in registers and stored one ahead. A frame of 3,600 tokens for two
+// streams on 14,400 keys of 8 bits, 8 heads of 64: 340 us, 546 TFLOP/s; the vector units are busy 45 % of the
+// time, the matrix units 20 %: at 64 channels the softmax is longer than its products, and two waves a SIMD do not
+// hide all of its latencies (three spill: 486 us). 128 channels in microscaled pages leave no registers
+// for the reads of 64 keys at once: they are taken by half (64 streams on a shared prefix: 55 -> 52 us).
 template <typename T, int D, int BITS>
 __device__ __forceinline__ void tile_block(const PagesCall& c, unsigned number, char* memory, FoundRows& found) {
     constexpr int ROWS = 64, BYTES = ROWS * D * 2;
@@ -153,7 +159,12 @@ __global__ __launch_bounds__(kThreads, 2) void pages_tile_kernel(PagesCall c) {
     tile_block<T, D, BITS>(c, blockIdx.x, lds, found);
 }
 
-// LDS of a wave of the few kernel: pages of the type have two tiles, one in flight.
+// 32 rows, all of them for each wave, whose waves take tiles of 32 keys in turn without a barrier, each through
+// LDS of its own, until they are joined. It fills the card where there are few rows, and reads the keys
+// for every 32 of them: bound by the caches, about 12 TB/s. 8 continuations of a clip, a frame of 256
+// tokens each, 8 FP16 heads of 64 on 4, 4,352 keys: 47 us (128 rows in parts: 57).
+//
+// LDS of a wave: pages of the type have two tiles, one in flight.
 template <int D, int BITS>
 constexpr int few_wave_bytes() {
     return (BITS == 16 ? 4 : 2) * 32 * D * 2;
@@ -288,7 +299,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || BITS != 16 ? 2 : 1) void 
     if (part == 0) store_sums<D>(p.a, pl, to_row.index, m, sum, kLift<T>);
 }
 
-// LDS of the token kernel: each wave's values, then the join.
+// 16 rows, for single tokens: as above, with v_mfma_f32_16x16x32 and keys straight from memory. Loads of the
+// next tile are in flight behind the products of this one. 32 streams' tokens on up to 18,001 keys, 32 heads of 128
+// on 8: 156 us in 8 bits (5.3 TB/s; 32 rows a block 217), 100 in 4 (4.3 TB/s). One token on 997 keys, 8 heads of 64:
+// 10.6 us, a chain of latencies (16 waves; four and a join 12.7).
+//
+// LDS: each wave's values, then the join.
 template <int D, int WAVES>
 constexpr int token_bytes() {
     constexpr int values = WAVES * 32 * D * 2, join = WAVES * 16 * (D + 4) * 4;
@@ -428,7 +444,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 2) void pages_token_k
 }
 
 // The prefix for many rows and the sequences' own keys for single tokens in one launch: the first
-// is bound by the products, the second by memory, and a CU takes a workgroup of each.
+// is bound by the products, the second by memory, and a CU takes a workgroup of each. 64 streams' tokens
+// on a prefix of 14,400 and up to 901 of their own, 32 heads of 128 on 8: 68 us with the join (in two launches 80;
+// 3.3 TB/s, the prefix read once), in 8 bits 52. Workgroups for the prefix: 128 78 us, 192 68, 256 68, 320 73, 512 80; in
+// 8 bits 77, 58, 52, 61, 59.
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(kThreads, 2) void pages_mixed_kernel(PagesCall c) {
     __shared__ __attribute__((aligned(1024))) char lds[tile_bytes<D>()];
@@ -447,7 +466,7 @@ __global__ __launch_bounds__(kThreads, 2) void pages_mixed_kernel(PagesCall c) {
 
 // The parts (64 at most) of a row and head, by PER waves: lane s of each has part s's maximum and sum;
 // the waves take the parts' outputs in turn and are added in order. A part that saw nothing has
-// written no output.
+// written no output. Bound by latency: 2,048 rows of 128 channels in 16 parts 6 us, in two 4.8.
 template <typename T, int D, int PER>
 __global__ __launch_bounds__(kThreads) void pages_join_kernel(AttentionArgs a, int parts) {
     typedef float vec __attribute__((ext_vector_type(D / 64)));

