@@ -546,12 +546,13 @@ struct PlanOf {
 //   64 channels, 16 bits: 128 at 4,000 47 -> 40 and at 8,000 73 -> 75; 192 at 4,000 74 -> 68; 456 at 4,000
 //     155 -> 187.
 //   128 channels, 8 bits: 128 at 3,000 55 -> 43; 256 at 12,000 274 -> 255; 928 at 4,000 221 -> 242.
-//     4 bits: 64 at 4,000 43 -> 52, 256 at 4,000 112 -> 125. 16 bits: 32 at 4,000 36 -> 37, 128 at 4,000
-//     61 -> 93.
+//     4 bits: 4 at 300 15 -> 11; 64 at 700 28 -> 20, at 2,000 32 -> 34, at 4,000 43 -> 52; 128 at 1,200 35 -> 22, at
+//     2,000 45 -> 40; 256 at 700 31 -> 32, at 4,000 112 -> 125. 16 bits: 4 at 300 18 -> 12; 64 at 600 27 -> 27; 128 at
+//     600 27 -> 24, at 2,000 44 -> 52; 256 at 600 28 -> 47.
 bool few_of(int dim, int bits, int64_t wide, int64_t keys) {
     if (dim == 64 && bits) return wide <= 256 || (wide <= 1024 && keys <= 8192);
     if (dim == 64) return wide <= 256 && keys <= 6144;
-    return bits == 8 && wide <= 256;
+    return bits == 8 ? wide <= 256 : wide <= 128 && keys <= (bits ? 2048 : 1024);
 }
 
 // Up to 16 rows take the token kernel. Keys are taken in parts where workgroups would leave the card idle,
