@@ -49,7 +49,7 @@ __device__ __forceinline__ Run kv_run_of(const AttentionArgs& a, int s) {
 struct Span {
     int sink, lo, hi;
 };
-__device__ __forceinline__ Span span_of(const AttentionArgs& a, int p, int n) {
+__host__ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int p, int n) {
     if (p < 0) return Span{0, 0, 0};
     const int64_t f = p / a.frame, fr = a.frame;
     int64_t hi = a.ahead < 0 ? n : (f + a.ahead + 1) * fr;

@@ -14,7 +14,7 @@ namespace {
 struct Divide {
     uint32_t factor;
     int shift;
-    __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * factor) >> shift); }
+    __host__ __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * factor) >> shift); }
 };
 inline Divide divide_by(int d) {
     int bits = 0;
@@ -29,7 +29,7 @@ struct Window {
     int frame, sinks;
     uint32_t ahead, back;
 
-    __device__ __forceinline__ Span at(int p, int n) const {
+    __host__ __device__ __forceinline__ Span at(int p, int n) const {
         if (p < 0) return Span{0, 0, 0};
         const uint32_t start = by_frame(p) * frame, end = start + ahead;
         const int hi = end < (uint32_t)n ? (int)end : n;
@@ -39,7 +39,7 @@ struct Window {
     }
 };
 inline Window window_of(const AttentionArgs& a) {
-    const auto tokens = [&](int64_t frames) { return frames < INT32_MAX / a.frame ? (uint32_t)(frames * a.frame) : (uint32_t)INT32_MAX; };
+    const auto tokens = [&](int64_t frames) { return frames <= INT32_MAX / a.frame ? (uint32_t)(frames * a.frame) : (uint32_t)INT32_MAX; };
     return Window{divide_by(a.frame), a.frame, (int)tokens(a.sinks), a.ahead < 0 ? (uint32_t)INT32_MAX : tokens((int64_t)a.ahead + 1),
                   a.back < 0 ? (uint32_t)INT32_MAX : tokens(a.back)};
 }
