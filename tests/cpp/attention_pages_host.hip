@@ -2,16 +2,19 @@
 // Reads a question a line from stdin, answers each with a line:
 //   divide D N                               N / D as the kernels divide
 //   window FRAME AHEAD BACK SINKS P N        what position P sees of N keys: sink lo hi of Window::at, then of span_of
+//   plan DIM BITS SEQUENCES KV_HEADS GROUP Q_TOKENS MAX_Q MAX_KV MAX_PREFIX FRAME BACK SINKS
+//                                            shared both parts; rows waves blocks splits of own; of the prefix
 #include <cstdio>
 #include <cstring>
 
 #include "dcn_attention_pages.hpp"
+#include "dcn_attention_plan.hpp"
 
 int main() {
     using namespace dcn;
     char what[16];
     while (std::scanf("%15s", what) == 1) {
-        long long x[8] = {};
+        long long x[12] = {};
         const auto read = [&](int n) {
             for (int i = 0; i < n; ++i)
                 if (std::scanf("%lld", &x[i]) != 1) return false;
@@ -27,6 +30,11 @@ int main() {
             a.sinks = (int)x[3];
             const fa::Span s = fa::window_of(a).at((int)x[4], (int)x[5]), t = fa::span_of(a, (int)x[4], (int)x[5]);
             std::printf("%d %d %d %d %d %d\n", s.sink, s.lo, s.hi, t.sink, t.lo, t.hi);
+        } else if (!std::strcmp(what, "plan") && read(12)) {
+            const fa::PlanOf p = fa::plan_of((int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)x[4], x[5], (int)x[6], (int)x[7], (int)x[8], (int)x[9],
+                                             (int)x[10], (int)x[11]);
+            std::printf("%d %d %d %d %d %d %d %d %d %d %d\n", p.shared, p.both, p.parts, p.own.rows, p.own.waves, p.own.blocks, p.own.splits,
+                        p.prefix.rows, p.prefix.waves, p.prefix.blocks, p.prefix.splits);
         } else {
             return 2;
         }

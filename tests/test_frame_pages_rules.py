@@ -1,14 +1,17 @@
-"""What the kernels of attention over pages compute of positions, on the host: the library's own functions,
-compiled into a small program."""
+"""What the kernels of attention over pages compute of positions, and how a call is shared out among them, on the
+host: the library's own functions, compiled into a small program."""
 from __future__ import annotations
 
+import random
 import shutil
 import subprocess
 from pathlib import Path
 
 import pytest
 
+from jasnamacos_amd import _lib
 from jasnamacos_amd import build as dcn_build
+from jasnamacos_amd import frame_attention as fa
 
 LAST = 2**31 - 1
 SOURCE = Path(__file__).resolve().parent / "cpp" / "attention_pages_host.hip"
@@ -59,3 +62,42 @@ def test_windows_next_to_the_largest_numbers(ask):
         want = span(*case)
         assert got[3:] == want, ("any type", case, got, want)
         assert got[:3] == want, (case, got, want)
+
+
+def test_division_by_sizes(ask):
+    """0 .. 2^31 - 1 by any number from 1 on, at multiples, next to them and at random."""
+    r = random.Random(1)
+    sizes = {1, 2, 3, 5, 6, 7, 29, 64, 100, 255, 256, 3600, 65535, 65536, 65537, 2**30 - 1, 2**30, 2**30 + 1, LAST - 1, LAST}
+    sizes |= {r.randint(1, 2**r.randint(1, 31) - 1) for _ in range(200)}
+    pairs = []
+    for d in sorted(sizes):
+        for q in {0, 1, 2, LAST // d - 1, LAST // d, r.randint(0, LAST // d), r.randint(0, LAST // d)}:
+            pairs += [(d, n) for n in (q * d - 1, q * d, q * d + 1, r.randint(0, LAST), LAST) if 0 <= n <= LAST]
+    for (d, n), got in zip(pairs, ask(f"divide {d} {n}" for d, n in pairs)):
+        assert got == [n // d], (n, d)
+
+
+class Plan:
+    def __init__(self, values):
+        self.shared, self.both, self.parts, self.rows, self.waves, self.blocks, self.splits = values[:7]
+        self.prefix_rows, self.prefix_waves, self.prefix_blocks, self.prefix_splits = values[7:]
+
+
+def plan(ask, dim, bits, hq, hk, nq, nk, prefix, frame, back, sinks, q_tokens):
+    """How a call with these lengths as its bounds is shared out."""
+    max_q = min(max(nq), q_tokens)
+    return Plan(ask([f"plan {dim} {bits} {len(nq)} {hk} {hq // hk} {q_tokens} {max_q} {max(nk)} {prefix} {frame} {back} {sinks}"])[0])
+
+
+@pytest.mark.parametrize("bits", [0, 8, 4])
+@pytest.mark.parametrize("sequences,keys,prefix", [(64, 16, 16000), (64, 16, 60000), (1, 60000, 0), (1, 60000, 900), (300, 200, 500)])
+def test_workspaces_have_room_for_the_parts(ask, bits, sequences, keys, prefix):
+    """FP32 of each part of a row: its channels, a maximum and a sum, in a line of four more."""
+    lib = _lib.load()
+    s = fa._ATTENTION.pack(1, sequences, 8, 8, 64, 1, -1, 0, 0, 1, keys, 1.0, sequences, 0, *[0] * 16)
+    p = fa._PAGES.pack(64, 16, 4000, 8, 64, 1, bits, 0, 0, 0, 0, 0)
+    size = lib.dcn_attention_pages_workspace_bytes(s, p, fa._PREFIX.pack(4000, prefix, 0, 0))
+    got = plan(ask, 64, bits, 8, 8, [1] * sequences, [keys], prefix, 1, -1, 0, sequences)
+    assert size == (0 if got.parts == 1 else sequences * 8 * got.parts * (64 + 4) * 4)
+    assert got.shared == ((sequences - 1) * prefix * 8 * 64 * (bits or 16) / 4 > 120e6)
+    assert got.parts == got.splits + got.shared * got.prefix_splits and (got.parts > 1 or not got.shared)
