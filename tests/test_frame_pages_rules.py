@@ -12,6 +12,7 @@ import pytest
 from jasnamacos_amd import _lib
 from jasnamacos_amd import build as dcn_build
 from jasnamacos_amd import frame_attention as fa
+from frame_pages_cases import BITS, READ_ONCE, TILES, name_of, rows_of, scaled
 
 LAST = 2**31 - 1
 SOURCE = Path(__file__).resolve().parent / "cpp" / "attention_pages_host.hip"
@@ -101,3 +102,22 @@ def test_workspaces_have_room_for_the_parts(ask, bits, sequences, keys, prefix):
     assert size == (0 if got.parts == 1 else sequences * 8 * got.parts * (64 + 4) * 4)
     assert got.shared == ((sequences - 1) * prefix * 8 * 64 * (bits or 16) / 4 > 120e6)
     assert got.parts == got.splits + got.shared * got.prefix_splits and (got.parts > 1 or not got.shared)
+
+
+def plan_of(ask, case, bits):
+    name, dim, hq, hk, page, prefix, nq, nk, frame, back, ahead, sinks = case
+    return plan(ask, dim, bits, hq, hk, nq, nk, prefix, frame, back, sinks, rows_of(case))
+
+
+@pytest.mark.parametrize("bits", BITS)
+def test_cases_that_are_read_once(ask, bits):
+    for (prefix_rows, rows), case in READ_ONCE:
+        got = plan_of(ask, scaled(case, bits), bits)
+        assert (got.shared, got.prefix_rows, got.rows) == (1, prefix_rows, rows), (name_of(case), vars(got))
+
+
+@pytest.mark.parametrize("bits", BITS)
+def test_cases_of_128_rows(ask, bits):
+    for case in TILES:
+        got = plan_of(ask, case, bits)
+        assert (got.shared, got.both, got.rows) == (0, case[5] > 0, 128), (name_of(case), vars(got))
