@@ -883,7 +883,8 @@ typedef struct dcn_prefix {
  * P + kv_lens[s] - nq + i, and frames, the window and sinks count from the prefix's first token.
  * shape.max_kv bounds kv_lens. Where sequences of few queries would read much of the prefix again, its keys
  * are read once for all of them (heads of 64 and 128 channels in 16 bits) and the results
- * joined in FP32. (width + table_width) * page_tokens must be below 2^31 - 63. */
+ * joined in FP32. (width + table_width) * page_tokens must be below 2^31 - 63. A launch has a workgroup for each
+ * 16 to 128 rows, below 2^24 in all as above. */
 size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages,
                                            const dcn_prefix* prefix);
 dcn_status dcn_attention_pages_dev(dcn_context* ctx, const dcn_attention_shape* shape, const dcn_pages* pages,

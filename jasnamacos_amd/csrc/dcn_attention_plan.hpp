@@ -88,5 +88,14 @@ inline PlanOf plan_of(int dim, int bits, int sequences, int kv_heads, int group,
     return p;
 }
 
+// Whether every launch of a plan has fewer than 2^32 threads along x: these workgroups over the prefix and over the
+// sequences' own keys (in one launch or two), and the join of `rows` rows and heads of a sequence.
+constexpr int kJoinByRow = 8;  // up to so many parts a wave joins a row, else a workgroup does
+inline bool launches_fit(const PlanOf& p, unsigned prefix_grid, unsigned own_grid, int64_t rows) {
+    const int64_t most = (INT64_C(1) << 32) / 64;  // waves
+    return (int64_t)prefix_grid * p.prefix.waves + (int64_t)own_grid * p.own.waves < most &&
+           (p.parts == 1 || rows < (p.parts <= kJoinByRow ? most - 4 : most / 4));
+}
+
 }  // namespace fa
 }  // namespace dcn

@@ -557,7 +557,7 @@ hipError_t run_blocks(const PagesCall& c, const Blocks& b, hipStream_t stream) {
 template <typename T, int D>
 hipError_t join(const AttentionArgs& a, int parts, hipStream_t stream) {
     const int64_t rows = (int64_t)a.max_q * a.q_heads;
-    if (parts <= 8)
+    if (parts <= kJoinByRow)
         pages_join_kernel<T, D, 1><<<dim3((unsigned)((rows + kWaves - 1) / kWaves), 1, a.sequences), kThreads, 0, stream>>>(a, parts);
     else
         pages_join_kernel<T, D, kWaves><<<dim3((unsigned)rows, 1, a.sequences), kThreads, 0, stream>>>(a, parts);
@@ -577,9 +577,7 @@ hipError_t run(const PagesAttention& p, const PlanOf& plan, hipStream_t stream) 
     if (!pages_grid(plan.own.blocks, plan.own.splits, plan.own.per, a.kv_heads, a.sequences, &c.own)) return hipErrorInvalidConfiguration;
     if (plan.shared && !pages_grid(plan.prefix.blocks, plan.prefix.splits, plan.prefix.per, a.kv_heads, 1, &c.prefix))
         return hipErrorInvalidConfiguration;
-    // Every launch has fewer than 2^32 threads along x.
-    const int64_t rows = (int64_t)a.max_q * a.q_heads, most = (INT64_C(1) << 32) / 1024;
-    if ((int64_t)c.prefix.grid + c.own.grid >= most || (plan.parts > 1 && rows >= most)) return hipErrorInvalidConfiguration;
+    if (!launches_fit(plan, c.prefix.grid, c.own.grid, (int64_t)a.max_q * a.q_heads)) return hipErrorInvalidConfiguration;
     if (plan.shared && plan.prefix.rows == 128 && plan.own.rows == 16) {
         pages_mixed_kernel<T, D, BITS><<<c.prefix.grid + c.own.grid, kThreads, 0, stream>>>(c);
         if (hipError_t e = hipGetLastError()) return e;

@@ -3,7 +3,8 @@
 //   divide D N                               N / D as the kernels divide
 //   window FRAME AHEAD BACK SINKS P N        what position P sees of N keys: sink lo hi of Window::at, then of span_of
 //   plan DIM BITS SEQUENCES KV_HEADS GROUP Q_TOKENS MAX_Q MAX_KV MAX_PREFIX FRAME BACK SINKS
-//                                            shared both parts; rows waves blocks splits of own; of the prefix
+//                                            shared both parts; rows waves blocks splits of own; of the prefix;
+//                                            workgroups of the prefix, own; whether the launches fit
 #include <cstdio>
 #include <cstring>
 
@@ -33,8 +34,12 @@ int main() {
         } else if (!std::strcmp(what, "plan") && read(12)) {
             const fa::PlanOf p = fa::plan_of((int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)x[4], x[5], (int)x[6], (int)x[7], (int)x[8], (int)x[9],
                                              (int)x[10], (int)x[11]);
-            std::printf("%d %d %d %d %d %d %d %d %d %d %d\n", p.shared, p.both, p.parts, p.own.rows, p.own.waves, p.own.blocks, p.own.splits,
-                        p.prefix.rows, p.prefix.waves, p.prefix.blocks, p.prefix.splits);
+            fa::PagesGrid own{}, prefix{};
+            const bool grids = fa::pages_grid(p.own.blocks, p.own.splits, p.own.per, (int)x[3], x[2], &own) &&
+                               (!p.shared || fa::pages_grid(p.prefix.blocks, p.prefix.splits, p.prefix.per, (int)x[3], 1, &prefix));
+            std::printf("%d %d %d %d %d %d %d %d %d %d %d %u %u %d\n", p.shared, p.both, p.parts, p.own.rows, p.own.waves, p.own.blocks, p.own.splits,
+                        p.prefix.rows, p.prefix.waves, p.prefix.blocks, p.prefix.splits, prefix.grid, own.grid,
+                        grids && fa::launches_fit(p, prefix.grid, own.grid, x[6] * x[3] * x[4]));
         } else {
             return 2;
         }

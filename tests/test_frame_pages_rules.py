@@ -81,7 +81,7 @@ def test_division_by_sizes(ask):
 class Plan:
     def __init__(self, values):
         self.shared, self.both, self.parts, self.rows, self.waves, self.blocks, self.splits = values[:7]
-        self.prefix_rows, self.prefix_waves, self.prefix_blocks, self.prefix_splits = values[7:]
+        self.prefix_rows, self.prefix_waves, self.prefix_blocks, self.prefix_splits, self.prefix_grid, self.grid, self.fits = values[7:]
 
 
 def plan(ask, dim, bits, hq, hk, nq, nk, prefix, frame, back, sinks, q_tokens):
@@ -121,3 +121,21 @@ def test_cases_of_128_rows(ask, bits):
     for case in TILES:
         got = plan_of(ask, case, bits)
         assert (got.shared, got.both, got.rows) == (0, case[5] > 0, 128), (name_of(case), vars(got))
+
+
+def test_launches_of_less_than_2_24_workgroups(ask):
+    """They fit, whatever the threads of a workgroup, as every launch has fewer than 2^32 threads; larger ones do not."""
+    for dim in (64, 128):
+        for bits in BITS:
+            for sequences, heads, new in ((65535, 65, 1), (65535, 255, 1), (65535, 250, 17), (60000, 2, 16000), (1, 3, 600_000_000)):
+                got = plan(ask, dim, bits, heads, heads, [new] * sequences, [50], 0, 1, -1, 0, sequences * new)
+                assert got.grid < 2**24 and got.grid * 64 * got.waves < 2**32 and got.fits, (dim, bits, sequences, heads, new, vars(got))
+            for sequences, heads, new in ((65535, 258, 1), (65535, 65535, 1), (65535, 100, 3000)):
+                assert not plan(ask, dim, bits, heads, heads, [new] * sequences, [50], 0, 1, -1, 0, sequences * new).fits
+            # A prefix that is read once, and the join of its parts.
+            for sequences, heads, fits in ((60, 65535, 1), (16000, 500, 1), (65535, 65535, 0)):
+                got = plan(ask, dim, bits, heads, heads, [1] * sequences, [50], 4000, 1, -1, 0, sequences)
+                assert got.shared and got.fits == fits, (dim, bits, sequences, heads, vars(got))
+            for heads, queries, fits in ((50000, 120, 1), (65535, 127, 1)):  # rows to join: up to 2^23
+                got = plan(ask, dim, bits, heads, heads, [queries] * 2, [50], 100, 1, -1, 0, 2 * queries)
+                assert got.shared and got.fits == fits and got.parts > 1, (dim, bits, heads, vars(got))
