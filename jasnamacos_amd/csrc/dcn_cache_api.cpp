@@ -63,8 +63,10 @@ dcn_status check_call(dcn_context* ctx, const dcn_attention_shape* shape, const 
 // Whether the matrix kernels take a call of these sizes: as in the paged call, and rows of all sequences
 // and of the pool that an int counts.
 bool matrix_call(const dcn_attention_shape* s, const dcn_pages* p) {
-    const int64_t rows = (int64_t)p->cache.pages * p->cache.page_tokens * (p->bits ? p->cache.kv_heads : 1);
-    return matrix_heads(s) && p->cache.page_tokens >= 8 && rows <= INT32_MAX && s->q_tokens * (s->q_heads / s->kv_heads) < INT32_MAX - 256;
+    // By division: the products of sizes that no memory has may pass 64 bits.
+    return matrix_heads(s) && matrix_pool(&p->cache) &&
+           (!p->bits || (int64_t)p->cache.pages * p->cache.page_tokens <= INT32_MAX / p->cache.kv_heads) &&
+           s->q_tokens <= (INT32_MAX - 257) / (s->q_heads / s->kv_heads);
 }
 size_t workspace_of(const dcn_attention_shape* s, const dcn_pages* pages, const dcn::PagesAttention& p) {
     return matrix_call(s, pages) ? dcn::attention_pages_workspace(*s, pages->bits, p.max_prefix)

@@ -139,3 +139,17 @@ def test_launches_of_less_than_2_24_workgroups(ask):
             for heads, queries, fits in ((50000, 120, 1), (65535, 127, 1)):  # rows to join: up to 2^23
                 got = plan(ask, dim, bits, heads, heads, [queries] * 2, [50], 100, 1, -1, 0, 2 * queries)
                 assert got.shared and got.fits == fits and got.parts > 1, (dim, bits, heads, vars(got))
+
+
+@pytest.mark.parametrize("pages,page_tokens,heads", [(LAST, 2**30, 8), (LAST, 64, 8), (2**20, 512, 8), (LAST // (8 * 16) + 1, 16, 8)])
+def test_pools_of_more_rows_than_an_int_counts(pages, page_tokens, heads):
+    """They take the kernel of any type, whose rows have 64 bits: the workspace is for its parts. (2^31 - 1 pages
+    of 2^30 tokens of 8 heads are more than 64 bits count.)"""
+    def size(**sizes):
+        s = fa._ATTENTION.pack(1, 1, heads, heads, sizes.get("dim", 64), 1, -1, 0, 0, 1, 2000, 1.0, 1, 0, *[0] * 16)
+        p = fa._PAGES.pack(sizes.get("pages", pages), sizes.get("page_tokens", page_tokens), 2**20 if page_tokens < 1024 else 1, heads,
+                           sizes.get("dim", 64), 1, 8, 0, 0, 0, 0, 0)
+        return _lib.load().dcn_attention_pages_workspace_bytes(s, p, None)
+    line = lambda dim: (dim + 4) * 4 * heads  # noqa: E731
+    assert size(pages=4, page_tokens=64) == 0  # the matrix kernels: one workgroup a head
+    assert size() == size(dim=96) // line(96) * line(64) > 0
