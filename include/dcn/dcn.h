@@ -849,7 +849,8 @@ typedef struct dcn_pages {
     void* v_scales;
 } dcn_pages;
 /* dcn_cache_append_dev into a microscaled cache. Keys are quantised from their rotation in
- * FP32, without a rounding to the dtype in between. q_out must not overlap q. */
+ * FP32, without a rounding to the dtype in between. q_out must not overlap q, k or v: such a call is refused, and
+ * one in which it lies among their rows with strides other than theirs. */
 dcn_status dcn_cache_append_mx_dev(dcn_context* ctx, const dcn_pages* pages, const dcn_append_shape* shape,
                                    const dcn_rotary* rotary, const void* d_q, const void* d_k, const void* d_v,
                                    const int32_t* d_positions, const float* d_freq, const int32_t* d_cu_q,

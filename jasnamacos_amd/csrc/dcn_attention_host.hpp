@@ -68,6 +68,29 @@ inline dcn_status check_out_strides(dcn_context* ctx, const char* name, const in
     return DCN_OK;
 }
 
+// Whether an output's rows lie on an input's ([tokens][heads][dim] each, on their element size): exact where both have
+// the same strides; among rows of other strides they are taken to.
+inline bool rows_meet(const void* in, const int64_t* in_s, int in_heads, const void* out, const int64_t* out_s, int out_heads, int64_t tokens,
+                      int dim, int size) {
+    typedef __int128 wide;  // a stride has 40 bits, a count 31
+    const auto last = [&](const int64_t* s, int heads) { return (wide)(tokens - 1) * s[0] + (wide)(heads - 1) * s[1] + dim; };
+    const wide apart = ((wide)(uintptr_t)out - (wide)(uintptr_t)in) / size;
+    if (apart >= last(in_s, in_heads) || -apart >= last(out_s, out_heads)) return false;
+    if ((tokens > 1 && in_s[0] != out_s[0]) || ((in_heads > 1 || out_heads > 1) && in_s[1] != out_s[1])) return true;
+    // Row i, head h of the output is at apart + (i - j) ts + (h - g) hs from row j, head g of the input.
+    const wide ts = tokens > 1 ? in_s[0] : 0;
+    for (int64_t heads = 1 - (int64_t)in_heads; heads < out_heads; ++heads) {
+        const wide from = apart + heads * (wide)in_s[1];
+        wide rows = ts ? -from / ts : 0;  // the nearest are this one and its neighbours
+        rows = rows > tokens - 1 ? tokens - 1 : (rows < 1 - tokens ? 1 - tokens : rows);
+        for (wide r = rows - 1; r <= rows + 1; ++r) {
+            const wide at = from + r * ts;
+            if (r > -tokens && r < tokens && at < dim && -at < dim) return true;
+        }
+    }
+    return false;
+}
+
 inline dcn_status check_rotary(dcn_context* ctx, const dcn_rotary* r, dcn::RotaryArgs* out) {
     REQUIRE_SHAPE(known_dtype(r->dtype), "rotary dtype " + std::to_string(r->dtype) + " is unknown");
     REQUIRE_SHAPE(r->head_dim >= 1 && r->head_dim <= 65536, "rotary head_dim must be 1..65536");

@@ -94,6 +94,13 @@ dcn_status dcn_cache_append_mx_dev(dcn_context* ctx, const dcn_pages* pages, con
         if (!shape->tokens || !shape->sequences) return DCN_OK;
         DCN_TRY(check_append_pointers(ctx, cache, shape, r, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out));
         if (d_q && d_q == d_q_out) return fail(ctx, DCN_INVALID_ARGUMENT, "q_out is q: an append of this kind does not turn in place");
+        // Workgroups read rows that others may have written by then.
+        const auto meets = [&](const void* in, const int64_t* strides, int heads) {
+            return rows_meet(in, strides, heads, d_q_out, shape->q_out_stride, shape->q_heads, shape->tokens, r.dim, size_of(cache->dtype));
+        };
+        if (d_q && (meets(d_q, shape->q_stride, shape->q_heads) || meets(d_k, shape->k_stride, cache->kv_heads) ||
+                    meets(d_v, shape->v_stride, cache->kv_heads)))
+            return fail(ctx, DCN_INVALID_ARGUMENT, "q_out lies on q, k or v, or among their rows with other strides");
         DCN_TRY(check_buffers(ctx, pages));
         fill_append(&a, &r, cache, shape, d_q, d_k, d_v, d_positions, d_freq, d_cu_q, d_kv_lens, d_table, d_q_out);
         DCN_HIP(ctx, dcn::launch_append_mx(cache->dtype, a, mx, r, (hipStream_t)stream));

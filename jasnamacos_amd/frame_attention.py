@@ -241,7 +241,7 @@ class CacheAppend(_Handle):
 
     def run_mx_dev(self, k, v, pages: "MxPages", table, cu_q, kv_lens, rotary: Rotary | None = None, positions=None, freq=None,
                    q=None, q_out=None, stream=None) -> None:
-        """run_dev into a microscaled cache (dcn_cache_append_mx_dev)."""
+        """run_dev into a microscaled cache (dcn_cache_append_mx_dev); q_out lies on none of q, k and v."""
         if k is None:
             raise DeformConvError(INVALID_ARGUMENT, "k is missing")
         cache = _mx(pages)._pack(table, k.dtype, self.ctx.device)

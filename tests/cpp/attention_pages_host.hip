@@ -5,9 +5,12 @@
 //   plan DIM BITS SEQUENCES KV_HEADS GROUP Q_TOKENS MAX_Q MAX_KV MAX_PREFIX FRAME BACK SINKS
 //                                            shared both parts; rows waves blocks splits of own; of the prefix;
 //                                            workgroups of the prefix, own; whether the launches fit
+//   meet IN_AT TS HS HEADS OUT_AT TS HS HEADS TOKENS DIM SIZE
+//                                            whether rows of an output lie on those of an input (places in bytes)
 #include <cstdio>
 #include <cstring>
 
+#include "dcn_attention_host.hpp"
 #include "dcn_attention_pages.hpp"
 #include "dcn_attention_plan.hpp"
 
@@ -40,6 +43,9 @@ int main() {
             std::printf("%d %d %d %d %d %d %d %d %d %d %d %u %u %d\n", p.shared, p.both, p.parts, p.own.rows, p.own.waves, p.own.blocks, p.own.splits,
                         p.prefix.rows, p.prefix.waves, p.prefix.blocks, p.prefix.splits, prefix.grid, own.grid,
                         grids && fa::launches_fit(p, prefix.grid, own.grid, x[6] * x[3] * x[4]));
+        } else if (!std::strcmp(what, "meet") && read(11)) {
+            const int64_t in[2] = {x[1], x[2]}, out[2] = {x[5], x[6]};
+            std::printf("%d\n", host::rows_meet((const void*)x[0], in, (int)x[3], (const void*)x[4], out, (int)x[7], x[8], (int)x[9], (int)x[10]));
         } else {
             return 2;
         }

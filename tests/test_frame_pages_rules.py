@@ -153,3 +153,33 @@ def test_pools_of_more_rows_than_an_int_counts(pages, page_tokens, heads):
     line = lambda dim: (dim + 4) * 4 * heads  # noqa: E731
     assert size(pages=4, page_tokens=64) == 0  # the matrix kernels: one workgroup a head
     assert size() == size(dim=96) // line(96) * line(64) > 0
+
+
+def test_rows_that_lie_on_others(ask):
+    """Against the places themselves, for tensors that lie in memory in many ways."""
+    r = random.Random(2)
+    questions, want = [], []
+    for _ in range(4000):
+        tokens, dim, size = r.randint(1, 6), r.choice([1, 2, 4]), r.choice([2, 4])
+        in_heads, out_heads = r.randint(1, 5), r.randint(1, 5)
+        hs = dim + r.choice([0, 0, 1, 5])
+        ts = r.choice([1, 2, 3]) * (max(in_heads, out_heads) * hs + r.choice([0, 1]))
+        if r.random() < 0.3:  # heads first
+            hs, ts = tokens * dim + r.choice([0, 2]), dim
+        in_s = (0 if r.random() < 0.1 else ts, 0 if r.random() < 0.1 else hs)
+        apart = r.randint(-3 * ts * tokens, 3 * ts * tokens) if r.random() < 0.5 else r.choice([-1, 1]) * r.choice([0, hs, in_heads * hs, out_heads * hs])
+        places = lambda at, s, heads: {at + i * s[0] + h * s[1] + c for i in range(tokens) for h in range(heads) for c in range(dim)}  # noqa: E731
+        meets = bool(places(0, in_s, in_heads) & places(apart, (ts, hs), out_heads))
+        same = (tokens == 1 or in_s[0] == ts) and (in_heads == out_heads == 1 or in_s[1] == hs)
+        if not same and not meets:
+            continue  # other strides: rows in between may count as met
+        questions.append(f"meet {1 << 20} {in_s[0]} {in_s[1]} {in_heads} {(1 << 20) + apart * size} {ts} {hs} {out_heads} {tokens} {dim} {size}")
+        want.append([int(meets)])
+    assert 500 < sum(w[0] for w in want) < len(want) - 500
+    for question, w, got in zip(questions, want, ask(questions)):
+        assert got == w, question
+    # Sizes that a product of 64 bits does not hold, and tensors apart of other strides.
+    big, far = 2**40 - 1, 1 << 46
+    assert ask([f"meet 64 {big} 64 1 {64 + 2**33} {big} 64 1 {LAST} 64 2", f"meet 64 {big} 64 1 {64 + 2 * big * 1000} {big} 64 1 {LAST} 64 2",
+                f"meet 64 1536 64 8 {far} 512 64 8 100000 64 2", f"meet {far} 512 64 8 64 1536 64 8 100000 64 2",
+                f"meet 64 1536 64 8 {64 + 2 * 1024} 512 64 8 100000 64 2"]) == [[0], [1], [0], [0], [1]]
