@@ -838,7 +838,8 @@ dcn_status dcn_attention_backward_dev(dcn_context* ctx, const dcn_attention_shap
  *
  * dcn_pages: a cache with the buffers it lies in. cache.dtype is that of the tensors
  * outside; bits 8 or 4: microscaled; 0: pages of that dtype as dcn_cache has them (the scales are
- * then ignored), which only dcn_attention_pages_dev takes, with a prefix. */
+ * then ignored), which only dcn_attention_pages_dev takes, with a prefix. Codes are aligned to 16
+ * bytes, scales to 4. */
 typedef struct dcn_pages {
     dcn_cache cache;
     int32_t bits;

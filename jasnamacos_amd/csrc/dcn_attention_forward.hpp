@@ -12,6 +12,9 @@ namespace {
 template <typename T>
 constexpr float kLift = __is_same(T, _Float16) ? 6.f : 0.f;
 constexpr float kSlack = 8.f;
+// Weights are rounded to T for the product with the values, half a step each (BF16 2^-8 of a weight, FP16 2^-11):
+// FP32 products have a sixteenth of the 16-bit ones' rate. Their sum is of the unrounded ones. The outputs are
+// 1.2 to 1.45 times as far from 64 bits as with FP32 weights, most of it being their own rounding.
 
 // One wave's 32 rows: queries, sums and the running maximum.
 template <typename T, int D>

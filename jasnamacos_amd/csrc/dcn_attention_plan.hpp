@@ -20,7 +20,7 @@ struct PlanOf {
 
 // Whether more than 32 rows take 32-row workgroups, whose waves share the keys out, and not 128-row ones.
 // The small ones fill the card where there are few (wide: 128-row workgroups) and read the keys four times
-// as often. Measured (us, 128 rows -> 32; 8 query heads on 4):
+// as often. Measured (us, 128 rows -> 32; 8 query heads on 4 throughout, other groups were not tried):
 //   64 channels, 8 bits: wide 32 at 3,000 keys 29 -> 24; 128 at 12,000 104 -> 94; 256 at 12,000 198 -> 159;
 //     456 at 4,000 100 -> 72 and at 12,000 310 -> 305; 464 at 14,400 344 -> 365; 928 at 4,000 154 -> 135;
 //     2,048 at 12,000 914 -> 924. 4 bits: 256 at 16,000 252 -> 199.
@@ -40,8 +40,10 @@ inline bool few_of(int dim, int bits, int64_t wide, int64_t keys) {
 // until about 512 are there (two a CU): one token of 32 streams on 18,001 keys of 8 bits, 32 heads of 128
 // on 8, in one part 217 us, in two 156, in six 170. Tiles of 128 rows write long parts, so only whole
 // shares are taken: a frame of 3,600 tokens for two streams, 464 workgroups, 340 us in one part and 470 in
-// two. Up to 64 tiles for single tokens go to one workgroup of many waves: a join costs more (997 keys,
-// 8 heads of 64: 10.6 us, in parts 12.7).
+// two. Up to four tiles of 32 keys a wave go to one workgroup of many waves for single tokens: a join costs more.
+// That is 64 tiles at 64 channels (16 waves; 997 keys, 8 heads: 10.6 us, in parts 12.7) and 32 at 128 (8 waves;
+// 8 heads on 8 bits, in one workgroup and in parts: 1,280 keys 13.3 and 13.6, 1,500 keys 16.2 and 13.4, 2,040 keys
+// 19.0 and 13.0).
 inline Blocks blocks_of(int dim, int64_t rows, int64_t pairs, int64_t keys, int64_t resident, bool few) {
     Blocks b;
     b.rows = rows <= 16 ? 16 : (few ? 32 : 128);

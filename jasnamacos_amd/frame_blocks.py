@@ -226,7 +226,8 @@ class FrameStream:
     def fork(self, copies: int, of: int = 0) -> "FrameStream":
         """Streams that each continue stream `of` of these in their own way, from its next frame on. What is
         kept of its frames is copied once for all of them, on the current stream, as it is now. Of a stream
-        that was not forked itself."""
+        that was not forked itself. A step is a whole frame: its rows fill blocks of their own, each of which reads
+        the shared frames (calls of few tokens read a long prefix once for all streams)."""
         if self.prefix is not None:
             raise ValueError("these streams continue another one: fork that one instead")
         if not self.time:
