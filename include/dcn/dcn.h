@@ -883,9 +883,10 @@ typedef struct dcn_prefix {
  * the sequences share a prefix (null: none). With a prefix of P tokens, sequence s's keys are the
  * prefix's and then its own kv_lens[s], of which its table speaks: query i of nq is token
  * P + kv_lens[s] - nq + i, and frames, the window and sinks count from the prefix's first token.
- * shape.max_kv bounds kv_lens; lengths past the table's width count as its tokens, below zero as none. Where sequences of few queries would read much of the prefix again, its keys
- * are read once for all of them (heads of 64 and 128 channels in 16 bits) and the results
- * joined in FP32. (width + table_width) * page_tokens must be below 2^31 - 63. A launch has a workgroup for each
+ * shape.max_kv bounds kv_lens; lengths past the table's width count as its tokens, below zero as
+ * none. Where sequences of few queries would read much of the prefix again, its keys are read
+ * once for all of them (heads of 64 and 128 channels in 16 bits) and the results joined in FP32.
+ * (width + table_width) * page_tokens must be below 2^31 - 63. A launch has a workgroup for each
  * 16 to 128 rows, below 2^24 in all as above. */
 size_t dcn_attention_pages_workspace_bytes(const dcn_attention_shape* shape, const dcn_pages* pages,
                                            const dcn_prefix* prefix);
